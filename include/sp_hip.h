@@ -23,6 +23,7 @@ extern "C" {
 
 #define SP_DTYPE_F32 0
 #define SP_DTYPE_F16 1
+#define SP_DTYPE_BF16 2   /* the 8-bit block cache's calls only */
 
 /* ======================================================================== */
 /* Ship cache  (sp_cuda_cache_t, shannon_prime_cuda.h:29-46)                */
@@ -435,6 +436,89 @@ int  sp_hip_hier_attn_decode(const sp_hip_hier_cache_t *hc, int layer, int n_kv,
 int  sp_hip_hier_attn_decode_seqs(const sp_hip_hier_cache_t *hc, int layer, int n_seq, const int *seq_start,
                                   const int *seq_len, const float *d_q, int n_q, float kq_scale, float *d_scores,
                                   float *d_out, void *stream);
+
+/* ======================================================================== */
+/* 8-bit block cache                                                        */
+/* ======================================================================== */
+/* Keys and values as OCP E4M3 numbers in blocks of 64 positions, with one power of
+ * two as the scale of each block and KV head (K and V apart): 1 byte per element, for
+ * layers or models where the spectral caches' 3 to 5 bits are too few, and for prompts,
+ * which the other caches do not attend over. The reference names fp8 kernels
+ * (shannon_prime_fp8.cu, llama-cpp-b8861-full-engine.patch:243) without their source.
+ *
+ * The cache is a pool of n_blocks blocks per layer. A sequence is a row of block numbers,
+ * the same for every layer: positions [64 j, 64 j + 64) are in block d_table[i][j]. Which
+ * block is whose is the caller's affair; sequences may share blocks that no call writes. */
+#define SP_FP8_BLOCK 64
+
+typedef struct {
+    sp_config_t config;    /* head_dim (64, 96, 128 or 256), n_layers, n_heads_kv are used */
+    int         n_blocks;
+    void       *d_k_codes; /* [n_layers][n_blocks][n_heads_kv][64 * head_dim] E4M3, in the kernels' order */
+    void       *d_v_codes;
+    void       *d_k_exp;   /* [n_layers][n_blocks][n_heads_kv] bytes b: scale 2^(b - 127) */
+    void       *d_v_exp;
+    void       *stream;
+    void       *priv;      /* device, attention workspace */
+} sp_hip_fp8_cache_t;
+
+/* The sequences of a call. All arrays are on the device and are read when the launch runs,
+ * so a captured call follows what they hold at each replay.
+ *
+ * Row r of sequence i (d_row[i] <= r < d_row[i + 1]) is its position
+ * d_len[i] - d_row[i + 1] + r: the call's rows are the sequence's newest positions, and
+ * d_len counts them. d_row ascends and d_row[n_seq] <= n_rows; rows that no sequence has are
+ * neither read nor written. Without d_row sequence i has the one row i (n_rows = n_seq).
+ *
+ * A position is in the cache if it is not negative and its table entry exists and lies in
+ * [0, n_blocks). Others (a length past the table, an entry of -1) are never accessed: write
+ * passes over them, read gives zeros, attention leaves them out. */
+typedef struct {
+    int            n_seq;
+    int            table_stride;  /* entries of a table row */
+    const int32_t *d_table;       /* [n_seq][table_stride] */
+    const int32_t *d_len;         /* [n_seq] */
+    const int32_t *d_row;         /* [n_seq + 1] or NULL */
+    int            n_rows;        /* rows of the call's tensors */
+} sp_hip_fp8_batch_t;
+
+/* 0 or -1 (sp_hip_last_error). The memory is cleared: a fresh block holds zeros. */
+int  sp_hip_fp8_cache_init(sp_hip_fp8_cache_t *c, const sp_config_t *cfg, int n_blocks, void *stream);
+void sp_hip_fp8_cache_free(sp_hip_fp8_cache_t *c);
+
+/* Quantise the batch's rows into their blocks, K and V of every head in one launch: element
+ * (r, h, d) at r*row_stride + h*head_dim + d, row_stride >= n_heads_kv*head_dim, dtype F32,
+ * F16 or BF16; NULL d_k or d_v skips that side.
+ * scale = 2^e with the least e in [-40, 40] that puts the block's largest magnitude at most
+ * at 448 * 2^e, code = E4M3 of x / scale rounded to nearest even. A block that holds older
+ * positions of its sequence (the rows start inside it) takes max(e, its old e), and if that
+ * is larger its older codes are rounded again at the new scale; rows that start at a block's
+ * first position begin it anew. NaN is stored as 0 and magnitudes past 448 * 2^40, infinity
+ * among them, as that: what a cache holds is finite, so no position that a mask hides can
+ * reach a result. Two sequences of one call must not write the same block (the result of
+ * such a block is unspecified). */
+int  sp_hip_fp8_write(sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *batch, const void *d_k,
+                      const void *d_v, long long row_stride, int dtype, void *stream);
+/* The batch's rows read back: code * scale, rounded to dtype. */
+int  sp_hip_fp8_read(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *batch, void *d_k, void *d_v,
+                     long long row_stride, int dtype, void *stream);
+
+/* Attention of the batch's rows over their sequences, causal: the query at position p sees
+ * the positions t <= p, and with window > 0 only t > p - window. Row r, head n at
+ * r*q_stride + n*head_dim in d_q and r*out_stride + n*head_dim in d_out, both of `dtype`;
+ * query head n reads KV head n / (n_q / n_heads_kv), any number per KV head.
+ *   d_out = softmax(kq_scale * q . K) V      d_lse [n_rows][n_q] fp32 (may be NULL): the log
+ * of the sum of exp(kq_scale * q . K). A row that sees nothing gets zeros and -infinity.
+ * The call's own positions are read from the cache: write them first. decode takes one row
+ * per sequence (d_row NULL), prefill any number.
+ * The workspace belongs to the cache and is allocated by init: two attention calls on one
+ * cache may not overlap. Results do not depend on which block of threads finishes first. */
+int  sp_hip_fp8_attn_decode(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *batch, const void *d_q,
+                            long long q_stride, int n_q, int dtype, float kq_scale, int window, void *d_out,
+                            long long out_stride, float *d_lse, void *stream);
+int  sp_hip_fp8_attn_prefill(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *batch, const void *d_q,
+                             long long q_stride, int n_q, int dtype, float kq_scale, int window, void *d_out,
+                             long long out_stride, float *d_lse, void *stream);
 
 /* ======================================================================== */
 /* System 1/2 dual cache (DualKvCache, kv_cache.h:238-310,                  */

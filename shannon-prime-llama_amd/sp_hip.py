@@ -14,6 +14,8 @@ INCLUDE_DIR = os.path.join(os.path.dirname(HERE), "include")
 SP_MAX_BANDS = 16
 DTYPE_F32 = 0
 DTYPE_F16 = 1
+DTYPE_BF16 = 2  # the 8-bit block cache's calls
+FP8_BLOCK = 64
 NORM_FINAL = 0
 NORM_STAGE = 1
 
@@ -89,6 +91,16 @@ class SpHipDualCache(C.Structure):
 
 
 DUAL_SQFREE, DUAL_HIER = 1, 2
+
+
+class SpHipFp8Cache(C.Structure):
+    _fields_ = [("config", SpConfig), ("n_blocks", C.c_int), ("d_k_codes", C.c_void_p), ("d_v_codes", C.c_void_p),
+                ("d_k_exp", C.c_void_p), ("d_v_exp", C.c_void_p), ("stream", C.c_void_p), ("priv", C.c_void_p)]
+
+
+class SpHipFp8Batch(C.Structure):
+    _fields_ = [("n_seq", C.c_int), ("table_stride", C.c_int), ("d_table", C.c_void_p), ("d_len", C.c_void_p),
+                ("d_row", C.c_void_p), ("n_rows", C.c_int)]
 
 
 class SpHipColdLayer(C.Structure):
@@ -237,6 +249,12 @@ def lib():
         L.sp_hip_sqfree_attn_decode.argtypes = [vp, i, i, vp, i, f, vp, vp, vp]
         for name in ("sp_hip_attn_decode_seqs", "sp_hip_sqfree_attn_decode_seqs", "sp_hip_hier_attn_decode_seqs"):
             getattr(L, name).argtypes = [vp, i, i, vp, vp, vp, i, f, vp, vp, vp]
+        L.sp_hip_fp8_cache_init.argtypes = [vp, vp, i, vp]
+        L.sp_hip_fp8_cache_free.argtypes = [vp]
+        for name in ("sp_hip_fp8_write", "sp_hip_fp8_read"):
+            getattr(L, name).argtypes = [vp, i, vp, vp, vp, ll, i, vp]
+        for name in ("sp_hip_fp8_attn_decode", "sp_hip_fp8_attn_prefill"):
+            getattr(L, name).argtypes = [vp, i, vp, vp, ll, i, i, f, i, vp, ll, vp, vp]
         L.sp_hip_vht2_forward.argtypes = [vp, i, i, i, vp]
         L.sp_hip_band_quantize.argtypes = [vp, vp, vp, i, vp]
         L.sp_hip_band_dequantize.argtypes = [vp, vp, vp, i, vp]
@@ -401,6 +419,36 @@ class DualCache:
             self.free()
         except Exception:
             pass
+
+
+class Fp8Cache:
+    """sp_hip_fp8_cache_t owner (8-bit block cache: a pool of n_blocks blocks of 64
+    positions per layer)."""
+
+    def __init__(self, cfg, n_blocks, stream=0):
+        self.c = SpHipFp8Cache()
+        check(lib().sp_hip_fp8_cache_init(C.byref(self.c), C.byref(cfg), n_blocks, C.c_void_p(stream)),
+              "sp_hip_fp8_cache_init")
+        self.ref = C.byref(self.c)
+
+    def free(self):
+        if self.c.priv:
+            lib().sp_hip_fp8_cache_free(self.ref)
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class Fp8Batch:
+    """sp_hip_fp8_batch_t over device arrays of the caller's (addresses; d_row 0: one row
+    per sequence)."""
+
+    def __init__(self, n_seq, table_stride, d_table, d_len, d_row=0, n_rows=None):
+        self.c = SpHipFp8Batch(n_seq, table_stride, d_table, d_len, d_row or None, n_seq if n_rows is None else n_rows)
+        self.ref = C.byref(self.c)
 
 
 def header_symbols():
