@@ -224,9 +224,11 @@ def _inputs(case, seed):
 
 
 class _Memory:
-    """Device memory that a cache owns, as torch can take it without a copy."""
+    """Device memory that a cache owns, as torch can take it without a copy: the tensor holds
+    this object, and this object the cache."""
 
-    def __init__(self, ptr, shape):
+    def __init__(self, cache, ptr, shape):
+        self.cache = cache
         self.__cuda_array_interface__ = dict(shape=tuple(shape), typestr="|u1", data=(int(ptr), False), version=2)
 
 
@@ -238,7 +240,7 @@ def prepare(case, seed):
         s["cache"] = S.Fp8Cache(cfg, s["n_blocks"], torch.cuda.current_stream().cuda_stream)
         c = s["cache"].c
         for name, ptr in (("k", c.d_k_codes), ("k_exp", c.d_k_exp), ("v", c.d_v_codes), ("v_exp", c.d_v_exp)):
-            mine = torch.as_tensor(_Memory(ptr, s[name].shape), device="cuda")
+            mine = torch.as_tensor(_Memory(s["cache"], ptr, s[name].shape), device="cuda")
             mine.copy_(s[name])
             s[name] = mine
         s["batch"] = S.Fp8Batch(case["seqs"], s["table"].shape[1], s["table"].data_ptr(), s["d_len"].data_ptr(),
