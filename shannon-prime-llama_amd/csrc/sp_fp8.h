@@ -61,7 +61,7 @@ struct SpFp8Attn {
     int negate;
     float *part;    // partial results, SP_FP8_SLOTS slots of 32 rows of hd + 2 floats
     int *counters;  // one per slot, zero between calls
-    int target;     // blocks that fill the chip
+    int target;     // CUs; the launch makes it the blocks that fill them
 };
 
 hipError_t sp_fp8_launch_write(const SpFp8Copy &A, int hd, int dtype, hipStream_t s);
@@ -69,7 +69,7 @@ hipError_t sp_fp8_launch_read(const SpFp8Copy &A, int hd, int dtype, hipStream_t
 hipError_t sp_fp8_launch_attn(const SpFp8Attn &A, int hd, int dtype, hipStream_t s);
 size_t sp_fp8_workspace_floats(int hd);
 
-#define SP_FP8_SLOTS 2048
+#define SP_FP8_SLOTS 1024
 
 __device__ __forceinline__ int sp_fp8_floor64(int x) { return x >> 6; }  // arithmetic: toward -inf
 

@@ -51,9 +51,10 @@ __device__ __forceinline__ float column_sum(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
-__device__ __forceinline__ long long wave_sum(long long v) {
+template <class T, class Op>
+__device__ __forceinline__ T wave_all(T v, Op op) {
 #pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
+    for (int d = 32; d; d >>= 1) v = op(v, __shfl_xor(v, d, 64));
     return v;
 }
 
@@ -65,50 +66,84 @@ struct Share {
     int slot;  // of the partial result, in units of KV heads; group's first: slot - split
 };
 
-// The work is divided on the device, so that lengths may change under a captured call: with T
-// the blocks that all column groups see and R = T / target, a column group of n blocks gets
-// ceil(n / R) shares. Groups of two or more shares number at most 2 * target shares in all
-// (n > R gives ceil(n / R) < 2 n / R), which bounds the partial results.
-__device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lane, int cols, Share &out) {
-    const SpFp8Seqs &S = A.s;
-    long long total = 0, rows = 0;
-    for (int i0 = 0; i0 < S.n_seq; i0 += 64) {
-        const int i = i0 + lane;
-        if (i < S.n_seq) {
-            int a, b, len;
-            sp_fp8_seq(S, i, a, b, len);
-            const int lo = A.window > 0 ? max(len - (b - a) - A.window + 1, 0) >> 6 : 0;
-            const int nb = max(min((len + 63) >> 6, S.stride) - lo, 0);
-            const long long ct = ((long long)(b - a) * A.G + cols - 1) / cols;
-            total += ct * nb;
-            rows += b - a;
-        }
+// A sequence's rows, length, column groups and the cache blocks that its rows see.
+struct Extent {
+    int a, b, len, ct, nb;
+};
+__device__ __forceinline__ Extent extent(const SpFp8Attn &A, int i, int cols) {
+    Extent e{0, 0, 0, 0, 0};
+    if (i < A.s.n_seq) {
+        sp_fp8_seq(A.s, i, e.a, e.b, e.len);
+        const int lo = A.window > 0 ? max(e.len - (e.b - e.a) - A.window + 1, 0) >> 6 : 0;
+        e.nb = max(min((e.len + 63) >> 6, A.s.stride) - lo, 0);
+        e.ct = (int)(((long long)(e.b - e.a) * A.G + cols - 1) / cols);
     }
-    total = wave_sum(total) * A.H;
-    if (wave_sum(rows) > S.n_rows) return false;  // the array of rows is not ascending
-    const int R = (int)max((total + A.target - 1) / A.target, 1ll);
-    int slots = 0;
-    for (int i0 = 0; i0 < S.n_seq; i0 += 64) {
-        const int i = i0 + lane;
-        int a = 0, b = 0, len = 0, ct = 0, ns = 1;
-        if (i < S.n_seq) {
-            sp_fp8_seq(S, i, a, b, len);
-            const int lo = A.window > 0 ? max(len - (b - a) - A.window + 1, 0) >> 6 : 0;
-            const int nb = max(min((len + 63) >> 6, S.stride) - lo, 0);
-            ct = (int)(((long long)(b - a) * A.G + cols - 1) / cols);
-            ns = max((nb + R - 1) / R, 1);
+    return e;
+}
+__device__ __forceinline__ int shares_of(int nb, int R, int least) {
+    return nb <= 2 * least ? 1 : (nb + R - 1) / R;
+}
+
+// The work is divided on the device, so that lengths may change under a captured call. With T
+// the blocks that all column groups see, a column group of n blocks gets ceil(n / R) shares,
+// R the first of R0, 5/4 R0, 3/2 R0 and 2 R0, R0 > T / target, that makes at most `target`
+// shares, if one does. R is at least `least`, one block a wave, and two blocks a wave are not
+// shared out: a share's own waves join their results in LDS, which costs far less than the
+// stores, the count and the loads (three memory latencies) that join shares. Groups of two or more shares (n > R, so
+// ceil(n / R) < 2 n / R) have at most 2 T / R < 2 target shares, which bounds the partial
+// results.
+__device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lane, int cols, int least, Share &out) {
+    const int n_seq = A.s.n_seq;
+    const auto fadd = [](float x, float y) { return x + y; };
+    const auto sat = [](unsigned x, unsigned y) { return min(x + y, 0x7fffffffu); };  // each at most 2^31 - 1
+    if (n_seq == 1) {  // nothing to search, and no exchange between lanes
+        const Extent e = extent(A, 0, cols);
+        const float T = (float)e.ct * (float)e.nb * (float)A.H;
+        const int R0 = max((int)(T / (float)A.target * 1.002f) + 1, least);
+        int R = 2 * R0;
+        for (int k = 2; k >= 0; k--) {
+            const int r = R0 + k * R0 / 4;
+            if ((float)shares_of(e.nb, r, least) * (float)e.ct * (float)A.H <= (float)A.target) R = r;
         }
-        const int n = ct * ns, sum = sp_fp8_scan(n, lane);
-        const int part = ns > 1 ? n : 0, psum = sp_fp8_scan(part, lane);
+        const int ns = shares_of(e.nb, R, least);
+        out = Share{0, e.a, e.b - e.a, e.len - (e.b - e.a), item / ns, item % ns, ns, item};
+        return item < e.ct * ns;
+    }
+    const Extent e0 = extent(A, lane, cols);  // kept: up to 64 sequences are read once
+    float T = (float)e0.ct * (float)e0.nb;
+    unsigned rows = (unsigned)(e0.b - e0.a);
+    for (int i0 = 64; i0 < n_seq; i0 += 64) {
+        const Extent e = extent(A, i0 + lane, cols);
+        T += (float)e.ct * (float)e.nb;
+        rows = sat(rows, (unsigned)(e.b - e.a));
+    }
+    T = wave_all(T, fadd) * (float)A.H;
+    if (A.s.row && wave_all(rows, sat) > (unsigned)A.s.n_rows) return false;  // d_row does not ascend
+    const int R0 = max((int)(T / (float)A.target * 1.002f) + 1, least);
+    float n[3] = {0.0f, 0.0f, 0.0f};
+    for (int i0 = 0; i0 < n_seq; i0 += 64) {
+        const Extent e = i0 ? extent(A, i0 + lane, cols) : e0;
+#pragma unroll
+        for (int k = 0; k < 3; k++) n[k] += (float)e.ct * (float)shares_of(e.nb, R0 + k * R0 / 4, least);
+    }
+    int R = 2 * R0;
+#pragma unroll
+    for (int k = 2; k >= 0; k--)
+        if (wave_all(n[k], fadd) * (float)A.H <= (float)A.target) R = R0 + k * R0 / 4;
+    int slots = 0;
+    for (int i0 = 0; i0 < n_seq; i0 += 64) {
+        const Extent e = i0 ? extent(A, i0 + lane, cols) : e0;
+        const int ns = shares_of(e.nb, R, least), mine = e.ct * ns, sum = sp_fp8_scan(mine, lane);
+        const int part = ns > 1 ? mine : 0, psum = sp_fp8_scan(part, lane);
         const unsigned long long past = __ballot(sum > item);
         if (past) {
             const int l = __ffsll(past) - 1;
             out.seq = i0 + l;
-            out.r0 = __shfl(a, l, 64);
-            out.n_new = __shfl(b, l, 64) - out.r0;
-            out.first = __shfl(len, l, 64) - out.n_new;
+            out.r0 = __shfl(e.a, l, 64);
+            out.n_new = __shfl(e.b, l, 64) - out.r0;
+            out.first = __shfl(e.len, l, 64) - out.n_new;
             out.n_split = __shfl(ns, l, 64);
-            const int at = item - (__shfl(sum, l, 64) - __shfl(n, l, 64));
+            const int at = item - (__shfl(sum, l, 64) - __shfl(mine, l, 64));
             out.ct = at / out.n_split;
             out.split = at - out.ct * out.n_split;
             out.slot = slots + __shfl(psum, l, 64) - __shfl(part, l, 64) + at;
@@ -168,9 +203,22 @@ __device__ __forceinline__ void finish(const SpFp8Attn &A, long long row, int he
         A.lse[row * A.H * A.G + head] = l == 0.0f ? -INFINITY : (m - P_TOP + __log2f(l)) * 0.69314718055994531f;
 }
 
-template <int HD, int DT, int NW>
+// Joins partial results (m, l, o pair) in order.
+struct Acc {
+    float M = -INFINITY, L = 0.0f, x = 0.0f, y = 0.0f;
+    __device__ __forceinline__ void add(float m, float l, float px, float py) {
+        const float Mn = fmaxf(M, m), f0 = weight(M, Mn), f = weight(m, Mn);
+        L = L * f0 + l * f;
+        x = x * f0 + px * f;
+        y = y * f0 + py * f;
+        M = Mn;
+    }
+};
+
+// CG groups of 16 columns share each block's loads and conversions.
+template <int HD, int DT, int NW, int CG>
 __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
-    constexpr int COLS = 16, NC = HD / 32, ND = HD / 16, TILE = 64 * HD, ROW = HD + 2;
+    constexpr int COLS = 16 * CG, NC = HD / 32, ND = HD / 16, TILE = 64 * HD, ROW = HD + 2, NT = NW * 64;
     constexpr bool SPLIT2 = DT == SP_DTYPE_F32;
     constexpr int NH = SPLIT2 ? 2 : 1;
     typedef typename SpFp8Elem<DT>::T T;
@@ -179,8 +227,8 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.H;
     Share sh;
-    if (!find_share(A, blockIdx.x / A.H, lane, COLS, sh)) return;
-    const int n_cols = min((int)min((long long)sh.n_new * A.G - (long long)sh.ct * COLS, (long long)COLS), COLS);
+    if (!find_share(A, blockIdx.x / A.H, lane, COLS, NW, sh)) return;
+    const int n_cols = (int)min((long long)sh.n_new * A.G - (long long)sh.ct * COLS, (long long)COLS);
     const int col = lane & 15, g = lane >> 4;
     const long long c0 = (long long)sh.ct * COLS;
     const int tk0 = (int)(c0 / A.G), tk1 = (int)((c0 + n_cols - 1) / A.G);
@@ -191,80 +239,103 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
     const int per = max((j1 - j0 + sh.n_split - 1) / sh.n_split, 0);
     const int t0 = j0 + sh.split * per, t1 = min(t0 + per, j1);
 
+    // ---- this wave's blocks: t0 + w, t0 + w + NW, ... ----
+    // The chain of loads is length, table, codes: the table's and the first codes' loads are
+    // issued before anything waits for the queries or the scales.
+    const int mine = t1 > t0 + w ? (t1 - t0 - w + NW - 1) / NW : 0;
+    int blk = -1, ekb = 0, evb = 0;  // lane k: block number and scale bytes of the k-th block
+    const auto look_up = [&](int base) {
+        blk = base + lane < mine ? sp_fp8_block(A.s, sh.seq, t0 + w + NW * (base + lane)) : -1;
+    };
+    u4 kr[2 * NC], vr[ND];
+    const auto load_k = [&](int k) {
+        const int b = max(__builtin_amdgcn_readlane(blk, k), 0);  // none: read block 0, all masked
+        const uint8_t *p = A.k.codes + ((long long)b * A.H + h) * TILE + lane * 16;
+#pragma unroll
+        for (int n = 0; n < 2 * NC; n++) kr[n] = *reinterpret_cast<const u4 *>(p + n * 1024);
+    };
+    const auto load_v = [&](int k) {
+        const int b = max(__builtin_amdgcn_readlane(blk, k), 0);
+        const uint8_t *p = A.v.codes + ((long long)b * A.H + h) * TILE + lane * 16;
+#pragma unroll
+        for (int n = 0; n < ND; n++) vr[n] = *reinterpret_cast<const u4 *>(p + n * 1024);
+    };
+    const auto start = [&]() {
+        const long long at = (long long)max(blk, 0) * A.H + h;
+        ekb = A.k.exps[at];
+        evb = A.v.exps[at];
+        load_k(0);
+        load_v(0);
+    };
+    if (mine > 0) look_up(0);
+
     // ---- queries ----
-    const bool active = col < n_cols;
-    const long long cn = c0 + (active ? col : 0);
-    const int tk = (int)(cn / A.G), head = h * A.G + (int)(cn % A.G);
-    const int pos = active ? sh.first + tk : -1;
-    const int from = A.window > 0 ? pos - A.window : -1;  // sees (from, pos]
-    h8 q[NC][NH];
-    float cscale;
-    {
-        float x[NC][8], top = 0.0f;
+    bool active[CG];
+    int pos[CG], from[CG];  // sees (from, pos]
+    float x[CG][NC][8];
+#pragma unroll
+    for (int y = 0; y < CG; y++) {
+        active[y] = y * 16 + col < n_cols;
+        const long long cn = c0 + (active[y] ? y * 16 + col : 0);
+        const int tk = (int)(cn / A.G), head = h * A.G + (int)(cn % A.G);
+        pos[y] = active[y] ? sh.first + tk : -1;
+        from[y] = A.window > 0 ? pos[y] - A.window : -1;
         const T *src = reinterpret_cast<const T *>(A.q) + (sh.r0 + tk) * A.q_stride + (long long)head * HD + g * 8;
         const bool aligned = ((uintptr_t)A.q % (4 * sizeof(T))) == 0 && A.q_stride % 4 == 0;
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            load8<DT>(src + c * 32, aligned, x[c]);
+        for (int c = 0; c < NC; c++) load8<DT>(src + c * 32, aligned, x[y][c]);
+    }
+    if (mine > 0) start();
+    h8 q[CG][NC][NH];
+    float cscale[CG];
 #pragma unroll
-            for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[c][k]));
-        }
+    for (int y = 0; y < CG; y++) {
+        float top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[y][c][k]));
         top = column_max(top);
         int e = (__float_as_int(top) >> 23) - 127 - 14;
         e = top == 0.0f || !(top < INFINITY) ? 0 : max(e, -126);
         const float down = A.negate ? -sp_fp8_pow2(-e) : sp_fp8_pow2(-e);
-        cscale = A.c * sp_fp8_pow2(e);
+        cscale[y] = A.c * sp_fp8_pow2(e);
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const float y = active ? x[c][k] * down : 0.0f;
-                const _Float16 hi = (_Float16)y;
-                q[c][0][k] = hi;
-                if (SPLIT2) q[c][NH - 1][k] = (_Float16)(y - (float)hi);
+                const float v = active[y] ? x[y][c][k] * down : 0.0f;
+                const _Float16 hi = (_Float16)v;
+                q[y][c][0][k] = hi;
+                if (SPLIT2) q[y][c][NH - 1][k] = (_Float16)(v - (float)hi);
             }
     }
 
-    // ---- this wave's blocks: t0 + w, t0 + w + NW, ... ----
-    f4 o[ND];
+    f4 o[CG][ND];
+    float m[CG], l[CG];
 #pragma unroll
-    for (int d = 0; d < ND; d++) o[d] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;
+    for (int y = 0; y < CG; y++) {
+        m[y] = -INFINITY;
+        l[y] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[y][d] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     int ev_now = 0;
-    const int mine = t1 > t0 + w ? (t1 - t0 - w + NW - 1) / NW : 0;
     for (int base = 0; base < mine; base += 64) {
         const int count = min(mine - base, 64);
-        // lane k: block number and scales of the k-th block
-        int blk = -1, ek = 0, ev = 0;
-        if (lane < count) {
-            blk = sp_fp8_block(A.s, sh.seq, t0 + w + NW * (base + lane));
-            if (blk >= 0) {
-                ek = sp_fp8_exponent(A.k.exps[(long long)blk * A.H + h]);
-                ev = sp_fp8_exponent(A.v.exps[(long long)blk * A.H + h]);
-            }
+        if (base) {
+            look_up(base);
+            start();
         }
-        u4 kr[2 * NC], vr[ND];
-        const auto load_k = [&](int k) {
-            const int b = max(__builtin_amdgcn_readlane(blk, k), 0);  // none: read block 0, all masked
-            const uint8_t *p = A.k.codes + ((long long)b * A.H + h) * TILE + lane * 16;
-#pragma unroll
-            for (int n = 0; n < 2 * NC; n++) kr[n] = *reinterpret_cast<const u4 *>(p + n * 1024);
-        };
-        const auto load_v = [&](int k) {
-            const int b = max(__builtin_amdgcn_readlane(blk, k), 0);
-            const uint8_t *p = A.v.codes + ((long long)b * A.H + h) * TILE + lane * 16;
-#pragma unroll
-            for (int n = 0; n < ND; n++) vr[n] = *reinterpret_cast<const u4 *>(p + n * 1024);
-        };
-        load_k(0);
-        load_v(0);
         for (int k = 0; k < count; k++) {
             const int t = t0 + w + NW * (base + k);
             const bool none = __builtin_amdgcn_readlane(blk, k) < 0;
-            const float cs = cscale * sp_fp8_pow2(__builtin_amdgcn_readlane(ek, k));
-            f4 s[4];
+            const float kscale = sp_fp8_pow2(sp_fp8_exponent(__builtin_amdgcn_readlane(ekb, k)));
+            f4 s[CG][4];
 #pragma unroll
-            for (int n = 0; n < 4; n++) s[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int y = 0; y < CG; y++)
+#pragma unroll
+                for (int n = 0; n < 4; n++) s[y][n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -272,102 +343,115 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
                     const u4 r = kr[u * NC + c];
                     const h8 a = to_half(r[0], r[1]), b = to_half(r[2], r[3]);
 #pragma unroll
-                    for (int n = 0; n < NH; n++) {
-                        s[2 * u] = mma(a, q[c][n], s[2 * u]);
-                        s[2 * u + 1] = mma(b, q[c][n], s[2 * u + 1]);
-                    }
+                    for (int y = 0; y < CG; y++)
+#pragma unroll
+                        for (int n = 0; n < NH; n++) {
+                            s[y][2 * u] = mma(a, q[y][c][n], s[y][2 * u]);
+                            s[y][2 * u + 1] = mma(b, q[y][c][n], s[y][2 * u + 1]);
+                        }
                 }
             if (k + 1 < count) load_k(k + 1);
             const bool open = !none && t * 64 + 63 <= pos0 && (A.window <= 0 || t * 64 > pos1 - A.window);
-            float top = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < 4; n++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float x = s[n][i] * cs;
-                    if (!open) {
-                        const int at = t * 64 + n * 16 + 4 * g + i;
-                        x = !none && at <= pos && at > from ? x : -INFINITY;
-                    }
-                    s[n][i] = x;
-                    top = fmaxf(top, x);
-                }
-            const float m_new = fmaxf(m, column_max(top));
-            const float ref = m_new == -INFINITY ? 0.0f : m_new - P_TOP;
-            const float alpha = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
-            float sum = 0.0f;
-            h8 p[2][NH];
-#pragma unroll
-            for (int n = 0; n < 4; n++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float x = __builtin_amdgcn_exp2f(s[n][i] - ref);
-                    sum += x;
-                    const _Float16 hi = (_Float16)x;
-                    p[n / 2][0][(n % 2) * 4 + i] = hi;
-                    if (SPLIT2) p[n / 2][NH - 1][(n % 2) * 4 + i] = (_Float16)(x - (float)hi);
-                }
-            l = l * alpha + sum;
-            m = m_new;
-            const int ev_k = __builtin_amdgcn_readlane(ev, k);
-            const float f = alpha * sp_fp8_pow2(ev_now - ev_k);
+            const int ev_k = sp_fp8_exponent(__builtin_amdgcn_readlane(evb, k));
+            const float ev_step = sp_fp8_pow2(ev_now - ev_k);
             ev_now = ev_k;
-            if (__any(f != 1.0f)) {
+            h8 p[CG][2][NH];
 #pragma unroll
-                for (int d = 0; d < ND; d++) o[d] *= f;
+            for (int y = 0; y < CG; y++) {
+                const float cs = cscale[y] * kscale;
+                float top = -INFINITY;
+                // positions of this block that the column sees, counted from the lane's first: (before, upto]
+                const int lane0 = t * 64 + 4 * g, upto = none ? -1 : pos[y] - lane0, before = from[y] - lane0;
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        float x = s[y][n][i] * cs;
+                        if (!open) x = n * 16 + i <= upto && n * 16 + i > before ? x : -INFINITY;
+                        s[y][n][i] = x;
+                        top = fmaxf(top, x);
+                    }
+                const float m_new = fmaxf(m[y], column_max(top));
+                const float ref = m_new == -INFINITY ? 0.0f : m_new - P_TOP;
+                const float alpha = weight(m[y], m_new);
+                float sum = 0.0f;
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float x = __builtin_amdgcn_exp2f(s[y][n][i] - ref);
+                        sum += x;
+                        const _Float16 hi = (_Float16)x;
+                        p[y][n / 2][0][(n % 2) * 4 + i] = hi;
+                        if (SPLIT2) p[y][n / 2][NH - 1][(n % 2) * 4 + i] = (_Float16)(x - (float)hi);
+                    }
+                l[y] = l[y] * alpha + sum;
+                m[y] = m_new;
+                const float f = alpha * ev_step;
+                if (__any(f != 1.0f)) {
+#pragma unroll
+                    for (int d = 0; d < ND; d++) o[y][d] *= f;
+                }
             }
 #pragma unroll
             for (int d = 0; d < ND; d++) {
                 const h8 a = to_half(vr[d][0], vr[d][1]), b = to_half(vr[d][2], vr[d][3]);
 #pragma unroll
-                for (int n = 0; n < NH; n++) {
-                    o[d] = mma(a, p[0][n], o[d]);
-                    o[d] = mma(b, p[1][n], o[d]);
-                }
+                for (int y = 0; y < CG; y++)
+#pragma unroll
+                    for (int n = 0; n < NH; n++) {
+                        o[y][d] = mma(a, p[y][0][n], o[y][d]);
+                        o[y][d] = mma(b, p[y][1][n], o[y][d]);
+                    }
             }
             if (k + 1 < count) load_v(k + 1);
         }
     }
-    l = column_sum(l);
 
     // ---- the waves' results joined ----
     constexpr int LROW = HD + 4;
     const float unit = sp_fp8_pow2(ev_now);
-    if (active) {
-        float *rec = smem + (w * n_cols + col) * LROW;
 #pragma unroll
-        for (int d = 0; d < ND; d++) *reinterpret_cast<f4 *>(rec + d * 16 + g * 4) = o[d] * unit;
-        if (g == 0) {
-            rec[HD] = m;
-            rec[HD + 1] = l;
+    for (int y = 0; y < CG; y++) {
+        const float sum = column_sum(l[y]);
+        if (active[y]) {
+            float *rec = smem + (w * n_cols + y * 16 + col) * LROW;
+#pragma unroll
+            for (int d = 0; d < ND; d++) *reinterpret_cast<f4 *>(rec + d * 16 + g * 4) = o[y][d] * unit;
+            if (g == 0) {
+                rec[HD] = m[y];
+                rec[HD + 1] = sum;
+            }
         }
     }
     __syncthreads();
     const long long slot = (long long)sh.slot * A.H + h;
-    for (int at = tid; at < n_cols * (HD / 2); at += NW * 64) {
+    const bool alone = sh.n_split == 1;
+    if (!alone && slot >= SP_FP8_SLOTS) return;  // (cannot be: see find_share)
+    const int pairs = n_cols * (HD / 2);
+    for (int at = tid; at < pairs; at += NT) {
         const int cc = at / (HD / 2), d = at % (HD / 2) * 2;
-        float M = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < NW; v++) M = fmaxf(M, smem[(v * n_cols + cc) * LROW + HD]);
-        float L = 0.0f, x = 0.0f, y = 0.0f;
-#pragma unroll
+        Acc acc;
+#pragma unroll 4
+        for (int v = 0; v < NW; v++) acc.M = fmaxf(acc.M, smem[(v * n_cols + cc) * LROW + HD]);
+#pragma unroll 4
         for (int v = 0; v < NW; v++) {
             const float *rec = smem + (v * n_cols + cc) * LROW;
-            const float f = weight(rec[HD], M);
-            L += rec[HD + 1] * f;
-            x += rec[d] * f;
-            y += rec[d + 1] * f;
+            const float f = weight(rec[HD], acc.M);
+            acc.L += rec[HD + 1] * f;
+            acc.x += rec[d] * f;
+            acc.y += rec[d + 1] * f;
         }
-        if (sh.n_split == 1) {
+        if (alone) {
             const long long n = c0 + cc;
-            finish<DT>(A, sh.r0 + n / A.G, h * A.G + (int)(n % A.G), HD, d, M, L, x, y);
-        } else if (slot < SP_FP8_SLOTS) {
+            finish<DT>(A, sh.r0 + n / A.G, h * A.G + (int)(n % A.G), HD, d, acc.M, acc.L, acc.x, acc.y);
+        } else {
             float *dst = A.part + (slot * COLS + cc) * ROW;
-            if (d == 0) put_pair(dst, M, L);
-            put_pair(dst + 2 + d, x, y);
+            if (d == 0) put_pair(dst, acc.M, acc.L);
+            put_pair(dst + 2 + d, acc.x, acc.y);
         }
     }
-    if (sh.n_split == 1 || slot >= SP_FP8_SLOTS) return;
+    if (alone) return;
 
     // ---- the last of the column group's shares to arrive joins them all, in their order ----
     // each block's stores are complete before it counts itself
@@ -382,66 +466,79 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
     }
     __syncthreads();
     if (!last_flag) return;
-    for (int at = tid; at < n_cols * (HD / 2); at += NW * 64) {
+    // groups of threads take runs of shares, so that a run's loads are in flight together
+    const int groups = pairs < NT ? min(NT / pairs, NW / 2) : 1, run = (sh.n_split + groups - 1) / groups;
+    for (int i0 = 0; i0 < pairs; i0 += NT) {
+        const int grp = groups == 1 ? 0 : tid / pairs, at = i0 + tid - grp * pairs;
+        const bool here = grp < groups && at < pairs;
         const int cc = at / (HD / 2), d = at % (HD / 2) * 2;
-        const float *src = A.part + (slot0 * COLS + cc) * ROW;
-        const long long step = (long long)A.H * COLS * ROW;
-        float M = -INFINITY, L = 0.0f, x = 0.0f, y = 0.0f;
-        for (int v0 = 0; v0 < sh.n_split; v0 += 8) {
-            f2 ml[8], xy[8];
+        const int v1 = min((grp + 1) * run, sh.n_split);
+        Acc acc;
+        if (here) {
+            const float *src = A.part + (slot0 * COLS + cc) * ROW;
+            const long long step = (long long)A.H * COLS * ROW;
+            for (int v0 = grp * run; v0 < v1; v0 += 8) {
+                f2 ml[8], xy[8];
 #pragma unroll
-            for (int v = 0; v < 8; v++) {
-                const float *rec = src + min(v0 + v, sh.n_split - 1) * step;
-                ml[v] = get_pair(rec);
-                xy[v] = get_pair(rec + 2 + d);
-            }
-            float Mn = M;
-#pragma unroll
-            for (int v = 0; v < 8; v++)
-                if (v0 + v < sh.n_split) Mn = fmaxf(Mn, ml[v].x);
-            const float f0 = weight(M, Mn);
-            L *= f0;
-            x *= f0;
-            y *= f0;
-#pragma unroll
-            for (int v = 0; v < 8; v++) {
-                const float f = v0 + v < sh.n_split ? weight(ml[v].x, Mn) : 0.0f;
-                if (v0 + v < sh.n_split) {
-                    L += ml[v].y * f;
-                    x += xy[v].x * f;
-                    y += xy[v].y * f;
+                for (int v = 0; v < 8; v++) {
+                    const float *rec = src + min(v0 + v, v1 - 1) * step;
+                    ml[v] = get_pair(rec);
+                    xy[v] = get_pair(rec + 2 + d);
                 }
+#pragma unroll
+                for (int v = 0; v < 8; v++)
+                    if (v0 + v < v1) acc.add(ml[v].x, ml[v].y, xy[v].x, xy[v].y);
             }
-            M = Mn;
         }
-        const long long n = c0 + cc;
-        finish<DT>(A, sh.r0 + n / A.G, h * A.G + (int)(n % A.G), HD, d, M, L, x, y);
+        if (groups > 1) {  // pairs < NT: one round
+            f4 *join = reinterpret_cast<f4 *>(smem);
+            if (here && grp) join[(grp - 1) * pairs + at] = f4{acc.M, acc.L, acc.x, acc.y};
+            __syncthreads();
+            if (here && !grp)
+                for (int v = 0; v < groups - 1; v++) {
+                    const f4 r = join[v * pairs + at];
+                    acc.add(r[0], r[1], r[2], r[3]);
+                }
+        }
+        if (here && !grp) {
+            const long long n = c0 + cc;
+            finish<DT>(A, sh.r0 + n / A.G, h * A.G + (int)(n % A.G), HD, d, acc.M, acc.L, acc.x, acc.y);
+        }
     }
 }
 
-template <int HD, int DT, int NW>
-hipError_t launch(const SpFp8Attn &A, hipStream_t s) {
-    constexpr int COLS = 16;
+template <int HD, int DT, int NW, int CG>
+hipError_t launch(const SpFp8Attn &A, int per_cu, hipStream_t s) {
+    constexpr int COLS = 16 * CG;
+    SpFp8Attn a = A;
+    a.target = min(A.target * per_cu, SP_FP8_SLOTS / 2);
     // column groups: each sequence's rows times G, in groups of COLS
     const long long groups = A.s.row ? ((long long)A.s.n_rows * A.G) / COLS + A.s.n_seq
                                      : (long long)A.s.n_seq * ((A.G + COLS - 1) / COLS);
     // shares: one per group, and at most target more over all KV heads
-    const long long blocks = (groups + (A.target + A.H - 1) / A.H) * A.H;
+    const long long blocks = (groups + (a.target + A.H - 1) / A.H) * A.H;
     if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
     const int cols = A.s.row ? COLS : (A.G < COLS ? A.G : COLS);
     const size_t lds = (size_t)NW * cols * (HD + 4) * sizeof(float);
-    SpFp8Attn a = A;
     void *args[] = {&a};
-    const void *f = (const void *)k_fp8_attn<HD, DT, NW>;
+    const void *f = (const void *)k_fp8_attn<HD, DT, NW, CG>;
     return hipLaunchKernel(f, dim3((unsigned)blocks), dim3(NW * 64), args, lds, s);
 }
 
+template <int HD, int DT>
+hipError_t launch_dt(const SpFp8Attn &A, hipStream_t s) {
+    constexpr int NW = HD == 256 ? 4 : 8;
+    constexpr int CG = HD == 256 || DT == SP_DTYPE_F32 ? 1 : 2;
+    if ((long long)A.s.n_rows * A.G > 16ll * A.s.n_seq) return launch<HD, DT, NW, CG>(A, 1, s);
+    return launch<HD, DT, NW, 1>(A, 1, s);
+}
+
 template <int HD>
-hipError_t launch_dt(const SpFp8Attn &A, int dtype, hipStream_t s) {
+hipError_t launch_hd(const SpFp8Attn &A, int dtype, hipStream_t s) {
     switch (dtype) {
-        case SP_DTYPE_F32: return launch<HD, SP_DTYPE_F32, 4>(A, s);
-        case SP_DTYPE_F16: return launch<HD, SP_DTYPE_F16, 4>(A, s);
-        case SP_DTYPE_BF16: return launch<HD, SP_DTYPE_BF16, 4>(A, s);
+        case SP_DTYPE_F32: return launch_dt<HD, SP_DTYPE_F32>(A, s);
+        case SP_DTYPE_F16: return launch_dt<HD, SP_DTYPE_F16>(A, s);
+        case SP_DTYPE_BF16: return launch_dt<HD, SP_DTYPE_BF16>(A, s);
     }
     return hipErrorInvalidValue;
 }
@@ -452,10 +549,10 @@ size_t sp_fp8_workspace_floats(int hd) { return (size_t)SP_FP8_SLOTS * 32 * (hd 
 
 hipError_t sp_fp8_launch_attn(const SpFp8Attn &A, int hd, int dtype, hipStream_t s) {
     switch (hd) {
-        case 64: return launch_dt<64>(A, dtype, s);
-        case 96: return launch_dt<96>(A, dtype, s);
-        case 128: return launch_dt<128>(A, dtype, s);
-        case 256: return launch_dt<256>(A, dtype, s);
+        case 64: return launch_hd<64>(A, dtype, s);
+        case 96: return launch_hd<96>(A, dtype, s);
+        case 128: return launch_hd<128>(A, dtype, s);
+        case 256: return launch_hd<256>(A, dtype, s);
     }
     return hipErrorInvalidValue;
 }

@@ -14,7 +14,7 @@
 namespace {
 
 struct Fp8Priv {
-    int device = 0;
+    int device = 0, cus = 256;
     float *part = nullptr;
     int *counters = nullptr;
 };
@@ -182,7 +182,7 @@ int attend(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *b, 
     A.negate = kq_scale < 0.0f;
     A.part = pv->part;
     A.counters = pv->counters;
-    A.target = SP_FP8_SLOTS / 2;
+    A.target = pv->cus;
     return ok(sp_fp8_launch_attn(A, hd, dtype, s), who) ? 0 : -1;
 }
 
@@ -213,7 +213,8 @@ extern "C" int sp_hip_fp8_cache_init(sp_hip_fp8_cache_t *c, const sp_config_t *c
     c->priv = pv;
     const hipStream_t s = (hipStream_t)stream;
     const size_t nexp = (size_t)tiles, ncode = nexp * SP_FP8_BLOCK * hd;
-    bool good = ok(hipGetDevice(&pv->device), who) && stream_ok(c, s, who);
+    bool good = ok(hipGetDevice(&pv->device), who) && stream_ok(c, s, who) &&
+                ok(hipDeviceGetAttribute(&pv->cus, hipDeviceAttributeMultiprocessorCount, pv->device), who);
     struct Piece {
         void **p;
         size_t bytes;
