@@ -59,15 +59,17 @@ struct SpFp8Attn {
     int window;
     float c;   // kq_scale * log2(e), not negative
     int negate;
-    float *part;    // partial results, SP_FP8_SLOTS slots of 32 rows of hd + 2 floats
-    int *counters;  // one per slot, zero between calls
+    float *part;    // partial results: sp_fp8_part_rows(hd) rows of hd + 2 floats
+    int *counters;  // SP_FP8_SLOTS, one per partial result, zero between calls
     int target;     // CUs; the launch makes it the blocks that fill them
 };
 
 hipError_t sp_fp8_launch_write(const SpFp8Copy &A, int hd, int dtype, hipStream_t s);
 hipError_t sp_fp8_launch_read(const SpFp8Copy &A, int hd, int dtype, hipStream_t s);
 hipError_t sp_fp8_launch_attn(const SpFp8Attn &A, int hd, int dtype, hipStream_t s);
-size_t sp_fp8_workspace_floats(int hd);
+// Rows of partial results: two for each CU's columns (256 of the prompt kernel's blocks, 128 at
+// head_dim 256) on 256 CUs; the kernel for few rows needs fewer.
+inline int sp_fp8_part_rows(int hd) { return hd == 256 ? 1 << 16 : 1 << 17; }
 
 #define SP_FP8_SLOTS 1024
 
@@ -128,3 +130,44 @@ struct SpFp8Elem<SP_DTYPE_BF16> {
 
 // 2^e for e in [-126, 127]
 __device__ __forceinline__ float sp_fp8_pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+namespace sp_fp8 {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+
+// Four elements of a row; `aligned`: at an address that a vector load takes.
+template <int DT>
+__device__ __forceinline__ f4 load4(const void *base, long long off, bool aligned) {
+    typedef typename SpFp8Elem<DT>::T T;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    const T *p = reinterpret_cast<const T *>(base) + off;
+    f4 x;
+    if (aligned) {
+        const T4 v = *reinterpret_cast<const T4 *>(p);
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = SpFp8Elem<DT>::get(v[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = SpFp8Elem<DT>::get(p[k]);
+    }
+    return x;
+}
+
+template <int DT>
+__device__ __forceinline__ void store4(void *base, long long off, f4 x, bool aligned) {
+    typedef typename SpFp8Elem<DT>::T T;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T *p = reinterpret_cast<T *>(base) + off;
+    T4 v;
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = SpFp8Elem<DT>::put(x[k]);
+    if (aligned) {
+        *reinterpret_cast<T4 *>(p) = v;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) p[k] = v[k];
+    }
+}
+
+}  // namespace sp_fp8

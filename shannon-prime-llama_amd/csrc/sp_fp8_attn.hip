@@ -24,8 +24,9 @@
 
 namespace {
 
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+using sp_fp8::f4;
+using sp_fp8::u4;
+using sp_fp8::store4;
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
@@ -106,7 +107,7 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
             if ((float)shares_of(e.nb, r, least) * (float)e.ct * (float)A.H <= (float)A.target) R = r;
         }
         const int ns = shares_of(e.nb, R, least);
-        out = Share{0, e.a, e.b - e.a, e.len - (e.b - e.a), item / ns, item % ns, ns, item};
+        out = Share{0, e.a, e.b - e.a, e.len - (e.b - e.a), e.ct - 1 - item / ns, item % ns, ns, item};
         return item < e.ct * ns;
     }
     const Extent e0 = extent(A, lane, cols);  // kept: up to 64 sequences are read once
@@ -144,8 +145,9 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
             out.first = __shfl(e.len, l, 64) - out.n_new;
             out.n_split = __shfl(ns, l, 64);
             const int at = item - (__shfl(sum, l, 64) - __shfl(mine, l, 64));
-            out.ct = at / out.n_split;
-            out.split = at - out.ct * out.n_split;
+            // the last column group first: under the causal mask it sees most
+            out.ct = __shfl(e.ct, l, 64) - 1 - at / out.n_split;
+            out.split = at % out.n_split;
             out.slot = slots + __shfl(psum, l, 64) - __shfl(part, l, 64) + at;
             return true;
         }
@@ -193,14 +195,19 @@ __device__ __forceinline__ float weight(float m, float M) {
 
 template <int DT>
 __device__ __forceinline__ void finish(const SpFp8Attn &A, long long row, int head, int hd, int d, float m, float l,
-                                       float o0, float o1) {
+                                       float o0, float o1, float p_top) {
     typedef typename SpFp8Elem<DT>::T T;
     T *out = reinterpret_cast<T *>(A.out) + row * A.out_stride + (long long)head * hd + d;
     const float r = l == 0.0f ? 0.0f : 1.0f / l;
     out[0] = SpFp8Elem<DT>::put(l == 0.0f ? 0.0f : o0 * r);
     out[1] = SpFp8Elem<DT>::put(l == 0.0f ? 0.0f : o1 * r);
     if (A.lse && d == 0)
-        A.lse[row * A.H * A.G + head] = l == 0.0f ? -INFINITY : (m - P_TOP + __log2f(l)) * 0.69314718055994531f;
+        A.lse[row * A.H * A.G + head] = l == 0.0f ? -INFINITY : (m - p_top + __log2f(l)) * 0.69314718055994531f;
+}
+
+// Whether a partial result has its place (always: see find_share).
+__device__ __forceinline__ bool slot_fits(long long slot, int cols, int hd) {
+    return slot < SP_FP8_SLOTS && (slot + 1) * cols <= (hd == 256 ? 1 << 16 : 1 << 17);
 }
 
 // Joins partial results (m, l, o pair) in order.
@@ -214,6 +221,66 @@ struct Acc {
         M = Mn;
     }
 };
+
+// The last of a column group's shares to arrive joins them all, in their order. Every thread of
+// the block calls it after its partial's stores. smem: at least NW * n_cols * HD floats.
+template <int HD, int DT, int NW, int COLS>
+__device__ __forceinline__ void join_shares(const SpFp8Attn &A, const Share &sh, int h, long long c0, int n_cols,
+                                            float *smem, int *last_flag) {
+    constexpr int NT = NW * 64, ROW = HD + 2;
+    const int tid = threadIdx.x, pairs = n_cols * (HD / 2);
+    // each block's stores are complete before it counts itself
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const long long slot0 = (long long)(sh.slot - sh.split) * A.H + h;
+    if (tid == 0) {
+        int *cnt = A.counters + slot0;
+        const int arrived = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *last_flag = arrived == sh.n_split - 1;
+        if (*last_flag) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+    }
+    __syncthreads();
+    if (!*last_flag) return;
+    // groups of threads take runs of shares, so that a run's loads are in flight together
+    const int groups = pairs < NT ? min(NT / pairs, NW / 2) : 1, run = (sh.n_split + groups - 1) / groups;
+    for (int i0 = 0; i0 < pairs; i0 += NT) {
+        const int grp = groups == 1 ? 0 : tid / pairs, at = i0 + tid - grp * pairs;
+        const bool here = grp < groups && at < pairs;
+        const int cc = at / (HD / 2), d = at % (HD / 2) * 2;
+        const int v1 = min((grp + 1) * run, sh.n_split);
+        Acc acc;
+        if (here) {
+            const float *src = A.part + (slot0 * COLS + cc) * ROW;
+            const long long step = (long long)A.H * COLS * ROW;
+            for (int v0 = grp * run; v0 < v1; v0 += 8) {
+                f2 ml[8], xy[8];
+#pragma unroll
+                for (int v = 0; v < 8; v++) {
+                    const float *rec = src + min(v0 + v, v1 - 1) * step;
+                    ml[v] = get_pair(rec);
+                    xy[v] = get_pair(rec + 2 + d);
+                }
+#pragma unroll
+                for (int v = 0; v < 8; v++)
+                    if (v0 + v < v1) acc.add(ml[v].x, ml[v].y, xy[v].x, xy[v].y);
+            }
+        }
+        if (groups > 1) {  // pairs < NT: one round
+            f4 *join = reinterpret_cast<f4 *>(smem);
+            if (here && grp) join[(grp - 1) * pairs + at] = f4{acc.M, acc.L, acc.x, acc.y};
+            __syncthreads();
+            if (here && !grp)
+                for (int v = 0; v < groups - 1; v++) {
+                    const f4 r = join[v * pairs + at];
+                    acc.add(r[0], r[1], r[2], r[3]);
+                }
+        }
+        if (here && !grp) {
+            const long long n = c0 + cc;
+            finish<DT>(A, sh.r0 + n / A.G, h * A.G + (int)(n % A.G), HD, d, acc.M, acc.L, acc.x, acc.y, P_TOP);
+        }
+    }
+}
 
 // CG groups of 16 columns share each block's loads and conversions.
 template <int HD, int DT, int NW, int CG>
@@ -427,7 +494,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
     __syncthreads();
     const long long slot = (long long)sh.slot * A.H + h;
     const bool alone = sh.n_split == 1;
-    if (!alone && slot >= SP_FP8_SLOTS) return;  // (cannot be: see find_share)
+    if (!alone && !slot_fits(slot, COLS, HD)) return;
     const int pairs = n_cols * (HD / 2);
     for (int at = tid; at < pairs; at += NT) {
         const int cc = at / (HD / 2), d = at % (HD / 2) * 2;
@@ -444,7 +511,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
         }
         if (alone) {
             const long long n = c0 + cc;
-            finish<DT>(A, sh.r0 + n / A.G, h * A.G + (int)(n % A.G), HD, d, acc.M, acc.L, acc.x, acc.y);
+            finish<DT>(A, sh.r0 + n / A.G, h * A.G + (int)(n % A.G), HD, d, acc.M, acc.L, acc.x, acc.y, P_TOP);
         } else {
             float *dst = A.part + (slot * COLS + cc) * ROW;
             if (d == 0) put_pair(dst, acc.M, acc.L);
@@ -453,58 +520,307 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
     }
     if (alone) return;
 
-    // ---- the last of the column group's shares to arrive joins them all, in their order ----
-    // each block's stores are complete before it counts itself
-    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    const long long slot0 = (long long)(sh.slot - sh.split) * A.H + h;
-    if (tid == 0) {
-        int *cnt = A.counters + slot0;
-        const int arrived = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last_flag = arrived == sh.n_split - 1;
-        if (last_flag) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
-    }
-    __syncthreads();
-    if (!last_flag) return;
-    // groups of threads take runs of shares, so that a run's loads are in flight together
-    const int groups = pairs < NT ? min(NT / pairs, NW / 2) : 1, run = (sh.n_split + groups - 1) / groups;
-    for (int i0 = 0; i0 < pairs; i0 += NT) {
-        const int grp = groups == 1 ? 0 : tid / pairs, at = i0 + tid - grp * pairs;
-        const bool here = grp < groups && at < pairs;
-        const int cc = at / (HD / 2), d = at % (HD / 2) * 2;
-        const int v1 = min((grp + 1) * run, sh.n_split);
-        Acc acc;
-        if (here) {
-            const float *src = A.part + (slot0 * COLS + cc) * ROW;
-            const long long step = (long long)A.H * COLS * ROW;
-            for (int v0 = grp * run; v0 < v1; v0 += 8) {
-                f2 ml[8], xy[8];
+    join_shares<HD, DT, NW, COLS>(A, sh, h, c0, n_cols, smem, &last_flag);
+}
+
+// ---------------------------------------------------------------------------
+// many rows: prompts and their chunks
+// ---------------------------------------------------------------------------
+// A block of threads holds 32 columns a wave and shares each cache block's conversion: the
+// codes become fp16 once, in LDS, in the operand order of v_mfma_f32_32x32x16_f16, two buffers
+// deep with one barrier a block. As above the scores are K q^T and the weights stay where they
+// were made: lane (column, half)'s registers 8 k .. 8 k + 7 are positions
+// 16 k + 8 (j / 4) + 4 half + j % 4, and V's operand is laid out for that order.
+//
+// The running maximum is a reference that is raised only when a score passes it by 2^8 (the
+// weights then still fit fp16 with their 2^6 at the reference), so that the output is rescaled
+// a few times in a whole sequence and no exchange between lanes is needed in the others. Weights
+// below 2^-20 of the reference are subnormal fp16 numbers then, rounded at 2^-31 of it. Split
+// weights (fp32 results) count from 2^14 and their reference follows within a factor of two, so
+// that the second part keeps its bits.
+typedef float f16x __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f16x mma32(h8 a, h8 b, f16x c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// LDS written before is seen after, by the whole block; loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+template <int HD, int DT, int NW>
+__global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
+    constexpr int COLS = 32 * NW, NS = HD / 16, ND = HD / 32, TILE = 64 * HD, ROW = HD + 2, NT = NW * 64, HT = NT / 2;
+    constexpr bool SPLIT2 = DT == SP_DTYPE_F32;
+    constexpr int NH = SPLIT2 ? 2 : 1;
+    constexpr float W_TOP = SPLIT2 ? 14.0f : 6.0f, W_SLACK = SPLIT2 ? 1.0f : 8.0f;
+    constexpr int KP = (HD * 4 + HT - 1) / HT;  // K pieces of 16 codes a thread (half the threads)
+    constexpr int VP = (HD * 2 + HT - 1) / HT;  // pairs of V pieces (the other half)
+    constexpr int RAW = KP > 2 * VP ? KP : 2 * VP;
+    typedef typename SpFp8Elem<DT>::T T;
+    extern __shared__ __align__(16) float smem[];  // two buffers of K and V, 64 * HD fp16 each
+    __shared__ int last_flag;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = blockIdx.x % A.H;
+    Share sh;
+    if (!find_share(A, blockIdx.x / A.H, lane, COLS, 8, sh)) return;
+    const int n_cols = (int)min((long long)sh.n_new * A.G - (long long)sh.ct * COLS, (long long)COLS);
+    const int col = lane & 31, half = lane >> 5;
+    const long long c0 = (long long)sh.ct * COLS;
+    const int pos0 = sh.first + (int)(c0 / A.G), pos1 = sh.first + (int)((c0 + n_cols - 1) / A.G);
+    const int j0 = A.window > 0 ? max(pos0 - A.window + 1, 0) >> 6 : 0;
+    const int j1 = min((pos1 >> 6) + 1, A.s.stride);
+    const int per = max((j1 - j0 + sh.n_split - 1) / sh.n_split, 0);
+    const int t0 = j0 + sh.split * per, n = max(min(t0 + per, j1) - t0, 0);
+
+    int blk = -1, ekb = 0, evb = 0;  // lane k: block number and scale bytes of the (base + k)-th block
+    const auto look_up = [&](int base) {
+        blk = base + lane < n ? sp_fp8_block(A.s, sh.seq, t0 + base + lane) : -1;
+        const long long at = (long long)max(blk, 0) * A.H + h;
+        ekb = A.k.exps[at];
+        evb = A.v.exps[at];
+    };
+    struct Facts {  // of a block that is on its way
+        bool none;
+        int ek, ev;
+    };
+    const auto facts = [&](int k) {
+        return Facts{__builtin_amdgcn_readlane(blk, k) < 0, sp_fp8_exponent(__builtin_amdgcn_readlane(ekb, k)),
+                     sp_fp8_exponent(__builtin_amdgcn_readlane(evb, k))};
+    };
+    // ---- staging: half of the threads bring K, half V ----
+    const bool stage_v = tid >= HT;
+    const int st = stage_v ? tid - HT : tid;
+    u4 raw[RAW];
+    const auto fetch = [&](int k) {  // k: within the looked-up 64
+        const long long b = (long long)max(__builtin_amdgcn_readlane(blk, k), 0) * A.H + h;  // none: block 0, masked
+        if (!stage_v) {
+            const uint8_t *p = A.k.codes + b * TILE;
 #pragma unroll
-                for (int v = 0; v < 8; v++) {
-                    const float *rec = src + min(v0 + v, v1 - 1) * step;
-                    ml[v] = get_pair(rec);
-                    xy[v] = get_pair(rec + 2 + d);
+            for (int i = 0; i < KP; i++)
+                if (KP * HT == HD * 4 || st + i * HT < HD * 4) raw[i] = *reinterpret_cast<const u4 *>(p + (st + i * HT) * 16);
+        } else {
+            const uint8_t *p = A.v.codes + b * TILE;
+#pragma unroll
+            for (int i = 0; i < VP; i++) {
+                const int x = st + i * HT;  // (D, gl, dg % 2, r): pieces g = gl and gl + 2 of channel group 2 D + dg % 2
+                if (VP * HT == HD * 2 || x < HD * 2) {
+                    const uint8_t *s = p + ((x >> 6) * 2 + ((x >> 4) & 1)) * 1024 + ((x >> 5) & 1) * 256 + (x & 15) * 16;
+                    raw[2 * i] = *reinterpret_cast<const u4 *>(s);
+                    raw[2 * i + 1] = *reinterpret_cast<const u4 *>(s + 512);
                 }
-#pragma unroll
-                for (int v = 0; v < 8; v++)
-                    if (v0 + v < v1) acc.add(ml[v].x, ml[v].y, xy[v].x, xy[v].y);
             }
         }
-        if (groups > 1) {  // pairs < NT: one round
-            f4 *join = reinterpret_cast<f4 *>(smem);
-            if (here && grp) join[(grp - 1) * pairs + at] = f4{acc.M, acc.L, acc.x, acc.y};
-            __syncthreads();
-            if (here && !grp)
-                for (int v = 0; v < groups - 1; v++) {
-                    const f4 r = join[v * pairs + at];
-                    acc.add(r[0], r[1], r[2], r[3]);
+    };
+    const auto stage = [&](int buf) {
+        h8 *kd = reinterpret_cast<h8 *>(smem) + buf * (2 * TILE / 8), *vd = kd + TILE / 8;
+        if (!stage_v) {
+#pragma unroll
+            for (int i = 0; i < KP; i++) {
+                const int x = st + i * HT, g = (x >> 4) & 3, r = x & 15, uc = x >> 6;  // uc = u * HD/32 + c
+                if (KP * HT == HD * 4 || x < HD * 4) {
+                    h8 *d = kd + (uc * 2 + (g >> 1)) * 64 + (g & 1) * 32 + r;
+                    d[0] = to_half(raw[i][0], raw[i][1]);
+                    d[16] = to_half(raw[i][2], raw[i][3]);
                 }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VP; i++) {
+                const int x = st + i * HT;
+                if (VP * HT == HD * 2 || x < HD * 2) {
+                    h8 *d = vd + (x >> 6) * 256 + (x & 63);
+#pragma unroll
+                    for (int t4 = 0; t4 < 4; t4++) d[t4 * 64] = to_half(raw[2 * i][t4], raw[2 * i + 1][t4]);
+                }
+            }
         }
-        if (here && !grp) {
-            const long long n = c0 + cc;
-            finish<DT>(A, sh.r0 + n / A.G, h * A.G + (int)(n % A.G), HD, d, acc.M, acc.L, acc.x, acc.y);
+    };
+    if (n > 0) {
+        look_up(0);
+        fetch(0);
+    }
+
+    // ---- queries ----
+    const int mycol = w * 32 + col;
+    const bool active = mycol < n_cols;
+    const long long cn = c0 + (active ? mycol : 0);
+    const int tk = (int)(cn / A.G), head = h * A.G + (int)(cn % A.G);
+    const long long row = (long long)sh.r0 + tk;
+    const int pos = active ? sh.first + tk : -1;
+    const int from = A.window > 0 ? pos - A.window : -1;  // sees (from, pos]
+    // of this wave's columns: whether there are any, and the range that each of them sees
+    const bool busy = w * 32 < n_cols;
+    const int wlast = min(w * 32 + 31, n_cols - 1);
+    const int wpos0 = sh.first + (int)((c0 + w * 32) / A.G), wpos1 = sh.first + (int)((c0 + wlast) / A.G);
+    h8 q[NS][NH];
+    float cscale;
+    {
+        const T *src = reinterpret_cast<const T *>(A.q) + row * A.q_stride + (long long)head * HD + half * 8;
+        const bool aligned = ((uintptr_t)A.q % (4 * sizeof(T))) == 0 && A.q_stride % 4 == 0;
+        float top = 0.0f;
+        float x[8];
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            load8<DT>(src + s * 16, aligned, x);
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
+        }
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        int e = (__float_as_int(top) >> 23) - 127 - 14;
+        e = top == 0.0f || !(top < INFINITY) ? 0 : max(e, -126);
+        const float down = A.negate ? -sp_fp8_pow2(-e) : sp_fp8_pow2(-e);
+        cscale = A.c * sp_fp8_pow2(e);
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            load8<DT>(src + s * 16, aligned, x);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float v = active ? x[k] * down : 0.0f;
+                const _Float16 hi = (_Float16)v;
+                q[s][0][k] = hi;
+                if (SPLIT2) q[s][NH - 1][k] = (_Float16)(v - (float)hi);
+            }
         }
     }
+
+    f16x o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d] = f16x{};
+    float m = -INFINITY, off = 0.0f, l = 0.0f;  // off = W_TOP - m, 0 where m is -inf
+    int ev_now = 0;
+    bool huge = false;  // a fused score - reference could be far above 0 where they should be equal
+    Facts now{true, 0, 0}, next{true, 0, 0};
+    if (n > 0) {
+        now = facts(0);
+        stage(0);
+        if (n > 1) {
+            fetch(1);
+            next = facts(1);
+        }
+    }
+    lds_barrier();
+    for (int k = 0; k < n; k++) {
+        const int t = t0 + k, ev = now.ev;
+        const h8 *kd = reinterpret_cast<const h8 *>(smem) + (k & 1) * (2 * TILE / 8) + lane, *vd = kd + TILE / 8;
+        const bool sees = busy && !now.none && t * 64 <= wpos1 && (A.window <= 0 || t * 64 + 63 > wpos0 - A.window);
+        h8 p[4][NH];
+        if (sees) {
+            f16x s[2];
+            s[0] = f16x{};
+            s[1] = f16x{};
+#pragma unroll
+            for (int c = 0; c < NS; c++) {
+                const h8 a = kd[c * 64], b = kd[(NS + c) * 64];
+#pragma unroll
+                for (int x = 0; x < NH; x++) {
+                    s[0] = mma32(a, q[c][x], s[0]);
+                    s[1] = mma32(b, q[c][x], s[1]);
+                }
+            }
+            // never 0: a masked score stays -inf when it is multiplied
+            float cs = fmaxf(cscale * sp_fp8_pow2(now.ek), 0x1p-126f);
+            if (!(t * 64 + 63 <= wpos0 && (A.window <= 0 || t * 64 > wpos1 - A.window))) {
+                const int lane0 = t * 64 + 4 * half, upto = pos - lane0, before = from - lane0;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int at = u * 32 + (i >> 2) * 8 + (i & 3);
+                        s[u][i] = at <= upto && at > before ? s[u][i] : -INFINITY;
+                    }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 32; i++) top = fmaxf(top, s[i >> 4][i & 15]);
+            const bool raise = m == -INFINITY ? top > -INFINITY : __builtin_fmaf(top, cs, off) > W_TOP + W_SLACK;
+            float f = sp_fp8_pow2(ev_now - ev);
+            ev_now = ev;
+            bool rescale = f != 1.0f;
+            if (__any(raise)) {
+                const float mx = fmaxf(top, __shfl_xor(top, 32, 64)) * cs, m_new = fmaxf(m, mx);
+                const float alpha = weight(m, m_new);
+                l *= alpha;
+                f *= alpha;
+                m = m_new;
+                off = m == -INFINITY ? 0.0f : W_TOP - m;
+                rescale = true;
+                huge = __any(fabsf(m) > 0x1p18f && m > -INFINITY);
+            }
+            if (huge) {  // the reference was rounded: round the scores as it was
+#pragma unroll
+                for (int i = 0; i < 32; i++) s[i >> 4][i & 15] *= cs;
+                cs = 1.0f;
+            }
+            if (rescale) {
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d] *= f;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], cs, off));
+                sum += x;
+                const _Float16 hi = (_Float16)x;
+                p[i >> 3][0][i & 7] = hi;
+                if (SPLIT2) p[i >> 3][NH - 1][i & 7] = (_Float16)(x - (float)hi);
+            }
+            l += sum;
+        }
+        if (k + 1 < n) stage((k + 1) & 1);
+        if (sees) {
+#pragma unroll
+            for (int t4 = 0; t4 < 4; t4++)
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const h8 a = vd[(d * 4 + t4) * 64];
+#pragma unroll
+                    for (int x = 0; x < NH; x++) o[d] = mma32(a, p[t4][x], o[d]);
+                }
+        }
+        now = next;
+        if (k + 2 < n) {
+            if (((k + 2) & 63) == 0) look_up(k + 2);
+            fetch((k + 2) & 63);
+            next = facts((k + 2) & 63);
+        }
+        lds_barrier();
+    }
+    l += __shfl_xor(l, 32, 64);
+
+    // ---- results ----
+    const bool alone = sh.n_split == 1;
+    const long long slot = (long long)sh.slot * A.H + h;
+    if (!alone && !slot_fits(slot, COLS, HD)) return;
+    const float unit = sp_fp8_pow2(ev_now);
+    if (active && alone) {
+        T *out = reinterpret_cast<T *>(A.out) + row * A.out_stride + (long long)head * HD;
+        const bool aligned = ((uintptr_t)A.out % (4 * sizeof(T))) == 0 && A.out_stride % 4 == 0;
+        const float r = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                f4 x;
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[j] = l == 0.0f ? 0.0f : o[d][i * 4 + j] * unit * r;
+                store4<DT>(out, d * 32 + i * 8 + half * 4, x, aligned);
+            }
+        if (A.lse && half == 0)
+            A.lse[row * A.H * A.G + head] = l == 0.0f ? -INFINITY : (m - W_TOP + __log2f(l)) * 0.69314718055994531f;
+    }
+    if (alone) return;
+    if (active) {
+        float *dst = A.part + (slot * COLS + mycol) * ROW;
+        if (half == 0) put_pair(dst, m + (P_TOP - W_TOP), l);  // the maximum whose weight would be 2^P_TOP
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                put_pair(dst + 2 + d * 32 + (i >> 1) * 8 + half * 4 + (i & 1) * 2, o[d][2 * i] * unit, o[d][2 * i + 1] * unit);
+    }
+    join_shares<HD, DT, NW, COLS>(A, sh, h, c0, n_cols, smem, &last_flag);
 }
 
 template <int HD, int DT, int NW, int CG>
@@ -526,10 +842,25 @@ hipError_t launch(const SpFp8Attn &A, int per_cu, hipStream_t s) {
 }
 
 template <int HD, int DT>
+hipError_t launch_wide(const SpFp8Attn &A, hipStream_t s) {
+    constexpr int NW = HD == 256 ? 4 : 8, COLS = 32 * NW;
+    SpFp8Attn a = A;
+    a.target = min(A.target, 256);
+    const long long groups = (long long)A.s.n_rows * A.G / COLS + A.s.n_seq;
+    const long long blocks = (groups + (a.target + A.H - 1) / A.H) * A.H;
+    if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
+    void *args[] = {&a};
+    const void *f = (const void *)k_fp8_attn_wide<HD, DT, NW>;
+    return hipLaunchKernel(f, dim3((unsigned)blocks), dim3(NW * 64), args, (size_t)HD * 512, s);
+}
+
+template <int HD, int DT>
 hipError_t launch_dt(const SpFp8Attn &A, hipStream_t s) {
     constexpr int NW = HD == 256 ? 4 : 8;
     constexpr int CG = HD == 256 || DT == SP_DTYPE_F32 ? 1 : 2;
-    if ((long long)A.s.n_rows * A.G > 16ll * A.s.n_seq) return launch<HD, DT, NW, CG>(A, 1, s);
+    const long long columns = (long long)A.s.n_rows * A.G;  // of each KV head
+    if (columns >= 64ll * A.s.n_seq && A.s.row) return launch_wide<HD, DT>(A, s);
+    if (columns > 16ll * A.s.n_seq) return launch<HD, DT, NW, CG>(A, 1, s);
     return launch<HD, DT, NW, 1>(A, 1, s);
 }
 
@@ -544,8 +875,6 @@ hipError_t launch_hd(const SpFp8Attn &A, int dtype, hipStream_t s) {
 }
 
 }  // namespace
-
-size_t sp_fp8_workspace_floats(int hd) { return (size_t)SP_FP8_SLOTS * 32 * (hd + 2); }
 
 hipError_t sp_fp8_launch_attn(const SpFp8Attn &A, int hd, int dtype, hipStream_t s) {
     switch (hd) {

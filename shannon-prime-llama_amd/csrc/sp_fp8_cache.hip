@@ -15,8 +15,10 @@
 
 namespace {
 
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+using sp_fp8::f4;
+using sp_fp8::u4;
+using sp_fp8::load4;
+using sp_fp8::store4;
 
 // The (sequence, cache block) pair of a grid index: sequence, block index in the sequence and
 // the call's rows of it. False: no such pair. Every lane of a wave agrees.
@@ -44,39 +46,6 @@ __device__ __forceinline__ bool pair_of(const SpFp8Seqs &S, int p, int lane, int
         p -= __shfl(sum, 63, 64);
     }
     return false;
-}
-
-template <int DT>
-__device__ __forceinline__ f4 load4(const void *base, long long off, bool aligned) {
-    typedef typename SpFp8Elem<DT>::T T;
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    const T *p = reinterpret_cast<const T *>(base) + off;
-    f4 x;
-    if (aligned) {
-        const T4 v = *reinterpret_cast<const T4 *>(p);
-#pragma unroll
-        for (int k = 0; k < 4; k++) x[k] = SpFp8Elem<DT>::get(v[k]);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++) x[k] = SpFp8Elem<DT>::get(p[k]);
-    }
-    return x;
-}
-
-template <int DT>
-__device__ __forceinline__ void store4(void *base, long long off, f4 x, bool aligned) {
-    typedef typename SpFp8Elem<DT>::T T;
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    T *p = reinterpret_cast<T *>(base) + off;
-    T4 v;
-#pragma unroll
-    for (int k = 0; k < 4; k++) v[k] = SpFp8Elem<DT>::put(x[k]);
-    if (aligned) {
-        *reinterpret_cast<T4 *>(p) = v;
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++) p[k] = v[k];
-    }
 }
 
 // Byte of (position t, channel d) in a tile; t and d multiples of 4 give a dword's first byte

@@ -218,13 +218,13 @@ extern "C" int sp_hip_fp8_cache_init(sp_hip_fp8_cache_t *c, const sp_config_t *c
     struct Piece {
         void **p;
         size_t bytes;
-        int fill;
+        int fill;  // -1: not cleared
     } pieces[] = {{&c->d_k_codes, ncode, 0}, {&c->d_v_codes, ncode, 0},
                   {&c->d_k_exp, nexp, 127 + SP_FP8_EMIN}, {&c->d_v_exp, nexp, 127 + SP_FP8_EMIN},
-                  {(void **)&pv->part, sp_fp8_workspace_floats(hd) * sizeof(float), 0},
+                  {(void **)&pv->part, (size_t)sp_fp8_part_rows(hd) * (hd + 2) * sizeof(float), -1},
                   {(void **)&pv->counters, SP_FP8_SLOTS * sizeof(int), 0}};
     for (const Piece &p : pieces)
-        good = good && ok(hipMalloc(p.p, p.bytes), who) && ok(hipMemsetAsync(*p.p, p.fill, p.bytes, s), who);
+        good = good && ok(hipMalloc(p.p, p.bytes), who) && (p.fill < 0 || ok(hipMemsetAsync(*p.p, p.fill, p.bytes, s), who));
     good = good && ok(hipStreamSynchronize(s), who);
     if (!good) {
         char why[256];

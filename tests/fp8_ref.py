@@ -105,14 +105,13 @@ class RefCache:
 
     def attend(self, layer, table, lens, row, n_rows, q, scale, window):
         """out [n_rows, n_q, hd], lse [n_rows, n_q], and the sums that bound a kernel's errors:
-        reach (the weights' mean of |v| and 2^-28 of its plain sum: weights below 2^-28 of the
-        largest are rounded at 2^-39 of that, as if they were as large) and steep (the largest
+        reach (the weights' mean of |v| in [0], its plain sum in [1]) and steep (the largest
         kq_scale * sum |q| |k| seen)."""
         n_q = q.shape[1]
         group = n_q // self.heads
         out = np.full((n_rows, n_q, self.hd), np.nan)
         lse = np.full((n_rows, n_q), np.nan)
-        reach = np.zeros((n_rows, n_q, self.hd))
+        reach = np.zeros((2, n_rows, n_q, self.hd))
         steep = np.zeros((n_rows, n_q))
         for i in range(len(lens)):
             r0, r1 = (row[i], row[i + 1]) if row is not None else (i, i + 1)
@@ -136,7 +135,8 @@ class RefCache:
                     t = w.sum(-1, keepdims=True)
                     sl = slice(h * group, (h + 1) * group)
                     out[r, sl] = w / t @ V[h][see]
-                    reach[r, sl] = w / t @ np.abs(V[h][see]) + 2.0 ** -28 * np.abs(V[h][see]).sum(0)
+                    reach[0, r, sl] = w / t @ np.abs(V[h][see])
+                    reach[1, r, sl] = np.abs(V[h][see]).sum(0)
                     lse[r, sl] = (m + np.log(t))[:, 0]
                     steep[r, sl] = (np.abs(qs) @ np.abs(K[h][see]).T).max(-1) * abs(scale)
         return out, lse, reach, steep
@@ -150,11 +150,14 @@ def bounds(dtype, hd, seen, out, reach, steep):
     and log2 e's own rounding), and with a split fp32 query 2^-22 more. Its weight: that, and
     2^-22 for the exponential and the running rescale. Sums of `seen` weights in fp32: seen 2^-24, a rescale
     for every 64. The product with V takes the weights rounded to fp16, 2^-11 (fp32: split, 2^-22),
-    and the result is rounded once to its type."""
+    and those of the smallest as if they were 2^-20 of the largest (fp16 numbers counted from 2^6
+    at the largest are normal down to 2^-14; split ones count from 2^14: 2^-28), and the result is
+    rounded once to its type."""
     half = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dtype]
     score = steep * ((hd + 4) * 2.0 ** -24 + (2.0 ** -22 if dtype == "f32" else 0.0))
     sums = (seen + seen / 16 + 64) * 2.0 ** -24 + 2.0 ** -22
     lse = score + sums + 2.0 ** -22
     w = 2 * (score + sums) + (2.0 ** -21 if dtype == "f32" else 2.0 ** -11)
     least = {"f32": 2.0 ** -149, "f16": 2.0 ** -25, "bf16": 2.0 ** -133}[dtype]
+    reach = reach[0] + (2.0 ** -28 if dtype == "f32" else 2.0 ** -20) * reach[1]
     return w[..., None] * reach + half * np.abs(out) + least, lse
