@@ -20,6 +20,8 @@
 // results, split in two. Sums, maxima and the running output are fp32. The running output counts in
 // units of the current V scale: when the scale or the maximum changes it is rescaled, and the
 // exponents' range (-40 to 40) keeps it finite.
+#include <type_traits>
+
 #include "sp_fp8.h"
 
 namespace {
@@ -52,11 +54,17 @@ __device__ __forceinline__ float column_sum(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
+// Results that all lanes agree on are taken into scalar registers (readfirstlane, readlane), so
+// that what follows from them is scalar too.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(float v) { return __int_as_float(uniform(__float_as_int(v))); }
+__device__ __forceinline__ unsigned uniform(unsigned v) { return (unsigned)uniform((int)v); }
+
 template <class T, class Op>
 __device__ __forceinline__ T wave_all(T v, Op op) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) v = op(v, __shfl_xor(v, d, 64));
-    return v;
+    return uniform(v);
 }
 
 // What one block of threads works on: `cols` columns from ct * cols of a sequence, one of
@@ -139,20 +147,21 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
         const unsigned long long past = __ballot(sum > item);
         if (past) {
             const int l = __ffsll(past) - 1;
+            const auto of = [l](int v) { return __builtin_amdgcn_readlane(v, l); };
             out.seq = i0 + l;
-            out.r0 = __shfl(e.a, l, 64);
-            out.n_new = __shfl(e.b, l, 64) - out.r0;
-            out.first = __shfl(e.len, l, 64) - out.n_new;
-            out.n_split = __shfl(ns, l, 64);
-            const int at = item - (__shfl(sum, l, 64) - __shfl(mine, l, 64));
+            out.r0 = of(e.a);
+            out.n_new = of(e.b) - out.r0;
+            out.first = of(e.len) - out.n_new;
+            out.n_split = of(ns);
+            const int at = item - (of(sum) - of(mine));
             // the last column group first: under the causal mask it sees most
-            out.ct = __shfl(e.ct, l, 64) - 1 - at / out.n_split;
+            out.ct = of(e.ct) - 1 - at / out.n_split;
             out.split = at % out.n_split;
-            out.slot = slots + __shfl(psum, l, 64) - __shfl(part, l, 64) + at;
+            out.slot = slots + of(psum) - of(part) + at;
             return true;
         }
-        item -= __shfl(sum, 63, 64);
-        slots += __shfl(psum, 63, 64);
+        item -= __builtin_amdgcn_readlane(sum, 63);
+        slots += __builtin_amdgcn_readlane(psum, 63);
     }
     return false;
 }
@@ -532,12 +541,18 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 // were made: lane (column, half)'s registers 8 k .. 8 k + 7 are positions
 // 16 k + 8 (j / 4) + 4 half + j % 4, and V's operand is laid out for that order.
 //
-// The running maximum is a reference that is raised only when a score passes it by 2^8 (the
-// weights then still fit fp16 with their 2^6 at the reference), so that the output is rescaled
-// a few times in a whole sequence and no exchange between lanes is needed in the others. Weights
-// below 2^-20 of the reference are subnormal fp16 numbers then, rounded at 2^-31 of it. Split
-// weights (fp32 results) count from 2^14 and their reference follows within a factor of two, so
-// that the second part keeps its bits.
+// The loop is pipelined by one cache block: the next block's scores go through the matrix cores
+// while this one's weights are computed, and the next one's maximum is taken during the product
+// with V, so that neither unit waits for the other.
+//
+// The running maximum is a reference that is raised only when a score passes it by 2^W_SLACK
+// (the weights, 2^W_TOP at the reference, then still fit fp16), so that the output is rescaled
+// a few times in a whole sequence and no exchange between lanes is needed in the others. The
+// output counts in units of the strongest V scale of late; a block whose scale is up to
+// 2^W_FOLD below has the difference taken off its weights' exponents, for nothing, and only
+// others rescale the output. In such a block weights below 2^-18 of the reference are subnormal
+// fp16 numbers, rounded at 2^-29 of it. Split weights (fp32 results) count from 2^14, their reference follows
+// within a factor of two and their unit always, so that the second part keeps its bits.
 typedef float f16x __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ f16x mma32(h8 a, h8 b, f16x c) {
@@ -554,12 +569,13 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     constexpr int COLS = 32 * NW, NS = HD / 16, ND = HD / 32, TILE = 64 * HD, ROW = HD + 2, NT = NW * 64, HT = NT / 2;
     constexpr bool SPLIT2 = DT == SP_DTYPE_F32;
     constexpr int NH = SPLIT2 ? 2 : 1;
-    constexpr float W_TOP = SPLIT2 ? 14.0f : 6.0f, W_SLACK = SPLIT2 ? 1.0f : 8.0f;
+    constexpr float W_TOP = SPLIT2 ? 14.0f : 12.0f, W_SLACK = SPLIT2 ? 1.0f : 3.0f;
+    constexpr int W_FOLD = SPLIT2 ? 0 : 8;
     constexpr int KP = (HD * 4 + HT - 1) / HT;  // K pieces of 16 codes a thread (half the threads)
     constexpr int VP = (HD * 2 + HT - 1) / HT;  // pairs of V pieces (the other half)
     constexpr int RAW = KP > 2 * VP ? KP : 2 * VP;
     typedef typename SpFp8Elem<DT>::T T;
-    extern __shared__ __align__(16) float smem[];  // two buffers of K and V, 64 * HD fp16 each
+    extern __shared__ __align__(16) float smem[];  // K, K, V, V: two buffers each, 64 * HD fp16
     __shared__ int last_flag;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.H;
@@ -574,27 +590,28 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     const int per = max((j1 - j0 + sh.n_split - 1) / sh.n_split, 0);
     const int t0 = j0 + sh.split * per, n = max(min(t0 + per, j1) - t0, 0);
 
-    int blk = -1, ekb = 0, evb = 0;  // lane k: block number and scale bytes of the (base + k)-th block
-    const auto look_up = [&](int base) {
-        blk = base + lane < n ? sp_fp8_block(A.s, sh.seq, t0 + base + lane) : -1;
-        const long long at = (long long)max(blk, 0) * A.H + h;
-        ekb = A.k.exps[at];
-        evb = A.v.exps[at];
-    };
-    struct Facts {  // of a block that is on its way
-        bool none;
+    // ---- where the blocks are: lane k of a window of 64 ----
+    int blk = -1, ekb = 0, evb = 0;
+    struct Facts {
+        int b;  // block number, -1: none
         int ek, ev;
     };
-    const auto facts = [&](int k) {
-        return Facts{__builtin_amdgcn_readlane(blk, k) < 0, sp_fp8_exponent(__builtin_amdgcn_readlane(ekb, k)),
-                     sp_fp8_exponent(__builtin_amdgcn_readlane(evb, k))};
+    const auto facts = [&](int k) {  // called with k = 0, 1, 2, ...
+        if ((k & 63) == 0) {
+            blk = k + lane < n ? sp_fp8_block(A.s, sh.seq, t0 + k + lane) : -1;
+            const long long at = (long long)max(blk, 0) * A.H + h;
+            ekb = A.k.exps[at];
+            evb = A.v.exps[at];
+        }
+        return Facts{__builtin_amdgcn_readlane(blk, k & 63), sp_fp8_exponent(__builtin_amdgcn_readlane(ekb, k & 63)),
+                     sp_fp8_exponent(__builtin_amdgcn_readlane(evb, k & 63))};
     };
-    // ---- staging: half of the threads bring K, half V ----
-    const bool stage_v = tid >= HT;
+    // ---- staging: half of the waves bring K, half V ----
+    const bool stage_v = w >= NW / 2;
     const int st = stage_v ? tid - HT : tid;
     u4 raw[RAW];
-    const auto fetch = [&](int k) {  // k: within the looked-up 64
-        const long long b = (long long)max(__builtin_amdgcn_readlane(blk, k), 0) * A.H + h;  // none: block 0, masked
+    const auto fetch = [&](int block) {
+        const long long b = (long long)max(block, 0) * A.H + h;  // none: block 0, masked
         if (!stage_v) {
             const uint8_t *p = A.k.codes + b * TILE;
 #pragma unroll
@@ -613,14 +630,14 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
             }
         }
     };
-    const auto stage = [&](int buf) {
-        h8 *kd = reinterpret_cast<h8 *>(smem) + buf * (2 * TILE / 8), *vd = kd + TILE / 8;
+    h8 *const kbuf = reinterpret_cast<h8 *>(smem), *const vbuf = kbuf + 2 * TILE / 8;
+    const auto stage = [&](int kb, int vb) {
         if (!stage_v) {
 #pragma unroll
             for (int i = 0; i < KP; i++) {
                 const int x = st + i * HT, g = (x >> 4) & 3, r = x & 15, uc = x >> 6;  // uc = u * HD/32 + c
                 if (KP * HT == HD * 4 || x < HD * 4) {
-                    h8 *d = kd + (uc * 2 + (g >> 1)) * 64 + (g & 1) * 32 + r;
+                    h8 *d = kbuf + kb * (TILE / 8) + (uc * 2 + (g >> 1)) * 64 + (g & 1) * 32 + r;
                     d[0] = to_half(raw[i][0], raw[i][1]);
                     d[16] = to_half(raw[i][2], raw[i][3]);
                 }
@@ -630,16 +647,17 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
             for (int i = 0; i < VP; i++) {
                 const int x = st + i * HT;
                 if (VP * HT == HD * 2 || x < HD * 2) {
-                    h8 *d = vd + (x >> 6) * 256 + (x & 63);
+                    h8 *d = vbuf + vb * (TILE / 8) + (x >> 6) * 256 + (x & 63);
 #pragma unroll
                     for (int t4 = 0; t4 < 4; t4++) d[t4 * 64] = to_half(raw[2 * i][t4], raw[2 * i + 1][t4]);
                 }
             }
         }
     };
+    Facts f0{-1, 0, 0}, f1{-1, 0, 0}, f2{-1, 0, 0};  // of blocks k, k + 1, k + 2
     if (n > 0) {
-        look_up(0);
-        fetch(0);
+        f0 = facts(0);
+        fetch(f0.b);
     }
 
     // ---- queries ----
@@ -650,7 +668,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     const long long row = (long long)sh.r0 + tk;
     const int pos = active ? sh.first + tk : -1;
     const int from = A.window > 0 ? pos - A.window : -1;  // sees (from, pos]
-    // of this wave's columns: whether there are any, and the range that each of them sees
+    // of this wave's columns: whether there are any, and their first and last position
     const bool busy = w * 32 < n_cols;
     const int wlast = min(w * 32 + 31, n_cols - 1);
     const int wpos0 = sh.first + (int)((c0 + w * 32) / A.G), wpos1 = sh.first + (int)((c0 + wlast) / A.G);
@@ -688,105 +706,181 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     f16x o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = f16x{};
-    float m = -INFINITY, off = 0.0f, l = 0.0f;  // off = W_TOP - m, 0 where m is -inf
+    // m: the reference; off = W_TOP - m, 0 while m is -inf; the output's unit is 2^ev_now
+    float m = -INFINITY, off = 0.0f, l = 0.0f;
     int ev_now = 0;
-    bool huge = false;  // a fused score - reference could be far above 0 where they should be equal
-    Facts now{true, 0, 0}, next{true, 0, 0};
-    if (n > 0) {
-        now = facts(0);
-        stage(0);
-        if (n > 1) {
-            fetch(1);
-            next = facts(1);
+    bool huge = false;  // the fused difference of a score and the reference would not be 0 where they are equal
+    // of the block whose weights come next: score scale, exponent offset, its part in l
+    float cs = 0.0f, shift = 0.0f, lmul = 1.0f;
+    h8 p[4][NH];
+
+    // next = K q^T of one block, and the weights p of the one before from its scores
+    const auto scores_weights = [&](auto with_scores, auto with_weights, const h8 *kd, f16x(&next)[2], const f16x(&s)[2]) {
+        float sum = 0.0f;
+        h8 a[2], b[2];  // K's operands are read one step ahead
+        if constexpr (decltype(with_scores)::value) {
+            a[0] = kd[0];
+            b[0] = kd[NS * 64];
         }
-    }
-    lds_barrier();
-    for (int k = 0; k < n; k++) {
-        const int t = t0 + k, ev = now.ev;
-        const h8 *kd = reinterpret_cast<const h8 *>(smem) + (k & 1) * (2 * TILE / 8) + lane, *vd = kd + TILE / 8;
-        const bool sees = busy && !now.none && t * 64 <= wpos1 && (A.window <= 0 || t * 64 + 63 > wpos0 - A.window);
-        h8 p[4][NH];
-        if (sees) {
-            f16x s[2];
-            s[0] = f16x{};
-            s[1] = f16x{};
 #pragma unroll
-            for (int c = 0; c < NS; c++) {
-                const h8 a = kd[c * 64], b = kd[(NS + c) * 64];
+        for (int c = 0; c < NS; c++) {
+            if constexpr (decltype(with_scores)::value) {
+                if (c + 1 < NS) {
+                    a[(c + 1) & 1] = kd[(c + 1) * 64];
+                    b[(c + 1) & 1] = kd[(NS + c + 1) * 64];
+                }
 #pragma unroll
                 for (int x = 0; x < NH; x++) {
-                    s[0] = mma32(a, q[c][x], s[0]);
-                    s[1] = mma32(b, q[c][x], s[1]);
+                    next[0] = mma32(a[c & 1], q[c][x], c || x ? next[0] : f16x{});
+                    next[1] = mma32(b[c & 1], q[c][x], c || x ? next[1] : f16x{});
                 }
             }
-            // never 0: a masked score stays -inf when it is multiplied
-            float cs = fmaxf(cscale * sp_fp8_pow2(now.ek), 0x1p-126f);
-            if (!(t * 64 + 63 <= wpos0 && (A.window <= 0 || t * 64 > wpos1 - A.window))) {
-                const int lane0 = t * 64 + 4 * half, upto = pos - lane0, before = from - lane0;
+            if constexpr (decltype(with_weights)::value) {
 #pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int at = u * 32 + (i >> 2) * 8 + (i & 3);
-                        s[u][i] = at <= upto && at > before ? s[u][i] : -INFINITY;
-                    }
+                for (int i = c * 16 / NS * 2; i < (c + 1) * 16 / NS * 2; i++) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], cs, shift));
+                    sum += x;
+                    const _Float16 hi = (_Float16)x;
+                    p[i >> 3][0][i & 7] = hi;
+                    if (SPLIT2) p[i >> 3][NH - 1][i & 7] = (_Float16)(x - (float)hi);
+                }
             }
-            float top = s[0][0];
-#pragma unroll
-            for (int i = 1; i < 32; i++) top = fmaxf(top, s[i >> 4][i & 15]);
-            const bool raise = m == -INFINITY ? top > -INFINITY : __builtin_fmaf(top, cs, off) > W_TOP + W_SLACK;
-            float f = sp_fp8_pow2(ev_now - ev);
-            ev_now = ev;
-            bool rescale = f != 1.0f;
-            if (__any(raise)) {
-                const float mx = fmaxf(top, __shfl_xor(top, 32, 64)) * cs, m_new = fmaxf(m, mx);
-                const float alpha = weight(m, m_new);
-                l *= alpha;
-                f *= alpha;
-                m = m_new;
-                off = m == -INFINITY ? 0.0f : W_TOP - m;
-                rescale = true;
-                huge = __any(fabsf(m) > 0x1p18f && m > -INFINITY);
-            }
-            if (huge) {  // the reference was rounded: round the scores as it was
-#pragma unroll
-                for (int i = 0; i < 32; i++) s[i >> 4][i & 15] *= cs;
-                cs = 1.0f;
-            }
-            if (rescale) {
-#pragma unroll
-                for (int d = 0; d < ND; d++) o[d] *= f;
-            }
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 32; i++) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], cs, off));
-                sum += x;
-                const _Float16 hi = (_Float16)x;
-                p[i >> 3][0][i & 7] = hi;
-                if (SPLIT2) p[i >> 3][NH - 1][i & 7] = (_Float16)(x - (float)hi);
-            }
-            l += sum;
         }
-        if (k + 1 < n) stage((k + 1) & 1);
-        if (sees) {
+        if constexpr (decltype(with_weights)::value) l += sum * lmul;
+    };
+    const auto mask = [&](const Facts &f, int k, f16x(&s)[2]) {
+        const int t = t0 + k;
+        if (f.b >= 0 && t * 64 + 63 <= wpos0 && (A.window <= 0 || t * 64 > wpos1 - A.window)) return;
+        const int lane0 = t * 64 + 4 * half, upto = f.b < 0 ? -1 : pos - lane0, before = from - lane0;
 #pragma unroll
-            for (int t4 = 0; t4 < 4; t4++)
+        for (int i = 0; i < 32; i++) {
+            const int at = (i >> 4) * 32 + ((i & 15) >> 2) * 8 + (i & 3);
+            s[i >> 4][i & 15] = at <= upto && at > before ? s[i >> 4][i & 15] : -INFINITY;
+        }
+    };
+    // out^T += V^T p^T of one block, and the largest score of the next
+    const auto values_top = [&](auto with_values, auto with_top, const h8 *vd, const f16x(&s)[2]) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int t4 = 0; t4 < 4; t4++) {
+            if constexpr (decltype(with_values)::value) {
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
                     const h8 a = vd[(d * 4 + t4) * 64];
 #pragma unroll
                     for (int x = 0; x < NH; x++) o[d] = mma32(a, p[t4][x], o[d]);
                 }
+            }
+            if constexpr (decltype(with_top)::value) {
+#pragma unroll
+                for (int i = t4 * 8; i < t4 * 8 + 8; i++) top = fmaxf(top, s[i >> 4][i & 15]);
+            }
         }
-        now = next;
-        if (k + 2 < n) {
-            if (((k + 2) & 63) == 0) look_up(k + 2);
-            fetch((k + 2) & 63);
-            next = facts((k + 2) & 63);
+        return top;
+    };
+    // the reference and the output's unit for a block with largest score `top` (this lane's)
+    const auto settle = [&](const Facts &f, float top, f16x(&s)[2]) {
+        // never 0: a masked score stays -inf when it is multiplied
+        cs = fmaxf(cscale * sp_fp8_pow2(f.ek), 0x1p-126f);
+        const bool raise = m == -INFINITY ? top > -INFINITY : __builtin_fmaf(top, cs, off) > W_TOP + W_SLACK;
+        float scale = 1.0f;
+        bool rescale = false;
+        if (f.ev > ev_now || f.ev < ev_now - W_FOLD) {
+            scale = sp_fp8_pow2(ev_now - f.ev);
+            ev_now = f.ev;
+            rescale = true;
         }
-        lds_barrier();
+        if (__any(raise)) {
+            const float mx = fmaxf(top, __shfl_xor(top, 32, 64)) * cs, m_new = fmaxf(m, mx);
+            const float alpha = weight(m, m_new);
+            l *= alpha;
+            scale *= alpha;
+            m = m_new;
+            off = m == -INFINITY ? 0.0f : W_TOP - m;
+            rescale = true;
+            huge = __any(fabsf(m) > 0x1p18f && m > -INFINITY);
+        }
+        if (huge) {  // the reference was rounded: round the scores as it was
+#pragma unroll
+            for (int i = 0; i < 32; i++) s[i >> 4][i & 15] *= cs;
+            cs = 1.0f;
+        }
+        if (rescale) {
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= scale;
+        }
+        shift = off + (float)(f.ev - ev_now);
+        lmul = sp_fp8_pow2(ev_now - f.ev);
+    };
+    const std::true_type yes;
+    const std::false_type no;
+
+    // ---- block 0's scores; K one block ahead of V from here ----
+    // Blocks past the last are fetched as block 0 and never used: no turn asks for its place.
+    f16x sa[2], sb[2];
+    if (n > 0) {
+        stage(0, 0);
+        f1 = facts(1);
+        f2 = facts(2);
+        fetch(f1.b);
     }
+    lds_barrier();
+    if (n > 0) {
+        if (busy) {
+            scores_weights(yes, no, kbuf + lane, sa, sa);
+            mask(f0, 0, sa);
+            ev_now = f0.ev;
+            settle(f0, values_top(no, yes, nullptr, sa), sa);
+        }
+        if (!stage_v) {
+            stage(1, 0);
+            fetch(f2.b);
+        }
+    }
+    lds_barrier();
+    // here: K of block k + 1 and V of block k are in LDS; registers hold K of k + 2 or V of k + 1
+    const auto bring = [&](int k, int buf) {
+        stage(buf, 1 - buf);
+        const Facts f3 = facts(k + 3);
+        fetch(stage_v ? f2.b : f3.b);
+        f1 = f2;
+        f2 = f3;
+    };
+    const auto turn = [&](int k, auto odd, f16x(&s)[2], f16x(&next)[2]) {
+        constexpr int B = decltype(odd)::value;
+        const Facts f = f1;
+        scores_weights(yes, yes, kbuf + (1 - B) * (TILE / 8) + lane, next, s);
+        bring(k, B);
+        mask(f, k + 1, next);
+        const float top = values_top(yes, yes, vbuf + B * (TILE / 8) + lane, next);
+        settle(f, top, next);
+        lds_barrier();
+    };
+    const std::integral_constant<int, 0> even;
+    const std::integral_constant<int, 1> odd;
+    if (busy) {
+        int k = 0;
+        for (; k + 2 < n; k += 2) {
+            turn(k, even, sa, sb);
+            turn(k + 1, odd, sb, sa);
+        }
+        if (k + 1 < n) {
+            turn(k, even, sa, sb);
+            sa[0] = sb[0];
+            sa[1] = sb[1];
+            k++;
+        }
+        if (k < n) {  // the last one: no more scores
+            scores_weights(no, yes, nullptr, sa, sa);
+            values_top(yes, no, vbuf + (k & 1) * (TILE / 8) + lane, sa);
+        }
+    } else {  // no columns: bring blocks for the other waves
+        for (int k = 0; k + 1 < n; k++) {
+            bring(k, k & 1);
+            lds_barrier();
+        }
+    }
+    lds_barrier();
     l += __shfl_xor(l, 32, 64);
 
     // ---- results ----

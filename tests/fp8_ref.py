@@ -150,14 +150,14 @@ def bounds(dtype, hd, seen, out, reach, steep):
     and log2 e's own rounding), and with a split fp32 query 2^-22 more. Its weight: that, and
     2^-22 for the exponential and the running rescale. Sums of `seen` weights in fp32: seen 2^-24, a rescale
     for every 64. The product with V takes the weights rounded to fp16, 2^-11 (fp32: split, 2^-22),
-    and those of the smallest as if they were 2^-20 of the largest (fp16 numbers counted from 2^6
-    at the largest are normal down to 2^-14; split ones count from 2^14: 2^-28), and the result is
-    rounded once to its type."""
+    and those of the smallest as if they were 2^-18 of the largest (fp16 numbers are normal down to
+    2^-14 and count from 2^12 at the largest, from 2^4 in a block whose V scale is 2^8 below
+    another's; split ones count from 2^14: 2^-28), and the result is rounded once to its type."""
     half = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dtype]
     score = steep * ((hd + 4) * 2.0 ** -24 + (2.0 ** -22 if dtype == "f32" else 0.0))
     sums = (seen + seen / 16 + 64) * 2.0 ** -24 + 2.0 ** -22
     lse = score + sums + 2.0 ** -22
     w = 2 * (score + sums) + (2.0 ** -21 if dtype == "f32" else 2.0 ** -11)
     least = {"f32": 2.0 ** -149, "f16": 2.0 ** -25, "bf16": 2.0 ** -133}[dtype]
-    reach = reach[0] + (2.0 ** -28 if dtype == "f32" else 2.0 ** -20) * reach[1]
+    reach = reach[0] + (2.0 ** -28 if dtype == "f32" else 2.0 ** -18) * reach[1]
     return w[..., None] * reach + half * np.abs(out) + least, lse
