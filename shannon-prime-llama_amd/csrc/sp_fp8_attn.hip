@@ -575,7 +575,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     constexpr int VP = (HD * 2 + HT - 1) / HT;  // pairs of V pieces (the other half)
     constexpr int RAW = KP > 2 * VP ? KP : 2 * VP;
     typedef typename SpFp8Elem<DT>::T T;
-    extern __shared__ __align__(16) float smem[];  // K, K, V, V: two buffers each, 64 * HD fp16
+    extern __shared__ __align__(16) float smem[];  // K, K, V, V: two places each, 64 * HD fp16
     __shared__ int last_flag;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.H;
@@ -596,7 +596,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
         int b;  // block number, -1: none
         int ek, ev;
     };
-    const auto facts = [&](int k) {  // called with k = 0, 1, 2, ...
+    const auto facts = [&](int k) __attribute__((always_inline)) {  // called with k = 0, 1, 2, ...
         if ((k & 63) == 0) {
             blk = k + lane < n ? sp_fp8_block(A.s, sh.seq, t0 + k + lane) : -1;
             const long long at = (long long)max(blk, 0) * A.H + h;
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     const bool stage_v = w >= NW / 2;
     const int st = stage_v ? tid - HT : tid;
     u4 raw[RAW];
-    const auto fetch = [&](int block) {
+    const auto fetch = [&](int block) __attribute__((always_inline)) {
         const long long b = (long long)max(block, 0) * A.H + h;  // none: block 0, masked
         if (!stage_v) {
             const uint8_t *p = A.k.codes + b * TILE;
@@ -631,7 +631,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
         }
     };
     h8 *const kbuf = reinterpret_cast<h8 *>(smem), *const vbuf = kbuf + 2 * TILE / 8;
-    const auto stage = [&](int kb, int vb) {
+    const auto stage = [&](int kb, int vb) __attribute__((always_inline)) {
         if (!stage_v) {
 #pragma unroll
             for (int i = 0; i < KP; i++) {
@@ -714,25 +714,36 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     float cs = 0.0f, shift = 0.0f, lmul = 1.0f;
     h8 p[4][NH];
 
-    // next = K q^T of one block, and the weights p of the one before from its scores
-    const auto scores_weights = [&](auto with_scores, auto with_weights, const h8 *kd, f16x(&next)[2], const f16x(&s)[2]) {
+    // next = K q^T of one block; of the one before, the weights from its scores and, sixteen
+    // positions at a time, out^T += V^T p^T (the last sixteen: product, afterwards).
+    const auto product = [&](auto group, const h8 *vd) __attribute__((always_inline)) {
+        constexpr int t4 = decltype(group)::value;
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            const h8 a = vd[(d * 4 + t4) * 64];
+#pragma unroll
+            for (int x = 0; x < NH; x++) o[d] = mma32(a, p[t4][x], o[d]);
+        }
+    };
+    const auto blend = [&](auto with_scores, auto with_weights, const h8 *kd, const h8 *vd, f16x(&next)[2],
+                           const f16x(&s)[2]) __attribute__((always_inline)) {
         float sum = 0.0f;
-        h8 a[2], b[2];  // K's operands are read one step ahead
+        h8 ka[2], kb[2];  // K's operands, read one step ahead
         if constexpr (decltype(with_scores)::value) {
-            a[0] = kd[0];
-            b[0] = kd[NS * 64];
+            ka[0] = kd[0];
+            kb[0] = kd[NS * 64];
         }
 #pragma unroll
         for (int c = 0; c < NS; c++) {
             if constexpr (decltype(with_scores)::value) {
                 if (c + 1 < NS) {
-                    a[(c + 1) & 1] = kd[(c + 1) * 64];
-                    b[(c + 1) & 1] = kd[(NS + c + 1) * 64];
+                    ka[(c + 1) & 1] = kd[(c + 1) * 64];
+                    kb[(c + 1) & 1] = kd[(NS + c + 1) * 64];
                 }
 #pragma unroll
                 for (int x = 0; x < NH; x++) {
-                    next[0] = mma32(a[c & 1], q[c][x], c || x ? next[0] : f16x{});
-                    next[1] = mma32(b[c & 1], q[c][x], c || x ? next[1] : f16x{});
+                    next[0] = mma32(ka[c & 1], q[c][x], c || x ? next[0] : f16x{});
+                    next[1] = mma32(kb[c & 1], q[c][x], c || x ? next[1] : f16x{});
                 }
             }
             if constexpr (decltype(with_weights)::value) {
@@ -744,11 +755,18 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
                     p[i >> 3][0][i & 7] = hi;
                     if (SPLIT2) p[i >> 3][NH - 1][i & 7] = (_Float16)(x - (float)hi);
                 }
+                // the sixteens whose weights were complete a step ago
+                const int done = c * 16 / NS * 2 / 8, before = c ? (c - 1) * 16 / NS * 2 / 8 : 0;
+                if (done > before) {
+                    if (done == 1) product(std::integral_constant<int, 0>(), vd);
+                    if (done == 2) product(std::integral_constant<int, 1>(), vd);
+                    if (done == 3) product(std::integral_constant<int, 2>(), vd);
+                }
             }
         }
         if constexpr (decltype(with_weights)::value) l += sum * lmul;
     };
-    const auto mask = [&](const Facts &f, int k, f16x(&s)[2]) {
+    const auto mask = [&](const Facts &f, int k, f16x(&s)[2]) __attribute__((always_inline)) {
         const int t = t0 + k;
         if (f.b >= 0 && t * 64 + 63 <= wpos0 && (A.window <= 0 || t * 64 > wpos1 - A.window)) return;
         const int lane0 = t * 64 + 4 * half, upto = f.b < 0 ? -1 : pos - lane0, before = from - lane0;
@@ -758,28 +776,14 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
             s[i >> 4][i & 15] = at <= upto && at > before ? s[i >> 4][i & 15] : -INFINITY;
         }
     };
-    // out^T += V^T p^T of one block, and the largest score of the next
-    const auto values_top = [&](auto with_values, auto with_top, const h8 *vd, const f16x(&s)[2]) {
-        float top = -INFINITY;
+    const auto largest = [&](const f16x(&s)[2]) __attribute__((always_inline)) {
+        float top = s[0][0];
 #pragma unroll
-        for (int t4 = 0; t4 < 4; t4++) {
-            if constexpr (decltype(with_values)::value) {
-#pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    const h8 a = vd[(d * 4 + t4) * 64];
-#pragma unroll
-                    for (int x = 0; x < NH; x++) o[d] = mma32(a, p[t4][x], o[d]);
-                }
-            }
-            if constexpr (decltype(with_top)::value) {
-#pragma unroll
-                for (int i = t4 * 8; i < t4 * 8 + 8; i++) top = fmaxf(top, s[i >> 4][i & 15]);
-            }
-        }
+        for (int i = 1; i < 32; i++) top = fmaxf(top, s[i >> 4][i & 15]);
         return top;
     };
     // the reference and the output's unit for a block with largest score `top` (this lane's)
-    const auto settle = [&](const Facts &f, float top, f16x(&s)[2]) {
+    const auto settle = [&](const Facts &f, float top, f16x(&s)[2]) __attribute__((always_inline)) {
         // never 0: a masked score stays -inf when it is multiplied
         cs = fmaxf(cscale * sp_fp8_pow2(f.ek), 0x1p-126f);
         const bool raise = m == -INFINITY ? top > -INFINITY : __builtin_fmaf(top, cs, off) > W_TOP + W_SLACK;
@@ -814,9 +818,11 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     };
     const std::true_type yes;
     const std::false_type no;
+    const std::integral_constant<int, 3> last16;
 
     // ---- block 0's scores; K one block ahead of V from here ----
     // Blocks past the last are fetched as block 0 and never used: no turn asks for its place.
+    constexpr int STEP = TILE / 8;
     f16x sa[2], sb[2];
     if (n > 0) {
         stage(0, 0);
@@ -827,10 +833,10 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     lds_barrier();
     if (n > 0) {
         if (busy) {
-            scores_weights(yes, no, kbuf + lane, sa, sa);
+            blend(yes, no, kbuf + lane, nullptr, sa, sa);
             mask(f0, 0, sa);
             ev_now = f0.ev;
-            settle(f0, values_top(no, yes, nullptr, sa), sa);
+            settle(f0, largest(sa), sa);
         }
         if (!stage_v) {
             stage(1, 0);
@@ -838,45 +844,44 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
         }
     }
     lds_barrier();
-    // here: K of block k + 1 and V of block k are in LDS; registers hold K of k + 2 or V of k + 1
-    const auto bring = [&](int k, int buf) {
-        stage(buf, 1 - buf);
+    // at turn k: K of block k + 1 and V of block k are in LDS, registers hold K of k + 2 or V of k + 1
+    const auto bring = [&](int k) __attribute__((always_inline)) {
+        stage(k & 1, 1 - (k & 1));
         const Facts f3 = facts(k + 3);
         fetch(stage_v ? f2.b : f3.b);
         f1 = f2;
         f2 = f3;
     };
-    const auto turn = [&](int k, auto odd, f16x(&s)[2], f16x(&next)[2]) {
-        constexpr int B = decltype(odd)::value;
+    const auto turn = [&](int k, f16x(&s)[2], f16x(&next)[2]) __attribute__((always_inline)) {
         const Facts f = f1;
-        scores_weights(yes, yes, kbuf + (1 - B) * (TILE / 8) + lane, next, s);
-        bring(k, B);
+        const h8 *vd = vbuf + (k & 1) * STEP + lane;
+        blend(yes, yes, kbuf + (1 - (k & 1)) * STEP + lane, vd, next, s);
+        bring(k);
+        product(last16, vd);
         mask(f, k + 1, next);
-        const float top = values_top(yes, yes, vbuf + B * (TILE / 8) + lane, next);
-        settle(f, top, next);
+        settle(f, largest(next), next);
         lds_barrier();
     };
-    const std::integral_constant<int, 0> even;
-    const std::integral_constant<int, 1> odd;
     if (busy) {
         int k = 0;
         for (; k + 2 < n; k += 2) {
-            turn(k, even, sa, sb);
-            turn(k + 1, odd, sb, sa);
+            turn(k, sa, sb);
+            turn(k + 1, sb, sa);
         }
         if (k + 1 < n) {
-            turn(k, even, sa, sb);
+            turn(k, sa, sb);
             sa[0] = sb[0];
             sa[1] = sb[1];
             k++;
         }
         if (k < n) {  // the last one: no more scores
-            scores_weights(no, yes, nullptr, sa, sa);
-            values_top(yes, no, vbuf + (k & 1) * (TILE / 8) + lane, sa);
+            const h8 *vd = vbuf + (k & 1) * STEP + lane;
+            blend(no, yes, nullptr, vd, sa, sa);
+            product(last16, vd);
         }
     } else {  // no columns: bring blocks for the other waves
         for (int k = 0; k + 1 < n; k++) {
-            bring(k, k & 1);
+            bring(k);
             lds_barrier();
         }
     }
