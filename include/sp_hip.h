@@ -467,8 +467,9 @@ typedef struct {
  *
  * Row r of sequence i (d_row[i] <= r < d_row[i + 1]) is its position
  * d_len[i] - d_row[i + 1] + r: the call's rows are the sequence's newest positions, and
- * d_len counts them. d_row ascends and d_row[n_seq] <= n_rows; rows that no sequence has are
- * neither read nor written. Without d_row sequence i has the one row i (n_rows = n_seq).
+ * d_len counts them. d_row ascends from at least 0 and d_row[n_seq] <= n_rows (where it does
+ * not, attention does nothing, and write and read stay within the call's rows); rows that no
+ * sequence has are neither read nor written. Without d_row sequence i has the one row i (n_rows = n_seq).
  *
  * A position is in the cache if it is not negative and its table entry exists and lies in
  * [0, n_blocks). Others (a length past the table, an entry of -1) are never accessed: write

@@ -97,14 +97,16 @@ __device__ __forceinline__ int sp_fp8_block(const SpFp8Seqs &S, int seq, int j) 
 // The exponent that a byte of the cache stands for; one that no write made counts as the nearest.
 __device__ __forceinline__ int sp_fp8_exponent(int b) { return min(max(b - 127, SP_FP8_EMIN), SP_FP8_EMAX); }
 
-// Inclusive sum over the lanes of a wave.
+// Inclusive sum over the lanes of a wave (every lane active): shifts inside the rows of 16, then
+// the rows' sums through scalar registers.
 __device__ __forceinline__ int sp_fp8_scan(int v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int t = __shfl_up(v, d, 64);
-        v += lane >= d ? t : 0;
-    }
-    return v;
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    const int a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31),
+              c = b + __builtin_amdgcn_readlane(v, 47);
+    return v + (lane < 16 ? 0 : lane < 32 ? a : lane < 48 ? b : c);
 }
 
 template <int DT>

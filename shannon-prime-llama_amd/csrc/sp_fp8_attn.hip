@@ -22,6 +22,7 @@
 // exponents' range (-40 to 40) keeps it finite.
 #include <type_traits>
 
+#include "sp_device.h"
 #include "sp_fp8.h"
 
 namespace {
@@ -58,14 +59,8 @@ __device__ __forceinline__ float column_sum(float v) {
 // that what follows from them is scalar too.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ float uniform(float v) { return __int_as_float(uniform(__float_as_int(v))); }
-__device__ __forceinline__ unsigned uniform(unsigned v) { return (unsigned)uniform((int)v); }
 
-template <class T, class Op>
-__device__ __forceinline__ T wave_all(T v, Op op) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = op(v, __shfl_xor(v, d, 64));
-    return uniform(v);
-}
+__device__ __forceinline__ float wave_sum(float v) { return uniform(sp_wave_sum_dpp(v)); }
 
 // What one block of threads works on: `cols` columns from ct * cols of a sequence, one of
 // n_split shares of the cache blocks that they see.
@@ -78,11 +73,13 @@ struct Share {
 // A sequence's rows, length, column groups and the cache blocks that its rows see.
 struct Extent {
     int a, b, len, ct, nb;
+    bool bad;  // d_row does not ascend here, or leaves the call's rows
 };
 __device__ __forceinline__ Extent extent(const SpFp8Attn &A, int i, int cols) {
-    Extent e{0, 0, 0, 0, 0};
+    Extent e{0, 0, 0, 0, 0, false};
     if (i < A.s.n_seq) {
         sp_fp8_seq(A.s, i, e.a, e.b, e.len);
+        e.bad = A.s.row && (A.s.row[i] != e.a || A.s.row[i + 1] != e.b);
         const int lo = A.window > 0 ? max(e.len - (e.b - e.a) - A.window + 1, 0) >> 6 : 0;
         e.nb = max(min((e.len + 63) >> 6, A.s.stride) - lo, 0);
         e.ct = (int)(((long long)(e.b - e.a) * A.G + cols - 1) / cols);
@@ -90,21 +87,19 @@ __device__ __forceinline__ Extent extent(const SpFp8Attn &A, int i, int cols) {
     return e;
 }
 __device__ __forceinline__ int shares_of(int nb, int R, int least) {
-    return nb <= 2 * least ? 1 : (nb + R - 1) / R;
+    return nb <= 4 * least ? 1 : (nb + R - 1) / R;
 }
 
 // The work is divided on the device, so that lengths may change under a captured call. With T
 // the blocks that all column groups see, a column group of n blocks gets ceil(n / R) shares,
 // R the first of R0, 5/4 R0, 3/2 R0 and 2 R0, R0 > T / target, that makes at most `target`
-// shares, if one does. R is at least `least`, one block a wave, and two blocks a wave are not
-// shared out: a share's own waves join their results in LDS, which costs far less than the
-// stores, the count and the loads (three memory latencies) that join shares. Groups of two or more shares (n > R, so
+// shares, if one does. R is at least `least`, and up to four times that is not shared out: a
+// share's own waves join their results in LDS, which costs less than the stores, the count and
+// the loads (three memory latencies) that join shares. Groups of two or more shares (n > R, so
 // ceil(n / R) < 2 n / R) have at most 2 T / R < 2 target shares, which bounds the partial
 // results.
 __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lane, int cols, int least, Share &out) {
     const int n_seq = A.s.n_seq;
-    const auto fadd = [](float x, float y) { return x + y; };
-    const auto sat = [](unsigned x, unsigned y) { return min(x + y, 0x7fffffffu); };  // each at most 2^31 - 1
     if (n_seq == 1) {  // nothing to search, and no exchange between lanes
         const Extent e = extent(A, 0, cols);
         const float T = (float)e.ct * (float)e.nb * (float)A.H;
@@ -116,18 +111,18 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
         }
         const int ns = shares_of(e.nb, R, least);
         out = Share{0, e.a, e.b - e.a, e.len - (e.b - e.a), e.ct - 1 - item / ns, item % ns, ns, item};
-        return item < e.ct * ns;
+        return !e.bad && item < e.ct * ns;
     }
     const Extent e0 = extent(A, lane, cols);  // kept: up to 64 sequences are read once
     float T = (float)e0.ct * (float)e0.nb;
-    unsigned rows = (unsigned)(e0.b - e0.a);
+    bool bad = e0.bad;
     for (int i0 = 64; i0 < n_seq; i0 += 64) {
         const Extent e = extent(A, i0 + lane, cols);
         T += (float)e.ct * (float)e.nb;
-        rows = sat(rows, (unsigned)(e.b - e.a));
+        bad = bad || e.bad;
     }
-    T = wave_all(T, fadd) * (float)A.H;
-    if (A.s.row && wave_all(rows, sat) > (unsigned)A.s.n_rows) return false;  // d_row does not ascend
+    if (__any(bad)) return false;  // the grid was made for rows that ascend
+    T = wave_sum(T) * (float)A.H;
     const int R0 = max((int)(T / (float)A.target * 1.002f) + 1, least);
     float n[3] = {0.0f, 0.0f, 0.0f};
     for (int i0 = 0; i0 < n_seq; i0 += 64) {
@@ -138,7 +133,7 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
     int R = 2 * R0;
 #pragma unroll
     for (int k = 2; k >= 0; k--)
-        if (wave_all(n[k], fadd) * (float)A.H <= (float)A.target) R = R0 + k * R0 / 4;
+        if (wave_sum(n[k]) * (float)A.H <= (float)A.target) R = R0 + k * R0 / 4;
     int slots = 0;
     for (int i0 = 0; i0 < n_seq; i0 += 64) {
         const Extent e = i0 ? extent(A, i0 + lane, cols) : e0;
@@ -303,7 +298,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.H;
     Share sh;
-    if (!find_share(A, blockIdx.x / A.H, lane, COLS, NW, sh)) return;
+    if (!find_share(A, blockIdx.x / A.H, lane, COLS, NW / 2, sh)) return;
     const int n_cols = (int)min((long long)sh.n_new * A.G - (long long)sh.ct * COLS, (long long)COLS);
     const int col = lane & 15, g = lane >> 4;
     const long long c0 = (long long)sh.ct * COLS;
@@ -580,7 +575,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.H;
     Share sh;
-    if (!find_share(A, blockIdx.x / A.H, lane, COLS, 8, sh)) return;
+    if (!find_share(A, blockIdx.x / A.H, lane, COLS, 4, sh)) return;
     const int n_cols = (int)min((long long)sh.n_new * A.G - (long long)sh.ct * COLS, (long long)COLS);
     const int col = lane & 31, half = lane >> 5;
     const long long c0 = (long long)sh.ct * COLS;

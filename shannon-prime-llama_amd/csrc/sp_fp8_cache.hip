@@ -21,9 +21,18 @@ using sp_fp8::load4;
 using sp_fp8::store4;
 
 // The (sequence, cache block) pair of a grid index: sequence, block index in the sequence and
-// the call's rows of it. False: no such pair. Every lane of a wave agrees.
+// the call's rows of it. False: no such pair. Every lane of a wave agrees, in scalar registers.
 __device__ __forceinline__ bool pair_of(const SpFp8Seqs &S, int p, int lane, int &seq, int &j, int &r0, int &first,
                                         int &last) {
+    if (!S.row || S.n_seq == 1) {  // nothing to search
+        seq = S.row ? 0 : p;
+        int r1, len;
+        sp_fp8_seq(S, seq, r0, r1, len);
+        first = len - (r1 - r0);
+        last = len - 1;
+        j = sp_fp8_floor64(first) + (S.row ? p : 0);
+        return r1 > r0 && j <= sp_fp8_floor64(last);
+    }
     for (int i0 = 0; i0 < S.n_seq; i0 += 64) {
         const int i = i0 + lane;
         int a = 0, b = 0, len = 0, n = 0;
@@ -35,15 +44,15 @@ __device__ __forceinline__ bool pair_of(const SpFp8Seqs &S, int p, int lane, int
         const unsigned long long past = __ballot(sum > p);
         if (past) {
             const int l = __ffsll(past) - 1;
+            const auto of = [l](int v) { return __builtin_amdgcn_readlane(v, l); };
             seq = i0 + l;
-            r0 = __shfl(a, l, 64);
-            const int r1 = __shfl(b, l, 64), ln = __shfl(len, l, 64);
-            first = ln - (r1 - r0);
-            last = ln - 1;
-            j = sp_fp8_floor64(first) + p - (__shfl(sum, l, 64) - __shfl(n, l, 64));
+            r0 = of(a);
+            first = of(len) - (of(b) - r0);
+            last = of(len) - 1;
+            j = sp_fp8_floor64(first) + p - (of(sum) - of(n));
             return true;
         }
-        p -= __shfl(sum, 63, 64);
+        p -= __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
 }
@@ -89,15 +98,11 @@ __global__ __launch_bounds__(NT) void k_fp8_write(SpFp8Copy A) {
     if (!side.codes) return;
     int seq, j, r0, first, last;
     if (!pair_of(A.s, blockIdx.x, lane, seq, j, r0, first, last)) return;
-    const int blk = sp_fp8_block(A.s, seq, j);
-    if (blk < 0) return;
     // the call's positions in this cache block: [lo, hi) of its 64
     const int lo = max(first - j * 64, 0), hi = min(last + 1 - j * 64, 64);
     const void *rows = A.rows[is_v];
     // row of position 0 of the block
     const long long row0 = (long long)r0 + ((long long)j * 64 - first);
-    uint8_t *exp_at = side.exps + (long long)blk * A.H + h;
-    const int e_old = lo > 0 ? sp_fp8_exponent(*exp_at) : SP_FP8_EMIN;
     f4 x[PER][4];
     float m = 0.0f;
     const float top = SP_FP8_MAX * 0x1p40f;
@@ -112,6 +117,10 @@ __global__ __launch_bounds__(NT) void k_fp8_write(SpFp8Copy A) {
                 x[k][i] = load4<DT>(rows, (row0 + t) * A.row_stride + (long long)h * HD + d, A.aligned);
         }
     }
+    const int blk = sp_fp8_block(A.s, seq, j);  // while the rows are on their way
+    if (blk < 0) return;
+    uint8_t *exp_at = side.exps + (long long)blk * A.H + h;
+    const int e_old = lo > 0 ? sp_fp8_exponent(*exp_at) : SP_FP8_EMIN;
 #pragma unroll
     for (int k = 0; k < PER; k++)
 #pragma unroll
@@ -188,6 +197,9 @@ __global__ __launch_bounds__(NT) void k_fp8_write(SpFp8Copy A) {
                 const int t = quad * 4 + i;
                 if (t >= lo && t < hi) *reinterpret_cast<unsigned *>(dst + k_byte<HD>(t, d)) = w[i];
             }
+        } else if (quad * 4 >= lo && quad * 4 + 4 <= hi) {
+#pragma unroll
+            for (int n = 0; n < 4; n++) *reinterpret_cast<unsigned *>(dst + v_byte(quad * 4, d + n)) = w[n];
         } else {
 #pragma unroll
             for (int n = 0; n < 4; n++)
