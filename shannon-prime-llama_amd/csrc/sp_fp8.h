@@ -59,9 +59,10 @@ struct SpFp8Attn {
     int window;
     float c;   // kq_scale * log2(e), not negative
     int negate;
-    float *part;    // partial results: sp_fp8_part_rows(hd) rows of hd + 2 floats
+    float *part;    // partial results: sp_fp8_part_rows(hd) rows of hd + 4 floats
     int *counters;  // SP_FP8_SLOTS, one per partial result, zero between calls
     int target;     // CUs; the launch makes it the blocks that fill them
+    int least;      // fewest cache blocks of a share (the launch's choice)
 };
 
 hipError_t sp_fp8_launch_write(const SpFp8Copy &A, int hd, int dtype, hipStream_t s);

@@ -82,7 +82,7 @@ __device__ __forceinline__ Extent extent(const SpFp8Attn &A, int i, int cols) {
         e.bad = A.s.row && (A.s.row[i] != e.a || A.s.row[i + 1] != e.b);
         const int lo = A.window > 0 ? max(e.len - (e.b - e.a) - A.window + 1, 0) >> 6 : 0;
         e.nb = max(min((e.len + 63) >> 6, A.s.stride) - lo, 0);
-        e.ct = (int)(((long long)(e.b - e.a) * A.G + cols - 1) / cols);
+        e.ct = ((e.b - e.a) * A.G + cols - 1) / cols;
     }
     return e;
 }
@@ -97,8 +97,9 @@ __device__ __forceinline__ int shares_of(int nb, int R, int least) {
 // share's own waves join their results in LDS, which costs less than the stores, the count and
 // the loads (three memory latencies) that join shares. Groups of two or more shares (n > R, so
 // ceil(n / R) < 2 n / R) have at most 2 T / R < 2 target shares, which bounds the partial
-// results.
-__device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lane, int cols, int least, Share &out) {
+// results. by_group: `item` counts column groups, and their first shares are found.
+__device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lane, int cols, int least, bool by_group,
+                                           Share &out) {
     const int n_seq = A.s.n_seq;
     if (n_seq == 1) {  // nothing to search, and no exchange between lanes
         const Extent e = extent(A, 0, cols);
@@ -110,6 +111,7 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
             if ((float)shares_of(e.nb, r, least) * (float)e.ct * (float)A.H <= (float)A.target) R = r;
         }
         const int ns = shares_of(e.nb, R, least);
+        if (by_group) item *= ns;
         out = Share{0, e.a, e.b - e.a, e.len - (e.b - e.a), e.ct - 1 - item / ns, item % ns, ns, item};
         return !e.bad && item < e.ct * ns;
     }
@@ -137,8 +139,8 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
     int slots = 0;
     for (int i0 = 0; i0 < n_seq; i0 += 64) {
         const Extent e = i0 ? extent(A, i0 + lane, cols) : e0;
-        const int ns = shares_of(e.nb, R, least), mine = e.ct * ns, sum = sp_fp8_scan(mine, lane);
-        const int part = ns > 1 ? mine : 0, psum = sp_fp8_scan(part, lane);
+        const int ns = shares_of(e.nb, R, least), mine = by_group ? e.ct : e.ct * ns, sum = sp_fp8_scan(mine, lane);
+        const int part = ns > 1 ? e.ct * ns : 0, psum = sp_fp8_scan(part, lane);
         const unsigned long long past = __ballot(sum > item);
         if (past) {
             const int l = __ffsll(past) - 1;
@@ -148,7 +150,7 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
             out.n_new = of(e.b) - out.r0;
             out.first = of(e.len) - out.n_new;
             out.n_split = of(ns);
-            const int at = item - (of(sum) - of(mine));
+            const int at = (item - (of(sum) - of(mine))) * (by_group ? out.n_split : 1);
             // the last column group first: under the causal mask it sees most
             out.ct = of(e.ct) - 1 - at / out.n_split;
             out.split = at % out.n_split;
@@ -178,16 +180,16 @@ __device__ __forceinline__ void load8(const typename SpFp8Elem<DT>::T *p, bool a
     }
 }
 
-struct f2 {
+struct Two {
     float x, y;
 };
 __device__ __forceinline__ void put_pair(float *p, float x, float y) {
-    const f2 v{x, y};
+    const Two v{x, y};
     __hip_atomic_store(reinterpret_cast<unsigned long long *>(p), __builtin_bit_cast(unsigned long long, v),
                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ f2 get_pair(const float *p) {
-    return __builtin_bit_cast(f2, __hip_atomic_load(reinterpret_cast<const unsigned long long *>(p), __ATOMIC_RELAXED,
+__device__ __forceinline__ Two get_pair(const float *p) {
+    return __builtin_bit_cast(Two, __hip_atomic_load(reinterpret_cast<const unsigned long long *>(p), __ATOMIC_RELAXED,
                                                     __HIP_MEMORY_SCOPE_AGENT));
 }
 
@@ -229,7 +231,7 @@ struct Acc {
 // The last of a column group's shares to arrive joins them all, in their order. Every thread of
 // the block calls it after its partial's stores. smem: at least NW * n_cols * HD floats.
 template <int HD, int DT, int NW, int COLS>
-__device__ __forceinline__ void join_shares(const SpFp8Attn &A, const Share &sh, int h, long long c0, int n_cols,
+__device__ __forceinline__ void join_shares(const SpFp8Attn &A, const Share &sh, int h, int c0, int n_cols,
                                             float *smem, int *last_flag) {
     constexpr int NT = NW * 64, ROW = HD + 2;
     const int tid = threadIdx.x, pairs = n_cols * (HD / 2);
@@ -257,7 +259,7 @@ __device__ __forceinline__ void join_shares(const SpFp8Attn &A, const Share &sh,
             const float *src = A.part + (slot0 * COLS + cc) * ROW;
             const long long step = (long long)A.H * COLS * ROW;
             for (int v0 = grp * run; v0 < v1; v0 += 8) {
-                f2 ml[8], xy[8];
+                Two ml[8], xy[8];
 #pragma unroll
                 for (int v = 0; v < 8; v++) {
                     const float *rec = src + min(v0 + v, v1 - 1) * step;
@@ -280,8 +282,8 @@ __device__ __forceinline__ void join_shares(const SpFp8Attn &A, const Share &sh,
                 }
         }
         if (here && !grp) {
-            const long long n = c0 + cc;
-            finish<DT>(A, sh.r0 + n / A.G, h * A.G + (int)(n % A.G), HD, d, acc.M, acc.L, acc.x, acc.y, P_TOP);
+            const int n = c0 + cc;
+            finish<DT>(A, sh.r0 + n / A.G, h * A.G + n % A.G, HD, d, acc.M, acc.L, acc.x, acc.y, P_TOP);
         }
     }
 }
@@ -298,11 +300,10 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.H;
     Share sh;
-    if (!find_share(A, blockIdx.x / A.H, lane, COLS, NW / 2, sh)) return;
-    const int n_cols = (int)min((long long)sh.n_new * A.G - (long long)sh.ct * COLS, (long long)COLS);
+    if (!find_share(A, blockIdx.x / A.H, lane, COLS, NW / 2, false, sh)) return;
+    const int c0 = sh.ct * COLS, n_cols = min(sh.n_new * A.G - c0, COLS);
     const int col = lane & 15, g = lane >> 4;
-    const long long c0 = (long long)sh.ct * COLS;
-    const int tk0 = (int)(c0 / A.G), tk1 = (int)((c0 + n_cols - 1) / A.G);
+    const int tk0 = c0 / A.G, tk1 = (c0 + n_cols - 1) / A.G;
     const int pos0 = sh.first + tk0, pos1 = sh.first + tk1;
     // the cache blocks that these columns see, and this share of them
     const int j0 = A.window > 0 ? max(pos0 - A.window + 1, 0) >> 6 : 0;
@@ -347,11 +348,10 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 #pragma unroll
     for (int y = 0; y < CG; y++) {
         active[y] = y * 16 + col < n_cols;
-        const long long cn = c0 + (active[y] ? y * 16 + col : 0);
-        const int tk = (int)(cn / A.G), head = h * A.G + (int)(cn % A.G);
+        const int cn = c0 + (active[y] ? y * 16 + col : 0), tk = cn / A.G, head = h * A.G + cn % A.G;
         pos[y] = active[y] ? sh.first + tk : -1;
         from[y] = A.window > 0 ? pos[y] - A.window : -1;
-        const T *src = reinterpret_cast<const T *>(A.q) + (sh.r0 + tk) * A.q_stride + (long long)head * HD + g * 8;
+        const T *src = reinterpret_cast<const T *>(A.q) + (long long)(sh.r0 + tk) * A.q_stride + (long long)head * HD + g * 8;
         const bool aligned = ((uintptr_t)A.q % (4 * sizeof(T))) == 0 && A.q_stride % 4 == 0;
 #pragma unroll
         for (int c = 0; c < NC; c++) load8<DT>(src + c * 32, aligned, x[y][c]);
@@ -514,8 +514,8 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
             acc.y += rec[d + 1] * f;
         }
         if (alone) {
-            const long long n = c0 + cc;
-            finish<DT>(A, sh.r0 + n / A.G, h * A.G + (int)(n % A.G), HD, d, acc.M, acc.L, acc.x, acc.y, P_TOP);
+            const int n = c0 + cc;
+            finish<DT>(A, sh.r0 + n / A.G, h * A.G + n % A.G, HD, d, acc.M, acc.L, acc.x, acc.y, P_TOP);
         } else {
             float *dst = A.part + (slot * COLS + cc) * ROW;
             if (d == 0) put_pair(dst, acc.M, acc.L);
@@ -530,15 +530,17 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 // ---------------------------------------------------------------------------
 // many rows: prompts and their chunks
 // ---------------------------------------------------------------------------
-// A block of threads holds 32 columns a wave and shares each cache block's conversion: the
-// codes become fp16 once, in LDS, in the operand order of v_mfma_f32_32x32x16_f16, two buffers
-// deep with one barrier a block. As above the scores are K q^T and the weights stay where they
-// were made: lane (column, half)'s registers 8 k .. 8 k + 7 are positions
-// 16 k + 8 (j / 4) + 4 half + j % 4, and V's operand is laid out for that order.
+// A block of threads holds CW columns a wave and shares each cache block's conversion: the codes
+// become fp16 once, in LDS, in the operand order of the matrix instructions, two places deep with
+// one barrier a block. As above the scores are K q^T and the weights stay where they were made.
+//   CW 32: v_mfma_f32_32x32x16_f16. Lane (column, sub of 2) has positions 8 (i / 4) + 4 sub + i % 4
+//          of each 32; V's operand is laid out for that order.
+//   CW 16: v_mfma_f32_16x16x32_f16. Lane (column, sub of 4) has positions 16 (i / 4) + 4 sub + i % 4.
+// A wave of 32 columns reads LDS half as often a column; one of 16 needs half of the registers,
+// which is what keeps several waves on a SIMD at head_dim 256.
 //
 // The loop is pipelined by one cache block: the next block's scores go through the matrix cores
-// while this one's weights are computed, and the next one's maximum is taken during the product
-// with V, so that neither unit waits for the other.
+// among this one's weights and its product with V, so that neither unit waits for the other.
 //
 // The running maximum is a reference that is raised only when a score passes it by 2^W_SLACK
 // (the weights, 2^W_TOP at the reference, then still fit fp16), so that the output is rescaled
@@ -550,18 +552,46 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 // within a factor of two and their unit always, so that the second part keeps its bits.
 typedef float f16x __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ f16x mma32(h8 a, h8 b, f16x c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-
 // LDS written before is seen after, by the whole block; loads from memory stay in flight.
 __device__ __forceinline__ void lds_barrier() {
     __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-template <int HD, int DT, int NW>
+template <int CW>
+struct Tile;
+template <>
+struct Tile<32> {
+    typedef f16x V;
+    static __device__ __forceinline__ V mma(h8 a, h8 b, V c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Tile<16> {
+    typedef f4 V;
+    static __device__ __forceinline__ V mma(h8 a, h8 b, V c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+// Place of a row's 16-byte piece s in the row of column c (HD / 8 pieces a row in LDS): the
+// pieces that 16 neighbouring columns read at once are in 16 different groups of four banks.
+template <int HD>
+__device__ __forceinline__ int turned(int c, int s) {
+    if (HD % 128 == 0) return s ^ (c & 15);
+    if (HD == 64) return s ^ ((c >> 1) & 7);
+    const int t = s + ((c >> 2) & 3);  // HD 96: rows of 12 pieces start at every fourth group
+    return t >= HD / 8 ? t - HD / 8 : t;
+}
+
+template <int HD, int DT, int NW, int CW>
 __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
-    constexpr int COLS = 32 * NW, NS = HD / 16, ND = HD / 32, TILE = 64 * HD, ROW = HD + 2, NT = NW * 64, HT = NT / 2;
+    typedef Tile<CW> M;
+    typedef typename M::V V;
+    constexpr int COLS = CW * NW, TILE = 64 * HD, NT = NW * 64, HT = NT / 2, ROW = HD + 4;
+    constexpr int VL = CW == 32 ? 16 : 4;   // values of a lane in a matrix instruction's result
+    constexpr int RB = 64 / CW;             // row blocks of a cache block's 64 positions
+    constexpr int NE = RB * VL;             // scores of a lane
+    constexpr int NP = NE / 8;              // steps of the product with V, eight weights of a lane each
+    constexpr int NS = CW == 32 ? HD / 16 : HD / 32;  // steps of the scores
+    constexpr int ND = HD / CW;             // row blocks of the output
+    constexpr int KE = CW == 32 ? 16 : 32;  // channels of a score step
     constexpr bool SPLIT2 = DT == SP_DTYPE_F32;
     constexpr int NH = SPLIT2 ? 2 : 1;
     constexpr float W_TOP = SPLIT2 ? 14.0f : 12.0f, W_SLACK = SPLIT2 ? 1.0f : 3.0f;
@@ -571,15 +601,13 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     constexpr int RAW = KP > 2 * VP ? KP : 2 * VP;
     typedef typename SpFp8Elem<DT>::T T;
     extern __shared__ __align__(16) float smem[];  // K, K, V, V: two places each, 64 * HD fp16
-    __shared__ int last_flag;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = blockIdx.x % A.H;
     Share sh;
-    if (!find_share(A, blockIdx.x / A.H, lane, COLS, 4, sh)) return;
-    const int n_cols = (int)min((long long)sh.n_new * A.G - (long long)sh.ct * COLS, (long long)COLS);
-    const int col = lane & 31, half = lane >> 5;
-    const long long c0 = (long long)sh.ct * COLS;
-    const int pos0 = sh.first + (int)(c0 / A.G), pos1 = sh.first + (int)((c0 + n_cols - 1) / A.G);
+    if (!find_share(A, blockIdx.x / A.H, lane, COLS, A.least, false, sh)) return;
+    const int c0 = sh.ct * COLS, n_cols = min(sh.n_new * A.G - c0, COLS);
+    const int col = lane & (CW - 1), sub = lane / CW;
+    const int pos0 = sh.first + c0 / A.G, pos1 = sh.first + (c0 + n_cols - 1) / A.G;
     const int j0 = A.window > 0 ? max(pos0 - A.window + 1, 0) >> 6 : 0;
     const int j1 = min((pos1 >> 6) + 1, A.s.stride);
     const int per = max((j1 - j0 + sh.n_split - 1) / sh.n_split, 0);
@@ -602,6 +630,8 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
                      sp_fp8_exponent(__builtin_amdgcn_readlane(evb, k & 63))};
     };
     // ---- staging: half of the waves bring K, half V ----
+    // K's piece (uc, g, r), uc = u * HD/32 + c. V's pieces in pairs: CW 32 takes g and g + 2 of a
+    // channel, which its operand has side by side; CW 16 two channel groups.
     const bool stage_v = w >= NW / 2;
     const int st = stage_v ? tid - HT : tid;
     u4 raw[RAW];
@@ -616,11 +646,13 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
             const uint8_t *p = A.v.codes + b * TILE;
 #pragma unroll
             for (int i = 0; i < VP; i++) {
-                const int x = st + i * HT;  // (D, gl, dg % 2, r): pieces g = gl and gl + 2 of channel group 2 D + dg % 2
+                const int x = st + i * HT;
                 if (VP * HT == HD * 2 || x < HD * 2) {
-                    const uint8_t *s = p + ((x >> 6) * 2 + ((x >> 4) & 1)) * 1024 + ((x >> 5) & 1) * 256 + (x & 15) * 16;
+                    // CW 32: x = (dg / 2, g % 2, dg % 2, r); CW 16: x = (dg / 2, g, r)
+                    const uint8_t *s = CW == 32 ? p + ((x >> 6) * 2 + ((x >> 4) & 1)) * 1024 + ((x >> 5) & 1) * 256 + (x & 15) * 16
+                                                : p + (x >> 6) * 2048 + (x & 63) * 16;
                     raw[2 * i] = *reinterpret_cast<const u4 *>(s);
-                    raw[2 * i + 1] = *reinterpret_cast<const u4 *>(s + 512);
+                    raw[2 * i + 1] = *reinterpret_cast<const u4 *>(s + (CW == 32 ? 512 : 1024));
                 }
             }
         }
@@ -630,11 +662,15 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
         if (!stage_v) {
 #pragma unroll
             for (int i = 0; i < KP; i++) {
-                const int x = st + i * HT, g = (x >> 4) & 3, r = x & 15, uc = x >> 6;  // uc = u * HD/32 + c
+                const int x = st + i * HT, g = (x >> 4) & 3, r = x & 15, uc = x >> 6;
                 if (KP * HT == HD * 4 || x < HD * 4) {
-                    h8 *d = kbuf + kb * (TILE / 8) + (uc * 2 + (g >> 1)) * 64 + (g & 1) * 32 + r;
+                    // row block and step of the operand, lane in it: CW 32 holds positions r and 16 + r of a
+                    // 32 in one row block, CW 16 in two
+                    h8 *d = kbuf + kb * (TILE / 8) +
+                            (CW == 32 ? (uc * 2 + (g >> 1)) * 64 + (g & 1) * 32 + r
+                                      : ((uc / (HD / 32)) * 2 * NS + uc % (HD / 32)) * 64 + (x & 63));
                     d[0] = to_half(raw[i][0], raw[i][1]);
-                    d[16] = to_half(raw[i][2], raw[i][3]);
+                    d[CW == 32 ? 16 : NS * 64] = to_half(raw[i][2], raw[i][3]);
                 }
             }
         } else {
@@ -642,9 +678,17 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
             for (int i = 0; i < VP; i++) {
                 const int x = st + i * HT;
                 if (VP * HT == HD * 2 || x < HD * 2) {
+                    // (opaque: else the conversions are shared with K's, and moved to where V's go)
+                    __asm__("" : "+v"(raw[2 * i]), "+v"(raw[2 * i + 1]));
                     h8 *d = vbuf + vb * (TILE / 8) + (x >> 6) * 256 + (x & 63);
+                    if (CW == 32) {
 #pragma unroll
-                    for (int t4 = 0; t4 < 4; t4++) d[t4 * 64] = to_half(raw[2 * i][t4], raw[2 * i + 1][t4]);
+                        for (int t4 = 0; t4 < 4; t4++) d[t4 * 64] = to_half(raw[2 * i][t4], raw[2 * i + 1][t4]);
+                    } else {
+#pragma unroll
+                        for (int t4 = 0; t4 < 4; t4++)
+                            d[t4 * 64] = to_half(raw[2 * i + t4 / 2][t4 % 2 * 2], raw[2 * i + t4 / 2][t4 % 2 * 2 + 1]);
+                    }
                 }
             }
         }
@@ -656,30 +700,53 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     }
 
     // ---- queries ----
-    const int mycol = w * 32 + col;
+    const int mycol = w * CW + col;
     const bool active = mycol < n_cols;
-    const long long cn = c0 + (active ? mycol : 0);
-    const int tk = (int)(cn / A.G), head = h * A.G + (int)(cn % A.G);
+    const int cn = c0 + (active ? mycol : 0), tk = cn / A.G, head = h * A.G + cn % A.G;
     const long long row = (long long)sh.r0 + tk;
     const int pos = active ? sh.first + tk : -1;
     const int from = A.window > 0 ? pos - A.window : -1;  // sees (from, pos]
     // of this wave's columns: whether there are any, and their first and last position
-    const bool busy = w * 32 < n_cols;
-    const int wlast = min(w * 32 + 31, n_cols - 1);
-    const int wpos0 = sh.first + (int)((c0 + w * 32) / A.G), wpos1 = sh.first + (int)((c0 + wlast) / A.G);
+    const bool busy = w * CW < n_cols;
+    const int wlast = min(w * CW + CW - 1, n_cols - 1);
+    const int wpos0 = sh.first + (c0 + w * CW) / A.G, wpos1 = sh.first + (c0 + wlast) / A.G;
     h8 q[NS][NH];
     float cscale;
     {
-        const T *src = reinterpret_cast<const T *>(A.q) + row * A.q_stride + (long long)head * HD + half * 8;
-        const bool aligned = ((uintptr_t)A.q % (4 * sizeof(T))) == 0 && A.q_stride % 4 == 0;
+        // Rows of 16-bit types go through LDS, in 16-byte pieces: loaded as they lie, and read
+        // back by column with a row's pieces turned around so that 16 columns' reads meet no bank
+        // twice. (Loaded by column, a wave's 16 bytes are in 16 or 32 rows at a time.)
+        const T *src = reinterpret_cast<const T *>(A.q) + row * A.q_stride + (long long)head * HD + sub * 8;
+        const bool aligned = (uintptr_t)A.q % (4 * sizeof(T)) == 0 && A.q_stride % 4 == 0;
+        const bool pieces = !SPLIT2 && (uintptr_t)A.q % 16 == 0 && A.q_stride % 8 == 0;
+        const auto piece = [&](int c, int s) {
+            return reinterpret_cast<u4 *>(smem) + c * (HD / 8) + turned<HD>(c, s);
+        };
+        if (pieces) {
+            u4 got[COLS * HD / 8 / NT];
+#pragma unroll
+            for (int i = 0; i < COLS * HD / 8 / NT; i++) {
+                const int at = tid + i * NT, nn = c0 + min(at / (HD / 8), n_cols - 1);
+                got[i] = *reinterpret_cast<const u4 *>(reinterpret_cast<const T *>(A.q) + (long long)(sh.r0 + nn / A.G) * A.q_stride +
+                                                       (long long)(h * A.G + nn % A.G) * HD + at % (HD / 8) * 8);
+            }
+#pragma unroll
+            for (int i = 0; i < COLS * HD / 8 / NT; i++) *piece((tid + i * NT) / (HD / 8), (tid + i * NT) % (HD / 8)) = got[i];
+            lds_barrier();
+        }
+        const auto eight = [&](int s, float x[8]) __attribute__((always_inline)) {
+            if (pieces) load8<DT>(reinterpret_cast<const T *>(piece(mycol, s * (KE / 8) + sub)), true, x);
+            else load8<DT>(src + s * KE, aligned, x);
+        };
         float top = 0.0f;
         float x[8];
 #pragma unroll
         for (int s = 0; s < NS; s++) {
-            load8<DT>(src + s * 16, aligned, x);
+            eight(s, x);
 #pragma unroll
             for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(x[k]));
         }
+        if (CW == 16) top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         int e = (__float_as_int(top) >> 23) - 127 - 14;
         e = top == 0.0f || !(top < INFINITY) ? 0 : max(e, -126);
@@ -687,7 +754,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
         cscale = A.c * sp_fp8_pow2(e);
 #pragma unroll
         for (int s = 0; s < NS; s++) {
-            load8<DT>(src + s * 16, aligned, x);
+            eight(s, x);
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const float v = active ? x[k] * down : 0.0f;
@@ -697,88 +764,91 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
             }
         }
     }
+    lds_barrier();  // the queries are in registers: LDS is for the blocks
 
-    f16x o[ND];
+    V o[ND];
 #pragma unroll
-    for (int d = 0; d < ND; d++) o[d] = f16x{};
+    for (int d = 0; d < ND; d++) o[d] = V{};
     // m: the reference; off = W_TOP - m, 0 while m is -inf; the output's unit is 2^ev_now
     float m = -INFINITY, off = 0.0f, l = 0.0f;
     int ev_now = 0;
     bool huge = false;  // the fused difference of a score and the reference would not be 0 where they are equal
     // of the block whose weights come next: score scale, exponent offset, its part in l
     float cs = 0.0f, shift = 0.0f, lmul = 1.0f;
-    h8 p[4][NH];
+    h8 p[NP][NH];
 
-    // next = K q^T of one block; of the one before, the weights from its scores and, sixteen
-    // positions at a time, out^T += V^T p^T (the last sixteen: product, afterwards).
-    const auto product = [&](auto group, const h8 *vd) __attribute__((always_inline)) {
-        constexpr int t4 = decltype(group)::value;
+    // out^T += V^T p^T for one of the NP steps
+    const auto product = [&](auto step, const h8 *vd) __attribute__((always_inline)) {
+        constexpr int t = decltype(step)::value;
 #pragma unroll
         for (int d = 0; d < ND; d++) {
-            const h8 a = vd[(d * 4 + t4) * 64];
+            const h8 a = vd[(d * NP + t) * 64];
 #pragma unroll
-            for (int x = 0; x < NH; x++) o[d] = mma32(a, p[t4][x], o[d]);
+            for (int x = 0; x < NH; x++) o[d] = M::mma(a, p[t][x], o[d]);
         }
     };
-    const auto blend = [&](auto with_scores, auto with_weights, const h8 *kd, const h8 *vd, f16x(&next)[2],
-                           const f16x(&s)[2]) __attribute__((always_inline)) {
+    // next = K q^T of one block; of the one before, the weights from its scores and all but the
+    // last step of the product with V
+    const auto blend = [&](auto with_scores, auto with_weights, const h8 *kd, const h8 *vd, V(&next)[RB],
+                           const V(&s)[RB]) __attribute__((always_inline)) {
         float sum = 0.0f;
-        h8 ka[2], kb[2];  // K's operands, read one step ahead
+        h8 ka[2][RB];  // K's operands are read one step ahead
         if constexpr (decltype(with_scores)::value) {
-            ka[0] = kd[0];
-            kb[0] = kd[NS * 64];
+#pragma unroll
+            for (int b = 0; b < RB; b++) ka[0][b] = kd[b * NS * 64];
         }
 #pragma unroll
         for (int c = 0; c < NS; c++) {
             if constexpr (decltype(with_scores)::value) {
                 if (c + 1 < NS) {
-                    ka[(c + 1) & 1] = kd[(c + 1) * 64];
-                    kb[(c + 1) & 1] = kd[(NS + c + 1) * 64];
+#pragma unroll
+                    for (int b = 0; b < RB; b++) ka[(c + 1) & 1][b] = kd[(b * NS + c + 1) * 64];
                 }
 #pragma unroll
-                for (int x = 0; x < NH; x++) {
-                    next[0] = mma32(ka[c & 1], q[c][x], c || x ? next[0] : f16x{});
-                    next[1] = mma32(kb[c & 1], q[c][x], c || x ? next[1] : f16x{});
-                }
+                for (int x = 0; x < NH; x++)
+#pragma unroll
+                    for (int b = 0; b < RB; b++) next[b] = M::mma(ka[c & 1][b], q[c][x], c || x ? next[b] : V{});
             }
             if constexpr (decltype(with_weights)::value) {
 #pragma unroll
-                for (int i = c * 16 / NS * 2; i < (c + 1) * 16 / NS * 2; i++) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 4][i & 15], cs, shift));
+                for (int i = c * (NE / 2) / NS * 2; i < (c + 1) * (NE / 2) / NS * 2; i++) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / VL][i % VL], cs, shift));
                     sum += x;
                     const _Float16 hi = (_Float16)x;
                     p[i >> 3][0][i & 7] = hi;
                     if (SPLIT2) p[i >> 3][NH - 1][i & 7] = (_Float16)(x - (float)hi);
                 }
-                // the sixteens whose weights were complete a step ago
-                const int done = c * 16 / NS * 2 / 8, before = c ? (c - 1) * 16 / NS * 2 / 8 : 0;
+                // the steps whose weights were complete before this one
+                const int done = c * (NE / 2) / NS * 2 / 8, before = c ? (c - 1) * (NE / 2) / NS * 2 / 8 : 0;
                 if (done > before) {
                     if (done == 1) product(std::integral_constant<int, 0>(), vd);
-                    if (done == 2) product(std::integral_constant<int, 1>(), vd);
-                    if (done == 3) product(std::integral_constant<int, 2>(), vd);
+                    if constexpr (NP == 4) {
+                        if (done == 2) product(std::integral_constant<int, 1>(), vd);
+                        if (done == 3) product(std::integral_constant<int, 2>(), vd);
+                    }
                 }
             }
         }
         if constexpr (decltype(with_weights)::value) l += sum * lmul;
     };
-    const auto mask = [&](const Facts &f, int k, f16x(&s)[2]) __attribute__((always_inline)) {
+    const auto mask = [&](const Facts &f, int k, V(&s)[RB]) __attribute__((always_inline)) {
         const int t = t0 + k;
         if (f.b >= 0 && t * 64 + 63 <= wpos0 && (A.window <= 0 || t * 64 > wpos1 - A.window)) return;
-        const int lane0 = t * 64 + 4 * half, upto = f.b < 0 ? -1 : pos - lane0, before = from - lane0;
+        const int lane0 = t * 64 + 4 * sub, upto = f.b < 0 ? -1 : pos - lane0, before = from - lane0;
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-            const int at = (i >> 4) * 32 + ((i & 15) >> 2) * 8 + (i & 3);
-            s[i >> 4][i & 15] = at <= upto && at > before ? s[i >> 4][i & 15] : -INFINITY;
+        for (int i = 0; i < NE; i++) {
+            const int at = CW == 32 ? (i >> 2) * 8 + (i & 3) : (i >> 2) * 16 + (i & 3);
+            s[i / VL][i % VL] = at <= upto && at > before ? s[i / VL][i % VL] : -INFINITY;
         }
     };
-    const auto largest = [&](const f16x(&s)[2]) __attribute__((always_inline)) {
+    const auto largest = [&](const V(&s)[RB]) __attribute__((always_inline)) {
         float top = s[0][0];
 #pragma unroll
-        for (int i = 1; i < 32; i++) top = fmaxf(top, s[i >> 4][i & 15]);
+        for (int i = 1; i < NE; i++) top = fmaxf(top, s[i / VL][i % VL]);
         return top;
     };
     // the reference and the output's unit for a block with largest score `top` (this lane's)
-    const auto settle = [&](const Facts &f, float top, f16x(&s)[2]) __attribute__((always_inline)) {
+    const auto settle = [&](const Facts &f, float top, V(&s)[RB]) __attribute__((always_inline)) {
         // never 0: a masked score stays -inf when it is multiplied
         cs = fmaxf(cscale * sp_fp8_pow2(f.ek), 0x1p-126f);
         const bool raise = m == -INFINITY ? top > -INFINITY : __builtin_fmaf(top, cs, off) > W_TOP + W_SLACK;
@@ -790,6 +860,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
             rescale = true;
         }
         if (__any(raise)) {
+            if (CW == 16) top = fmaxf(top, __shfl_xor(top, 16, 64));
             const float mx = fmaxf(top, __shfl_xor(top, 32, 64)) * cs, m_new = fmaxf(m, mx);
             const float alpha = weight(m, m_new);
             l *= alpha;
@@ -801,7 +872,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
         }
         if (huge) {  // the reference was rounded: round the scores as it was
 #pragma unroll
-            for (int i = 0; i < 32; i++) s[i >> 4][i & 15] *= cs;
+            for (int i = 0; i < NE; i++) s[i / VL][i % VL] *= cs;
             cs = 1.0f;
         }
         if (rescale) {
@@ -813,12 +884,12 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     };
     const std::true_type yes;
     const std::false_type no;
-    const std::integral_constant<int, 3> last16;
+    const std::integral_constant<int, NP - 1> last_step;
 
     // ---- block 0's scores; K one block ahead of V from here ----
     // Blocks past the last are fetched as block 0 and never used: no turn asks for its place.
     constexpr int STEP = TILE / 8;
-    f16x sa[2], sb[2];
+    V sa[RB], sb[RB];
     if (n > 0) {
         stage(0, 0);
         f1 = facts(1);
@@ -847,12 +918,12 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
         f1 = f2;
         f2 = f3;
     };
-    const auto turn = [&](int k, f16x(&s)[2], f16x(&next)[2]) __attribute__((always_inline)) {
+    const auto turn = [&](int k, V(&s)[RB], V(&next)[RB]) __attribute__((always_inline)) {
         const Facts f = f1;
         const h8 *vd = vbuf + (k & 1) * STEP + lane;
         blend(yes, yes, kbuf + (1 - (k & 1)) * STEP + lane, vd, next, s);
         bring(k);
-        product(last16, vd);
+        product(last_step, vd);
         mask(f, k + 1, next);
         settle(f, largest(next), next);
         lds_barrier();
@@ -865,14 +936,14 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
         }
         if (k + 1 < n) {
             turn(k, sa, sb);
-            sa[0] = sb[0];
-            sa[1] = sb[1];
+#pragma unroll
+            for (int b = 0; b < RB; b++) sa[b] = sb[b];
             k++;
         }
         if (k < n) {  // the last one: no more scores
             const h8 *vd = vbuf + (k & 1) * STEP + lane;
             blend(no, yes, nullptr, vd, sa, sa);
-            product(last16, vd);
+            product(last_step, vd);
         }
     } else {  // no columns: bring blocks for the other waves
         for (int k = 0; k + 1 < n; k++) {
@@ -881,40 +952,108 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
         }
     }
     lds_barrier();
+    if (CW == 16) l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 
     // ---- results ----
-    const bool alone = sh.n_split == 1;
-    const long long slot = (long long)sh.slot * A.H + h;
-    if (!alone && !slot_fits(slot, COLS, HD)) return;
+    // of lane values i .. i + 3 of row block d: channels from
+    const auto channel = [&](int d, int i) { return d * CW + i * 2 + 4 * sub; };
     const float unit = sp_fp8_pow2(ev_now);
-    if (active && alone) {
-        T *out = reinterpret_cast<T *>(A.out) + row * A.out_stride + (long long)head * HD;
-        const bool aligned = ((uintptr_t)A.out % (4 * sizeof(T))) == 0 && A.out_stride % 4 == 0;
-        const float r = l == 0.0f ? 0.0f : 1.0f / l;
+    if (sh.n_split > 1) {  // joined by k_fp8_attn_join
+        const long long slot = (long long)sh.slot * A.H + h;
+        if (active && slot_fits(slot, COLS, HD)) {
+            float *dst = A.part + (slot * COLS + mycol) * ROW;
+            // the maximum whose weight would be 2^P_TOP
+            if (sub == 0) *reinterpret_cast<Two *>(dst + HD) = Two{m + (P_TOP - W_TOP), l};
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int i = 0; i < VL; i += 4)
+                    *reinterpret_cast<f4 *>(dst + channel(d, i)) =
+                        f4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]} * unit;
+        }
+        return;
+    }
+    // as the queries came: by column into LDS, in rows to memory
+    const bool through = !SPLIT2 && (uintptr_t)A.out % 16 == 0 && A.out_stride % 8 == 0;
+    if (active) {
+        const float r = l == 0.0f ? 0.0f : unit / l;
+        const bool aligned = (uintptr_t)A.out % (4 * sizeof(T)) == 0 && A.out_stride % 4 == 0;
+        T *out = through ? reinterpret_cast<T *>(smem) : reinterpret_cast<T *>(A.out) + row * A.out_stride + (long long)head * HD;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < VL; i += 4) {
                 f4 x;
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[j] = l == 0.0f ? 0.0f : o[d][i * 4 + j] * unit * r;
-                store4<DT>(out, d * 32 + i * 8 + half * 4, x, aligned);
+                for (int j = 0; j < 4; j++) x[j] = l == 0.0f ? 0.0f : o[d][i + j] * r;
+                const int ch = channel(d, i);
+                if (through) store4<DT>(out, (mycol * (HD / 8) + turned<HD>(mycol, ch >> 3)) * 8 + (ch & 4), x, true);
+                else store4<DT>(out, ch, x, aligned);
             }
-        if (A.lse && half == 0)
+        if (A.lse && sub == 0)
             A.lse[row * A.H * A.G + head] = l == 0.0f ? -INFINITY : (m - W_TOP + __log2f(l)) * 0.69314718055994531f;
     }
-    if (alone) return;
-    if (active) {
-        float *dst = A.part + (slot * COLS + mycol) * ROW;
-        if (half == 0) put_pair(dst, m + (P_TOP - W_TOP), l);  // the maximum whose weight would be 2^P_TOP
+    if (!through) return;
+    lds_barrier();
 #pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                put_pair(dst + 2 + d * 32 + (i >> 1) * 8 + half * 4 + (i & 1) * 2, o[d][2 * i] * unit, o[d][2 * i + 1] * unit);
+    for (int i = 0; i < COLS * HD / 8 / NT; i++) {
+        const int at = tid + i * NT, c = at / (HD / 8), nn = c0 + c;
+        if (c < n_cols)
+            *reinterpret_cast<u4 *>(reinterpret_cast<T *>(A.out) + (long long)(sh.r0 + nn / A.G) * A.out_stride +
+                                    (long long)(h * A.G + nn % A.G) * HD + at % (HD / 8) * 8) =
+                reinterpret_cast<const u4 *>(smem)[c * (HD / 8) + turned<HD>(c, at % (HD / 8))];
     }
-    join_shares<HD, DT, NW, COLS>(A, sh, h, c0, n_cols, smem, &last_flag);
+}
+
+// Joins the shares of the column groups that have more than one, in their order. A launch of its
+// own: a group's partial results are 64 to 128 KB a share, too many for the last block to
+// arrive alone. Blocks of threads: (KV head, column group) by 32 columns.
+template <int HD, int DT, int COLS>
+__global__ __launch_bounds__(256) void k_fp8_attn_join(SpFp8Attn A) {
+    constexpr int ROW = HD + 4, PER = HD / 4;
+    typedef typename SpFp8Elem<DT>::T T;
+    const int h = blockIdx.x % A.H;
+    Share sh;
+    if (!find_share(A, blockIdx.x / A.H, threadIdx.x & 63, COLS, A.least, true, sh) || sh.n_split == 1) return;
+    const long long slot0 = (long long)sh.slot * A.H + h;
+    if (!slot_fits(slot0 + (long long)(sh.n_split - 1) * A.H, COLS, HD)) return;
+    const int c0 = sh.ct * COLS, n_cols = min(sh.n_new * A.G - c0, COLS);
+    const bool aligned = (uintptr_t)A.out % (4 * sizeof(T)) == 0 && A.out_stride % 4 == 0;
+    for (int at = threadIdx.x; at < 32 * PER; at += 256) {
+        const int c = blockIdx.y * 32 + at / PER, d = at % PER * 4;
+        if (c >= n_cols) return;
+        const float *src = A.part + (slot0 * COLS + c) * ROW;
+        const long long step = (long long)A.H * COLS * ROW;
+        float M = -INFINITY, L = 0.0f;
+        f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int v0 = 0; v0 < sh.n_split; v0 += 8) {
+            Two ml[8];
+            f4 part[8];
+#pragma unroll
+            for (int v = 0; v < 8; v++) {
+                const float *rec = src + min(v0 + v, sh.n_split - 1) * step;
+                ml[v] = *reinterpret_cast<const Two *>(rec + HD);
+                part[v] = *reinterpret_cast<const f4 *>(rec + d);
+            }
+#pragma unroll
+            for (int v = 0; v < 8; v++)
+                if (v0 + v < sh.n_split) {
+                    const float Mn = fmaxf(M, ml[v].x), a = weight(M, Mn), b = weight(ml[v].x, Mn);
+                    L = L * a + ml[v].y * b;
+                    x = x * a + part[v] * b;
+                    M = Mn;
+                }
+        }
+        const int nn = c0 + c, head = h * A.G + nn % A.G;
+        const long long row = (long long)sh.r0 + nn / A.G;
+        const float r = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = L == 0.0f ? 0.0f : x[j] * r;
+        store4<DT>(A.out, row * A.out_stride + (long long)head * HD + d, x, aligned);
+        if (A.lse && d == 0)
+            A.lse[row * A.H * A.G + head] = L == 0.0f ? -INFINITY : (M - P_TOP + __log2f(L)) * 0.69314718055994531f;
+    }
 }
 
 template <int HD, int DT, int NW, int CG>
@@ -937,15 +1076,23 @@ hipError_t launch(const SpFp8Attn &A, int per_cu, hipStream_t s) {
 
 template <int HD, int DT>
 hipError_t launch_wide(const SpFp8Attn &A, hipStream_t s) {
-    constexpr int NW = HD == 256 ? 4 : 8, COLS = 32 * NW;
+    constexpr int CW = HD == 256 && DT != SP_DTYPE_F32 ? 16 : 32, NW = HD == 256 && DT == SP_DTYPE_F32 ? 4 : 8;
+    constexpr int COLS = CW * NW;
     SpFp8Attn a = A;
     a.target = min(A.target, 256);
     const long long groups = (long long)A.s.n_rows * A.G / COLS + A.s.n_seq;
-    const long long blocks = (groups + (a.target + A.H - 1) / A.H) * A.H;
+    // With twice the blocks that the chip takes, sharing gains nothing. Below that a group is shared
+    // out where the others leave CUs idle, and a second launch joins the shares.
+    const bool share = groups * A.H < a.target;
+    a.least = share ? 4 : 1 << 28;
+    const long long blocks = (groups + (share ? (a.target + A.H - 1) / A.H : 0)) * A.H;
     if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
     void *args[] = {&a};
-    const void *f = (const void *)k_fp8_attn_wide<HD, DT, NW>;
-    return hipLaunchKernel(f, dim3((unsigned)blocks), dim3(NW * 64), args, (size_t)HD * 512, s);
+    const hipError_t e = hipLaunchKernel((const void *)k_fp8_attn_wide<HD, DT, NW, CW>, dim3((unsigned)blocks), dim3(NW * 64),
+                                         args, (size_t)HD * 512, s);
+    if (e != hipSuccess || !share) return e;
+    return hipLaunchKernel((const void *)k_fp8_attn_join<HD, DT, COLS>, dim3((unsigned)(groups * A.H), COLS / 32), dim3(256), args,
+                           0, s);
 }
 
 template <int HD, int DT>

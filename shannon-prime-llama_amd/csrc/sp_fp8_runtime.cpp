@@ -165,6 +165,7 @@ int attend(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *b, 
     if (!stream_ok(c, s, who)) return -1;
     if (b->n_rows == 0 || b->n_seq == 0) return 0;
     if (!d_q || !d_out) { sp_set_error("%s: q and out", who); return -1; }
+    if ((long long)b->n_rows * (n_q / H) > MAX_ROWS) { sp_set_error("%s: too many rows", who); return -1; }
     const Fp8Priv *pv = (const Fp8Priv *)c->priv;
     const OnDevice on(pv->device);
     if (!on.ok()) { sp_set_error("%s: the cache's device", who); return -1; }
@@ -221,7 +222,7 @@ extern "C" int sp_hip_fp8_cache_init(sp_hip_fp8_cache_t *c, const sp_config_t *c
         int fill;  // -1: not cleared
     } pieces[] = {{&c->d_k_codes, ncode, 0}, {&c->d_v_codes, ncode, 0},
                   {&c->d_k_exp, nexp, 127 + SP_FP8_EMIN}, {&c->d_v_exp, nexp, 127 + SP_FP8_EMIN},
-                  {(void **)&pv->part, (size_t)sp_fp8_part_rows(hd) * (hd + 2) * sizeof(float), -1},
+                  {(void **)&pv->part, (size_t)sp_fp8_part_rows(hd) * (hd + 4) * sizeof(float), -1},
                   {(void **)&pv->counters, SP_FP8_SLOTS * sizeof(int), 0}};
     for (const Piece &p : pieces)
         good = good && ok(hipMalloc(p.p, p.bytes), who) && (p.fill < 0 || ok(hipMemsetAsync(*p.p, p.fill, p.bytes, s), who));
