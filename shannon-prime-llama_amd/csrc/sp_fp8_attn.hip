@@ -1100,7 +1100,15 @@ hipError_t launch_dt(const SpFp8Attn &A, hipStream_t s) {
     constexpr int NW = HD == 256 ? 4 : 8;
     constexpr int CG = HD == 256 || DT == SP_DTYPE_F32 ? 1 : 2;
     const long long columns = (long long)A.s.n_rows * A.G;  // of each KV head
-    if (columns >= 64ll * A.s.n_seq && A.s.row) return launch_wide<HD, DT>(A, s);
+    // The kernel for many rows takes a cache block over 256 columns at once (128 at head_dim 256), this
+    // one over 32 (16) and reads it again for the next. Measured, few rows / many, 32 / 8 heads of 128:
+    //   columns a sequence   64            128           256           512          1024
+    //   1 sequence at 8K     27 / 41 us                  30 / 51       41 / 50      60 / 65
+    //   3 at 2 to 8K                                     41 / 50       77 / 63
+    //   12 at 1 to 4.5K      32 / 48       54 / 53       75 / 71
+    // 16 / 8 heads of 256, 1 at 8K: 256 columns 53 / 62, 512 78 / 71; 12 at 1 to 4.5K: 64 69 / 65.
+    constexpr int MANY = HD == 256 ? 512 : 1024;
+    if (A.s.row && columns >= MANY && columns >= MANY / 8 * (long long)A.s.n_seq) return launch_wide<HD, DT>(A, s);
     if (columns > 16ll * A.s.n_seq) return launch<HD, DT, NW, CG>(A, 1, s);
     return launch<HD, DT, NW, 1>(A, 1, s);
 }

@@ -335,7 +335,7 @@ def test_prefill_groups(group, new):
         P.check_attend(dtype, queries(rng, P, 2 * group, dtype), 0.2)
 
 
-@pytest.mark.parametrize("new,length", [(1, 20000), (6, 20001), (300, 9000), (1, 131072)])
+@pytest.mark.parametrize("new,length", [(1, 20000), (6, 20001), (300, 9000), (1, 131072), (257, 30000)])
 def test_long_sequences(new, length):
     """Work split over many shares of one sequence."""
     rng = np.random.default_rng(new)
@@ -348,6 +348,22 @@ def test_long_sequences(new, length):
     q = queries(rng, P, 4, "f32")
     a, b = P.attend("f32", q, 0.2), P.attend("f32", q, 0.2)
     assert all(np.array_equal(x, y) for x, y in zip(a, b)), "the order of arrival shows"
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_many_rows_shared_out(hd, dtype):
+    """Column groups of many rows whose cache blocks are divided over blocks of threads, beside
+    sequences that are not: one row, no rows, rows at the start."""
+    rng = np.random.default_rng(hd)
+    P = Pair(hd, 2, 80)
+    lens = [2500, 40, 700, 0]
+    news = [150, 1, 0, 0] if hd < 256 else [149, 3, 0, 0]
+    P.fill(rng, tables(rng, lens, 80, extra=1), lens, "f32", 0.5)
+    row = np.concatenate([[0], np.cumsum(news)]).tolist()
+    for group, window, pad in ((8, 0, 0), (9, 1500, 8), (8, 0, 1)):
+        P.batch(P.table, lens, row, row[-1] + 2)
+        P.check_attend(dtype, queries(rng, P, 2 * group, dtype), 1 / math.sqrt(hd), window, pad=pad)
 
 
 def test_tables_with_holes():
@@ -363,6 +379,9 @@ def test_tables_with_holes():
     P.check_attend("f32", queries(rng, P, 8, "f32"), 0.1)
     P.batch(t, lens, [0, 130, 133])
     P.check_attend("f16", queries(rng, P, 8, "f16"), 0.1, window=150)
+    P.batch(t, lens, [0, 500, 790])  # many rows
+    for dtype, window in (("f16", 150), ("bf16", 0), ("f32", 333)):
+        P.check_attend(dtype, queries(rng, P, 8, dtype), 0.1, window=window)
     P.batch([[-1, -1], [-1, 12]], [128, 100])  # nothing to see at all
     P.check_attend("f16", queries(rng, P, 8, "f16"), 0.1)
 
@@ -387,6 +406,7 @@ def test_scales_far_apart(kind):
         scale = 2.0 ** -58
     for dtype in ("f32", "bf16"):
         P.check_attend(dtype, q.to(TORCH[dtype]), scale)
+        P.check_attend(dtype, torch.cat([q, q, q], 1).to(TORCH[dtype]), scale)  # many rows
         P.batch([[0, 1, 2, 3, 4, 5]], [384])
         P.check_attend(dtype, q[:1].to(TORCH[dtype]), scale)
         P.batch([[0, 1, 2, 3, 4, 5]], [384], [0, 384])
@@ -405,7 +425,8 @@ def test_masked_places_hold_nothing_that_shows():
         x[150:] = 3e38
     P.write("f32", k, v)
     P.batch([[2, 4, 1]], [140], [0, 100])
-    out, _ = P.check_attend("bf16", queries(rng, P, 4, "bf16"), 0.1, window=90)
+    for n_q in (4, 12):
+        P.check_attend("bf16", queries(rng, P, n_q, "bf16"), 0.1, window=90)
     P.batch([[2, 4, 1]], [150])
     P.check_attend("f32", queries(rng, P, 4, "f32"), 0.1, window=64)
 
@@ -414,9 +435,9 @@ def test_not_finite_queries_stay_in_their_rows():
     rng = np.random.default_rng(8)
     P = Pair(64, 2, 8)
     P.fill(rng, tables(rng, [200, 130], 8), [200, 130])
-    for row in (None, [0, 70, 100]):
+    for row, n_q in ((None, 4), ([0, 70, 100], 4), ([0, 200, 330], 8)):
         P.batch(P.table, [200, 130], row)
-        q = queries(rng, P, 4, "f32")
+        q = queries(rng, P, n_q, "f32")
         good = P.attend("f32", q, 0.1)
         bad = q.clone()
         bad[1, 1, 3] = float("nan")
