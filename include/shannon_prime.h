@@ -45,7 +45,7 @@ typedef struct {
     int      use_mobius_mask;
     uint32_t k_ternary_mask;
     uint32_t v_ternary_mask;
-    int      use_fp8;    /* advisory; this library has no fp8 path (int codes) */
+    int      use_fp8;    /* advisory: the codec has int codes (8-bit blocks: sp_hip_fp8_cache_t) */
     int      vht2_norm;  /* SP_VHT2_NORM_FINAL (default) or SP_VHT2_NORM_STAGE */
 } sp_config_t;
 

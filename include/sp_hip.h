@@ -496,8 +496,8 @@ void sp_hip_fp8_cache_free(sp_hip_fp8_cache_t *c);
  * is larger its older codes are rounded again at the new scale; rows that start at a block's
  * first position begin it anew. NaN is stored as 0 and magnitudes past 448 * 2^40, infinity
  * among them, as that: what a cache holds is finite, so no position that a mask hides can
- * reach a result. Two sequences of one call must not write the same block (the result of
- * such a block is unspecified). */
+ * reach a result. A call must not reach the same block twice, from two sequences or from two
+ * entries of one (what such a block holds then is unspecified). */
 int  sp_hip_fp8_write(sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *batch, const void *d_k,
                       const void *d_v, long long row_stride, int dtype, void *stream);
 /* The batch's rows read back: code * scale, rounded to dtype. */
@@ -512,8 +512,9 @@ int  sp_hip_fp8_read(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_ba
  * of the sum of exp(kq_scale * q . K). A row that sees nothing gets zeros and -infinity.
  * The call's own positions are read from the cache: write them first. decode takes one row
  * per sequence (d_row NULL), prefill any number.
- * The workspace belongs to the cache and is allocated by init: two attention calls on one
- * cache may not overlap. Results do not depend on which block of threads finishes first. */
+ * Their workspaces belong to the cache and are allocated by init: a decode and a prefill call on
+ * one cache may overlap on two streams, two of a kind may not. Results do not depend on which
+ * block of threads finishes first. */
 int  sp_hip_fp8_attn_decode(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *batch, const void *d_q,
                             long long q_stride, int n_q, int dtype, float kq_scale, int window, void *d_out,
                             long long out_stride, float *d_lse, void *stream);

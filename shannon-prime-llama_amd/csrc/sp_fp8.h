@@ -59,7 +59,8 @@ struct SpFp8Attn {
     int window;
     float c;   // kq_scale * log2(e), not negative
     int negate;
-    float *part;    // partial results: sp_fp8_part_rows(hd) rows of hd + 4 floats
+    float *part;    // partial results: part_rows rows of hd + 4 floats
+    int part_rows;
     int *counters;  // SP_FP8_SLOTS, one per partial result, zero between calls
     int target;     // CUs; the launch makes it the blocks that fill them
     int least;      // fewest cache blocks of a share (the launch's choice)
@@ -68,9 +69,10 @@ struct SpFp8Attn {
 hipError_t sp_fp8_launch_write(const SpFp8Copy &A, int hd, int dtype, hipStream_t s);
 hipError_t sp_fp8_launch_read(const SpFp8Copy &A, int hd, int dtype, hipStream_t s);
 hipError_t sp_fp8_launch_attn(const SpFp8Attn &A, int hd, int dtype, hipStream_t s);
-// Rows of partial results: two for each CU's columns (256 of the prompt kernel's blocks, 128 at
-// head_dim 256) on 256 CUs; the kernel for few rows needs fewer.
-inline int sp_fp8_part_rows(int hd) { return hd == 256 ? 1 << 16 : 1 << 17; }
+// Rows of partial results. Shares number at most 512 (twice 256 CUs): of 32 columns in the kernel
+// for few rows, of 256 (128 at head_dim 256) in the one for many, which only prefill calls use.
+#define SP_FP8_DECODE_ROWS (512 * 32)
+inline int sp_fp8_prefill_rows(int hd) { return 512 * (hd == 256 ? 128 : 256); }
 
 #define SP_FP8_SLOTS 1024
 

@@ -104,7 +104,7 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
     if (n_seq == 1) {  // nothing to search, and no exchange between lanes
         const Extent e = extent(A, 0, cols);
         const float T = (float)e.ct * (float)e.nb * (float)A.H;
-        const int R0 = max((int)(T / (float)A.target * 1.002f) + 1, least);
+        const int R0 = max((int)min(T / (float)A.target * 1.002f, 0x1p24f) + 1, least);  // (2^24 blocks: a whole table row)
         int R = 2 * R0;
         for (int k = 2; k >= 0; k--) {
             const int r = R0 + k * R0 / 4;
@@ -125,7 +125,7 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
     }
     if (__any(bad)) return false;  // the grid was made for rows that ascend
     T = wave_sum(T) * (float)A.H;
-    const int R0 = max((int)(T / (float)A.target * 1.002f) + 1, least);
+    const int R0 = max((int)min(T / (float)A.target * 1.002f, 0x1p24f) + 1, least);  // (2^24 blocks: a whole table row)
     float n[3] = {0.0f, 0.0f, 0.0f};
     for (int i0 = 0; i0 < n_seq; i0 += 64) {
         const Extent e = i0 ? extent(A, i0 + lane, cols) : e0;
@@ -212,8 +212,8 @@ __device__ __forceinline__ void finish(const SpFp8Attn &A, long long row, int he
 }
 
 // Whether a partial result has its place (always: see find_share).
-__device__ __forceinline__ bool slot_fits(long long slot, int cols, int hd) {
-    return slot < SP_FP8_SLOTS && (slot + 1) * cols <= (hd == 256 ? 1 << 16 : 1 << 17);
+__device__ __forceinline__ bool slot_fits(const SpFp8Attn &A, long long slot, int cols) {
+    return slot < SP_FP8_SLOTS && (slot + 1) * cols <= A.part_rows;
 }
 
 // Joins partial results (m, l, o pair) in order.
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
     __syncthreads();
     const long long slot = (long long)sh.slot * A.H + h;
     const bool alone = sh.n_split == 1;
-    if (!alone && !slot_fits(slot, COLS, HD)) return;
+    if (!alone && !slot_fits(A, slot, COLS)) return;
     const int pairs = n_cols * (HD / 2);
     for (int at = tid; at < pairs; at += NT) {
         const int cc = at / (HD / 2), d = at % (HD / 2) * 2;
@@ -961,7 +961,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     const float unit = sp_fp8_pow2(ev_now);
     if (sh.n_split > 1) {  // joined by k_fp8_attn_join
         const long long slot = (long long)sh.slot * A.H + h;
-        if (active && slot_fits(slot, COLS, HD)) {
+        if (active && slot_fits(A, slot, COLS)) {
             float *dst = A.part + (slot * COLS + mycol) * ROW;
             // the maximum whose weight would be 2^P_TOP
             if (sub == 0) *reinterpret_cast<Two *>(dst + HD) = Two{m + (P_TOP - W_TOP), l};
@@ -1017,7 +1017,7 @@ __global__ __launch_bounds__(256) void k_fp8_attn_join(SpFp8Attn A) {
     Share sh;
     if (!find_share(A, blockIdx.x / A.H, threadIdx.x & 63, COLS, A.least, true, sh) || sh.n_split == 1) return;
     const long long slot0 = (long long)sh.slot * A.H + h;
-    if (!slot_fits(slot0 + (long long)(sh.n_split - 1) * A.H, COLS, HD)) return;
+    if (!slot_fits(A, slot0 + (long long)(sh.n_split - 1) * A.H, COLS)) return;
     const int c0 = sh.ct * COLS, n_cols = min(sh.n_new * A.G - c0, COLS);
     const bool aligned = (uintptr_t)A.out % (4 * sizeof(T)) == 0 && A.out_stride % 4 == 0;
     for (int at = threadIdx.x; at < 32 * PER; at += 256) {
@@ -1057,10 +1057,10 @@ __global__ __launch_bounds__(256) void k_fp8_attn_join(SpFp8Attn A) {
 }
 
 template <int HD, int DT, int NW, int CG>
-hipError_t launch(const SpFp8Attn &A, int per_cu, hipStream_t s) {
+hipError_t launch(const SpFp8Attn &A, hipStream_t s) {
     constexpr int COLS = 16 * CG;
     SpFp8Attn a = A;
-    a.target = min(A.target * per_cu, SP_FP8_SLOTS / 2);
+    a.target = min(A.target, 256);
     // column groups: each sequence's rows times G, in groups of COLS
     const long long groups = A.s.row ? ((long long)A.s.n_rows * A.G) / COLS + A.s.n_seq
                                      : (long long)A.s.n_seq * ((A.G + COLS - 1) / COLS);
@@ -1109,8 +1109,8 @@ hipError_t launch_dt(const SpFp8Attn &A, hipStream_t s) {
     // 16 / 8 heads of 256, 1 at 8K: 256 columns 53 / 62, 512 78 / 71; 12 at 1 to 4.5K: 64 69 / 65.
     constexpr int MANY = HD == 256 ? 512 : 1024;
     if (A.s.row && columns >= MANY && columns >= MANY / 8 * (long long)A.s.n_seq) return launch_wide<HD, DT>(A, s);
-    if (columns > 16ll * A.s.n_seq) return launch<HD, DT, NW, CG>(A, 1, s);
-    return launch<HD, DT, NW, 1>(A, 1, s);
+    if (columns > 16ll * A.s.n_seq) return launch<HD, DT, NW, CG>(A, s);
+    return launch<HD, DT, NW, 1>(A, s);
 }
 
 template <int HD>

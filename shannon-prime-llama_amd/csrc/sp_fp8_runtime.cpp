@@ -13,10 +13,18 @@
 
 namespace {
 
-struct Fp8Priv {
-    int device = 0, cus = 256;
+// Partial results of attention calls and the arrival counts of their shares: one for decode calls
+// and one for prefill calls, so that one of each may be under way on two streams.
+struct Workspace {
     float *part = nullptr;
     int *counters = nullptr;
+    int rows = 0;
+};
+
+struct Fp8Priv {
+    int device = 0, cus = 256;
+    void *memory = nullptr;  // codes, exponents and workspaces: one allocation
+    Workspace ws[2];
 };
 
 // The cache's device for the length of a call (the caller's current device may be another).
@@ -140,7 +148,7 @@ int copy_rows(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *
 
 int attend(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *b, const void *d_q, long long q_stride,
            int n_q, int dtype, float kq_scale, int window, void *d_out, long long out_stride, float *d_lse,
-           void *stream, const char *who) {
+           void *stream, int which, const char *who) {
     SpFp8Attn A;
     memset(&A, 0, sizeof(A));
     if (!batch_ok(c, layer, b, who, &A.s)) return -1;
@@ -181,8 +189,9 @@ int attend(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *b, 
     A.window = window >= MAX_ROWS ? 0 : window;  // no position is that far
     A.c = fabsf(kq_scale) * 1.4426950408889634f;
     A.negate = kq_scale < 0.0f;
-    A.part = pv->part;
-    A.counters = pv->counters;
+    A.part = pv->ws[which].part;
+    A.counters = pv->ws[which].counters;
+    A.part_rows = pv->ws[which].rows;
     A.target = pv->cus;
     return ok(sp_fp8_launch_attn(A, hd, dtype, s), who) ? 0 : -1;
 }
@@ -213,19 +222,35 @@ extern "C" int sp_hip_fp8_cache_init(sp_hip_fp8_cache_t *c, const sp_config_t *c
     c->stream = stream;
     c->priv = pv;
     const hipStream_t s = (hipStream_t)stream;
-    const size_t nexp = (size_t)tiles, ncode = nexp * SP_FP8_BLOCK * hd;
     bool good = ok(hipGetDevice(&pv->device), who) && stream_ok(c, s, who) &&
                 ok(hipDeviceGetAttribute(&pv->cus, hipDeviceAttributeMultiprocessorCount, pv->device), who);
-    struct Piece {
-        void **p;
-        size_t bytes;
-        int fill;  // -1: not cleared
-    } pieces[] = {{&c->d_k_codes, ncode, 0}, {&c->d_v_codes, ncode, 0},
-                  {&c->d_k_exp, nexp, 127 + SP_FP8_EMIN}, {&c->d_v_exp, nexp, 127 + SP_FP8_EMIN},
-                  {(void **)&pv->part, (size_t)sp_fp8_part_rows(hd) * (hd + 4) * sizeof(float), -1},
-                  {(void **)&pv->counters, SP_FP8_SLOTS * sizeof(int), 0}};
-    for (const Piece &p : pieces)
-        good = good && ok(hipMalloc(p.p, p.bytes), who) && (p.fill < 0 || ok(hipMemsetAsync(*p.p, p.fill, p.bytes, s), who));
+    const size_t nexp = (size_t)tiles, ncode = nexp * SP_FP8_BLOCK * hd;
+    pv->ws[0].rows = SP_FP8_DECODE_ROWS;
+    pv->ws[1].rows = sp_fp8_prefill_rows(hd);
+    size_t size = 0;
+    const auto place = [&size](size_t bytes) {
+        const size_t at = size;
+        size += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    // cleared to 0: codes and counters; to the least exponent: exponents; not cleared: partial results
+    const size_t k_at = place(ncode), v_at = place(ncode), count_at = place(2 * SP_FP8_SLOTS * sizeof(int)),
+                 ke_at = place(nexp), ve_at = place(nexp);
+    const size_t p0_at = place((size_t)pv->ws[0].rows * (hd + 4) * sizeof(float));
+    const size_t p1_at = place((size_t)pv->ws[1].rows * (hd + 4) * sizeof(float));
+    good = good && ok(hipMalloc(&pv->memory, size), who) && ok(hipMemsetAsync(pv->memory, 0, ke_at, s), who) &&
+           ok(hipMemsetAsync((char *)pv->memory + ke_at, 127 + SP_FP8_EMIN, p0_at - ke_at, s), who);
+    if (good) {
+        char *base = (char *)pv->memory;
+        c->d_k_codes = base + k_at;
+        c->d_v_codes = base + v_at;
+        c->d_k_exp = base + ke_at;
+        c->d_v_exp = base + ve_at;
+        pv->ws[0].part = (float *)(base + p0_at);
+        pv->ws[1].part = (float *)(base + p1_at);
+        pv->ws[0].counters = (int *)(base + count_at);
+        pv->ws[1].counters = pv->ws[0].counters + SP_FP8_SLOTS;
+    }
     good = good && ok(hipStreamSynchronize(s), who);
     if (!good) {
         char why[256];
@@ -243,8 +268,7 @@ extern "C" void sp_hip_fp8_cache_free(sp_hip_fp8_cache_t *c) {
     Fp8Priv *pv = (Fp8Priv *)c->priv;
     if (pv) {
         const OnDevice on(pv->device);
-        for (void *p : {c->d_k_codes, c->d_v_codes, c->d_k_exp, c->d_v_exp, (void *)pv->part, (void *)pv->counters})
-            if (p) (void)hipFree(p);
+        if (pv->memory) (void)hipFree(pv->memory);
         delete pv;
     }
     memset(c, 0, sizeof(*c));
@@ -268,12 +292,12 @@ extern "C" int sp_hip_fp8_attn_decode(const sp_hip_fp8_cache_t *c, int layer, co
         return -1;
     }
     return attend(c, layer, batch, d_q, q_stride, n_q, dtype, kq_scale, window, d_out, out_stride, d_lse, stream,
-                  "fp8_attn_decode");
+                  0, "fp8_attn_decode");
 }
 
 extern "C" int sp_hip_fp8_attn_prefill(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *batch,
                                        const void *d_q, long long q_stride, int n_q, int dtype, float kq_scale,
                                        int window, void *d_out, long long out_stride, float *d_lse, void *stream) {
     return attend(c, layer, batch, d_q, q_stride, n_q, dtype, kq_scale, window, d_out, out_stride, d_lse, stream,
-                  "fp8_attn_prefill");
+                  1, "fp8_attn_prefill");
 }

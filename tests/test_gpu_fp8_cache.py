@@ -41,6 +41,12 @@ class Pair:
                             self.keep[2].data_ptr() if row is not None else 0, self.n_rows)
         return self.b
 
+    def batch_of(self, lens, row):
+        """Another batch over the same table; the arrays of earlier ones stay."""
+        self.kept = getattr(self, "kept", []) + [self.keep]
+        self.batch(self.table, lens, row)
+        return self
+
     def set_lens(self, lens):
         self.lens = list(lens)
         self.keep[1].copy_(torch.tensor(lens, dtype=torch.int32))
@@ -594,3 +600,37 @@ def test_init_reports_what_it_cannot_have():
     torch.cuda.synchronize()
     assert S.lib().sp_hip_fp8_cache_init(C.byref(c), C.byref(S.config(128, 1, 1)), 4, None) == 0
     S.lib().sp_hip_fp8_cache_free(C.byref(c))
+
+
+def test_a_prompt_beside_a_decode_step():
+    """A prefill and a decode call on one cache at once, on two streams, both with shares to join."""
+    rng = np.random.default_rng(47)
+    P = Pair(128, 2, 300)
+    lens = [9000, 8000]
+    P.fill(rng, tables(rng, lens, 300), lens)
+    q1, q2 = queries(rng, P.batch_of(lens, [0, 300, 300]), 8, "f16"), None
+    a = P.b
+    q2 = queries(rng, P.batch_of(lens, None), 8, "f16")
+    b = P.b
+    first = [t.cuda() for t in (q1, q2)]
+    outs = [torch.zeros_like(t) for t in first]
+    L, want = S.lib(), []
+    streams = [torch.cuda.Stream() for _ in range(2)]
+
+    def call(i, stream):
+        f, batch = (L.sp_hip_fp8_attn_prefill, a) if i == 0 else (L.sp_hip_fp8_attn_decode, b)
+        S.check(f(P.dev.ref, 0, batch.ref, first[i].data_ptr(), 1024, 8, S.DTYPE_F16, 0.1, 0, outs[i].data_ptr(), 1024,
+                  None, stream), "attend")
+    torch.cuda.synchronize()
+    for i in range(2):
+        call(i, cur())
+        torch.cuda.synchronize()
+        want.append(outs[i].clone())
+    for _ in range(6):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for i in range(2):
+            call(i, streams[i].cuda_stream)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
