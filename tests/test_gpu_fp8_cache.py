@@ -367,9 +367,9 @@ def test_many_rows_shared_out(hd, dtype):
     news = [150, 1, 0, 0] if hd < 256 else [149, 3, 0, 0]
     P.fill(rng, tables(rng, lens, 80, extra=1), lens, "f32", 0.5)
     row = np.concatenate([[0], np.cumsum(news)]).tolist()
-    for group, window, pad in ((8, 0, 0), (9, 1500, 8), (8, 0, 1)):
+    for group, scale, window, pad in ((8, 1 / math.sqrt(hd), 0, 0), (9, -0.2, 1500, 8), (8, 0.0, 0, 1)):
         P.batch(P.table, lens, row, row[-1] + 2)
-        P.check_attend(dtype, queries(rng, P, 2 * group, dtype), 1 / math.sqrt(hd), window, pad=pad)
+        P.check_attend(dtype, queries(rng, P, 2 * group, dtype), scale, window, pad=pad)
 
 
 def test_tables_with_holes():
@@ -551,6 +551,43 @@ def test_captured_step_follows_lengths_and_tables():
         got = out.double().cpu().numpy(), lse.double().cpu().numpy()
         eager = P.check_attend("f16", qs, 0.1)
         assert np.array_equal(got[0], eager[0]) and np.array_equal(got[1], eager[1])
+
+
+def test_captured_chunk_follows_lengths():
+    """One graph of a chunk's write and attention, its shares joined by a second launch, replayed as
+    the sequence grows."""
+    rng = np.random.default_rng(33)
+    P = Pair(64, 2, 80)
+    table = tables(rng, [4000], 80)
+    new, n_q = 130, 16
+    P.fill(rng, table, [1500])
+    P.batch(table, [1500], [0, new])
+    k, v = (torch.zeros(new, 2, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q = torch.zeros(new, n_q, 64, dtype=torch.bfloat16, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros(new, n_q, device="cuda")
+    L = S.lib()
+
+    def step(stream):
+        S.check(L.sp_hip_fp8_write(P.dev.ref, 0, P.b.ref, k.data_ptr(), v.data_ptr(), 128, S.DTYPE_BF16, stream), "w")
+        S.check(L.sp_hip_fp8_attn_prefill(P.dev.ref, 0, P.b.ref, q.data_ptr(), n_q * 64, n_q, S.DTYPE_BF16, 0.125, 0,
+                                          out.data_ptr(), n_q * 64, lse.data_ptr(), stream), "a")
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(cur())
+    for length in (1630, 1760, 3900):
+        P.set_lens([length])
+        rows = [P.rows(rng, "bf16") for _ in range(2)]
+        qs = queries(rng, P, n_q, "bf16")
+        k.copy_(rows[0]), v.copy_(rows[1]), q.copy_(qs)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        P.ref.write(0, P.table, P.lens, P.row, new, *[x.double().numpy() for x in rows])
+        P.check_memory()
+        eager = P.check_attend("bf16", qs, 0.125)
+        assert np.array_equal(out.double().cpu().numpy(), eager[0])
+        assert np.array_equal(lse.double().cpu().numpy(), eager[1])
 
 
 def test_another_stream_and_two_caches():
