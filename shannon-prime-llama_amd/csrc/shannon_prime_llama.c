@@ -117,7 +117,7 @@ sp_llama_ctx_t *sp_llama_init_with_role(const sp_llama_params_t *params, sp_llam
     sp_llama_params_t p = *params;
     p.backend = backend;
     if (cfg.use_fp8)
-        fprintf(stderr, "[Shannon-Prime]%s SHANNON_PRIME_FP8=1 requested but this library has "
+        fprintf(stderr, "[Shannon-Prime]%s SHANNON_PRIME_FP8=1 requested but the bridge has "
                         "no fp8 path; using integer band codes.\n",
                 role == SP_LLAMA_ROLE_DRAFT ? " [draft]" : role == SP_LLAMA_ROLE_TARGET ? " [target]" : "");
     return sp_llama_init_config(&p, &cfg);

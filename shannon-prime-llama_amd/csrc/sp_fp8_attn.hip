@@ -288,7 +288,17 @@ __device__ __forceinline__ void join_shares(const SpFp8Attn &A, const Share &sh,
     }
 }
 
-// CG groups of 16 columns share each block's loads and conversions.
+// Few rows: one token a sequence, or several. A block of NW waves takes a share of the cache
+// blocks that its columns see, each wave every NW-th of them, and joins the waves' results in
+// LDS; CG groups of 16 columns share a block's loads and conversions. It is bound by memory: a
+// wave has 64 * head_dim codes of K and of V in flight and asks for the next as soon as the
+// registers are free, which takes eight waves a CU (four at head_dim 256) to keep HBM busy.
+// Measured: 2 x 131072 positions of 8 heads of 256 (1.07 GB) in 191 us, 5.6 TB/s; 16 sequences of 1 to 4K
+// of 32 heads of 96 with float32 rows (261 MB) in 54 us, 4.8 TB/s; one of 32768 of 8 heads of 128
+// (67 MB) in 18.2 us, of which the join of 32 shares takes 4 and an empty launch 4.2; 12 of 1 to
+// 4.5K with five rows each (73 MB) in 20.9 us; 777 positions of 8 heads of 64 in 7.1 us. With 16
+// waves of 128 registers the loop spills; four waves a block make more shares to join (22.0 us for
+// the 32768 where eight took 20.1 beside them).
 template <int HD, int DT, int NW, int CG>
 __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
     constexpr int COLS = 16 * CG, NC = HD / 32, ND = HD / 16, TILE = 64 * HD, ROW = HD + 2, NT = NW * 64;
@@ -537,7 +547,8 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 //          of each 32; V's operand is laid out for that order.
 //   CW 16: v_mfma_f32_16x16x32_f16. Lane (column, sub of 4) has positions 16 (i / 4) + 4 sub + i % 4.
 // A wave of 32 columns reads LDS half as often a column; one of 16 needs half of the registers,
-// which is what keeps several waves on a SIMD at head_dim 256.
+// which is what puts two waves on a SIMD at head_dim 256 (one of 32 columns took 77 us where two of
+// 16 take 61). At head_dim 128 both fit, and 32 columns win: 945 us against 1255.
 //
 // The loop is pipelined by one cache block: the next block's scores go through the matrix cores
 // among this one's weights and its product with V, so that neither unit waits for the other.
@@ -550,6 +561,13 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 // others rescale the output. In such a block weights below 2^-18 of the reference are subnormal
 // fp16 numbers, rounded at 2^-29 of it. Split weights (fp32 results) count from 2^14, their reference follows
 // within a factor of two and their unit always, so that the second part keeps its bits.
+//
+// Bound by the matrix cores and, beside them, by power: 2048 rows over 32768 positions, 32 / 8 heads
+// of 128, take 930 to 990 us by card (1.08 to 1.15 PFLOP/s; a large bf16 matrix product reaches 1.20 on
+// them), the matrix cores busy 46% of the cycles; the same loop with nothing but its matrix
+// instructions takes 595 us at a clock of 1.7 GHz. 2048 rows in a window of 1024, 16 / 8 heads of
+// 256: 61 us under the tracer, 54 in a run of calls (0.63 PFLOP/s), 18 blocks a column group with
+// 11 us before the first; LDS reads, the codes' conversion and the weights each hide a fifth of the rest.
 typedef float f16x __attribute__((ext_vector_type(16)));
 
 // LDS written before is seen after, by the whole block; loads from memory stay in flight.

@@ -10,7 +10,15 @@
 // codes belong to one block of threads and no atomic is needed. Thread items are four
 // positions by four channels: a load of four elements per position (rows stay coalesced:
 // 64 lanes cover two rows of head_dim 128), and four codes make a dword of either order
-// (K: four channels of a position, V: four positions of a channel).
+// (K: four channels of a position, V: four positions of a channel). A whole block's codes go
+// through LDS and out in 16-byte stores; a part of one is stored in dwords, and in bytes where
+// a dword of V has older positions.
+//
+// Both are bound by memory: each reads and writes what it has to once. Measured (one launch, K
+// and V): six prompts of head_dim 64, 86 MB with their float32 rows, written in 18.0 us
+// (4.8 TB/s, the rate of a large device copy); a 32K context of 8 heads of 128 read back as fp16,
+// 201 MB, in 36.2 us (5.6 TB/s); 2048 rows appended inside a block, 12.6 MB, in 7.6 us and one
+// row to each of 12 sequences in 4.9 us, where an empty launch takes 4.2.
 #include "sp_fp8.h"
 
 namespace {
