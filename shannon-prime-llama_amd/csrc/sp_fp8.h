@@ -78,9 +78,10 @@ inline int sp_fp8_prefill_rows(int hd) { return 512 * (hd == 256 ? 128 : 256); }
 
 __device__ __forceinline__ int sp_fp8_floor64(int x) { return x >> 6; }  // arithmetic: toward -inf
 
-// Rows and length of sequence i, whatever the arrays hold: 0 <= r0 <= r1 <= n_rows, len >= 0.
+// Rows and length of sequence i, whatever the arrays hold: 0 <= r0 <= r1 <= n_rows,
+// 0 <= len <= 2^30 (what the longest table row covers).
 __device__ __forceinline__ void sp_fp8_seq(const SpFp8Seqs &S, int i, int &r0, int &r1, int &len) {
-    len = max(S.len[i], 0);
+    len = min(max(S.len[i], 0), 1 << 30);
     if (S.row) {
         r0 = min(max(S.row[i], 0), S.n_rows);
         r1 = min(max(S.row[i + 1], r0), S.n_rows);

@@ -201,14 +201,14 @@ __device__ __forceinline__ float weight(float m, float M) {
 
 template <int DT>
 __device__ __forceinline__ void finish(const SpFp8Attn &A, long long row, int head, int hd, int d, float m, float l,
-                                       float o0, float o1, float p_top) {
+                                       float o0, float o1) {
     typedef typename SpFp8Elem<DT>::T T;
     T *out = reinterpret_cast<T *>(A.out) + row * A.out_stride + (long long)head * hd + d;
     const float r = l == 0.0f ? 0.0f : 1.0f / l;
     out[0] = SpFp8Elem<DT>::put(l == 0.0f ? 0.0f : o0 * r);
     out[1] = SpFp8Elem<DT>::put(l == 0.0f ? 0.0f : o1 * r);
     if (A.lse && d == 0)
-        A.lse[row * A.H * A.G + head] = l == 0.0f ? -INFINITY : (m - p_top + __log2f(l)) * 0.69314718055994531f;
+        A.lse[row * A.H * A.G + head] = l == 0.0f ? -INFINITY : (m - P_TOP + __log2f(l)) * 0.69314718055994531f;
 }
 
 // Whether a partial result has its place (always: see find_share).
@@ -283,7 +283,7 @@ __device__ __forceinline__ void join_shares(const SpFp8Attn &A, const Share &sh,
         }
         if (here && !grp) {
             const int n = c0 + cc;
-            finish<DT>(A, sh.r0 + n / A.G, h * A.G + n % A.G, HD, d, acc.M, acc.L, acc.x, acc.y, P_TOP);
+            finish<DT>(A, sh.r0 + n / A.G, h * A.G + n % A.G, HD, d, acc.M, acc.L, acc.x, acc.y);
         }
     }
 }
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
         }
         if (alone) {
             const int n = c0 + cc;
-            finish<DT>(A, sh.r0 + n / A.G, h * A.G + n % A.G, HD, d, acc.M, acc.L, acc.x, acc.y, P_TOP);
+            finish<DT>(A, sh.r0 + n / A.G, h * A.G + n % A.G, HD, d, acc.M, acc.L, acc.x, acc.y);
         } else {
             float *dst = A.part + (slot * COLS + cc) * ROW;
             if (d == 0) put_pair(dst, acc.M, acc.L);

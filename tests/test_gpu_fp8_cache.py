@@ -257,6 +257,51 @@ def test_many_sequences_and_empty_ones():
     P.check_attend("f32", q, 0.125)
 
 
+def test_many_sequences_one_long():
+    """Shares of a long sequence found behind more sequences than a wave has lanes."""
+    rng = np.random.default_rng(13)
+    P = Pair(64, 2, 330)
+    lens = [1 + (i * 29) % 130 for i in range(130)]
+    lens[97] = 5000
+    table = tables(rng, lens, 330)
+    P.fill(rng, table, lens)
+    P.batch(table, lens)
+    P.check_attend("f16", queries(rng, P, 8, "f16"), 0.2)
+    news = [min(n, 1 + i % 7) for i, n in enumerate(lens)]
+    P.batch(table, lens, np.concatenate([[0], np.cumsum(news)]).tolist(), sum(news) + 1)
+    P.check_attend("f32", queries(rng, P, 4, "f32"), 0.2, window=3000)
+
+
+def test_many_sequences_of_many_rows():
+    rng = np.random.default_rng(14)
+    lens = [40 + (i * 31) % 60 for i in range(70)]
+    lens[68] = 1900
+    P = Pair(64, 1, 190)
+    table = tables(rng, lens, 190)
+    P.fill(rng, table, lens)
+    P.batch(table, lens, [33 * i for i in range(71)])
+    for dtype in ("bf16", "f32"):
+        P.check_attend(dtype, queries(rng, P, 4, dtype), 0.2)
+
+
+def test_lengths_past_everything():
+    """Lengths at the end of an int: the table's positions are all seen, the rows' own are not there."""
+    rng = np.random.default_rng(15)
+    P = Pair(64, 1, 6)
+    P.fill(rng, [[0, 1], [2, 3, 4]], [128, 192])
+    P.batch([[0, 1, -1], [2, 3, 4]], [128, 192])
+    q = queries(rng, P, 2, "f32")
+    want = P.attend("f32", q, 0.2)
+    for row in (None, [0, 1, 2]):
+        P.batch([[0, 1, -1], [2, 3, 4]], [2 ** 31 - 1, 2 ** 30 + 7], row)
+        before = d2h(P.dev.c.d_k_codes, 6 * 64 * 64).copy()
+        k = torch.ones(2, 1, 64, device="cuda")
+        S.check(S.lib().sp_hip_fp8_write(P.dev.ref, 0, P.b.ref, k.data_ptr(), k.data_ptr(), 64, S.DTYPE_F32, cur()), "w")
+        assert np.array_equal(before, d2h(P.dev.c.d_k_codes, 6 * 64 * 64))
+        got = P.attend("f32", q, 0.2)
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
 def test_rows_array_out_of_order_touches_nothing_else():
     """An array of rows that does not ascend: within the call's rows and blocks whatever it holds."""
     rng = np.random.default_rng(4)
