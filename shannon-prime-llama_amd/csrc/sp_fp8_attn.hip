@@ -296,7 +296,7 @@ __device__ __forceinline__ void join_shares(const SpFp8Attn &A, const Share &sh,
 // Measured: 2 x 131072 positions of 8 heads of 256 (1.07 GB) in 191 us, 5.6 TB/s; 16 sequences of 1 to 4K
 // of 32 heads of 96 with float32 rows (261 MB) in 54 us, 4.8 TB/s; one of 32768 of 8 heads of 128
 // (67 MB) in 18.2 us, of which the join of 32 shares takes 4 and an empty launch 4.2; 12 of 1 to
-// 4.5K with five rows each (73 MB) in 20.9 us; 777 positions of 8 heads of 64 in 7.1 us. With 16
+// 4.5K with two to five rows each (73 MB) in 20.9 us; 777 positions of 8 heads of 64 in 7.1 us. With 16
 // waves of 128 registers the loop spills; four waves a block make more shares to join (22.0 us for
 // the 32768 where eight took 20.1 beside them).
 template <int HD, int DT, int NW, int CG>
@@ -547,8 +547,8 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 //          of each 32; V's operand is laid out for that order.
 //   CW 16: v_mfma_f32_16x16x32_f16. Lane (column, sub of 4) has positions 16 (i / 4) + 4 sub + i % 4.
 // A wave of 32 columns reads LDS half as often a column; one of 16 needs half of the registers,
-// which is what puts two waves on a SIMD at head_dim 256 (one of 32 columns took 77 us where two of
-// 16 take 61). At head_dim 128 both fit, and 32 columns win: 945 us against 1255.
+// which is what puts two waves on a SIMD at head_dim 256 (one of 32 columns takes 77 us where two of
+// 16 take 60). At head_dim 128 both fit, and 32 columns win: 907 us against 1190.
 //
 // The loop is pipelined by one cache block: the next block's scores go through the matrix cores
 // among this one's weights and its product with V, so that neither unit waits for the other.
@@ -563,10 +563,10 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 // within a factor of two and their unit always, so that the second part keeps its bits.
 //
 // Bound by the matrix cores and, beside them, by power: 2048 rows over 32768 positions, 32 / 8 heads
-// of 128, take 930 to 990 us by card (1.08 to 1.15 PFLOP/s; a large bf16 matrix product reaches 1.20 on
-// them), the matrix cores busy 46% of the cycles; the same loop with nothing but its matrix
+// of 128, take 890 us in a row of calls (1.2 PFLOP/s; a large bf16 matrix product reaches 1.19 to 1.24, by
+// card) and 960 alone, the matrix cores busy 51% of the cycles; the same loop with nothing but its matrix
 // instructions takes 595 us at a clock of 1.7 GHz. 2048 rows in a window of 1024, 16 / 8 heads of
-// 256: 61 us under the tracer, 54 in a run of calls (0.63 PFLOP/s), 18 blocks a column group with
+// 256: 59 us under the tracer, 52 in a run of calls (0.66 PFLOP/s), 18 blocks a column group with
 // 11 us before the first; LDS reads, the codes' conversion and the weights each hide a fifth of the rest.
 typedef float f16x __attribute__((ext_vector_type(16)));
 
@@ -1113,8 +1113,8 @@ hipError_t launch_wide(const SpFp8Attn &A, hipStream_t s) {
     SpFp8Attn a = A;
     a.target = min(A.target, 256);
     const long long groups = (long long)A.s.n_rows * A.G / COLS + A.s.n_seq;
-    // With twice the blocks that the chip takes, sharing gains nothing. Below that a group is shared
-    // out where the others leave CUs idle, and a second launch joins the shares.
+    // With a block for each CU sharing gains nothing. Below that a group is shared out where the
+    // others leave CUs idle, and a second launch joins the shares.
     const bool share = groups * A.H < a.target;
     a.least = share ? 4 : 1 << 28;
     const long long blocks = (groups + (share ? (a.target + A.H - 1) / A.H : 0)) * A.H;
@@ -1137,10 +1137,10 @@ hipError_t launch_dt(const SpFp8Attn &A, hipStream_t s) {
     // The kernel for many rows takes a cache block over 256 columns at once (128 at head_dim 256), this
     // one over 32 (16) and reads it again for the next. Measured, few rows / many, 32 / 8 heads of 128:
     //   columns a sequence   64            128           256           512          1024
-    //   1 sequence at 8K     27 / 41 us                  30 / 51       41 / 50      60 / 65
-    //   3 at 2 to 8K                                     41 / 50       77 / 63
-    //   12 at 1 to 4.5K      32 / 48       54 / 53       75 / 71
-    // 16 / 8 heads of 256, 1 at 8K: 256 columns 53 / 62, 512 78 / 71; 12 at 1 to 4.5K: 64 69 / 65.
+    //   1 sequence at 8K     27 / 41 us                  30 / 51       41 / 50      61 / 63
+    //   3 at 2 to 8K                                     42 / 49       78 / 61
+    //   12 at 1 to 4.5K      32 / 48       54 / 51       75 / 67
+    // 16 / 8 heads of 256, 1 at 8K: 256 columns 51 / 61, 512 75 / 69; 12 at 1 to 4.5K: 64 68 / 63.
     constexpr int MANY = HD == 256 ? 512 : 1024;
     if (A.s.row && columns >= MANY && columns >= MANY / 8 * (long long)A.s.n_seq) return launch_wide<HD, DT>(A, s);
     if (columns > 16ll * A.s.n_seq) return launch<HD, DT, NW, CG>(A, s);
