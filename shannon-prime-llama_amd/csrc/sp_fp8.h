@@ -70,7 +70,7 @@ hipError_t sp_fp8_launch_write(const SpFp8Copy &A, int hd, int dtype, hipStream_
 hipError_t sp_fp8_launch_read(const SpFp8Copy &A, int hd, int dtype, hipStream_t s);
 hipError_t sp_fp8_launch_attn(const SpFp8Attn &A, int hd, int dtype, hipStream_t s);
 // Rows of partial results. Shares number at most 512 (twice 256 CUs): of 32 columns in the kernel
-// for few rows, of 256 (128 at head_dim 256) in the one for many, which only prefill calls use.
+// for few rows, of at most 256 (128 at head_dim 256) in the one for many, which only prefill calls use.
 #define SP_FP8_DECODE_ROWS (512 * 32)
 inline int sp_fp8_prefill_rows(int hd) { return 512 * (hd == 256 ? 128 : 256); }
 

@@ -548,7 +548,10 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 //   CW 16: v_mfma_f32_16x16x32_f16. Lane (column, sub of 4) has positions 16 (i / 4) + 4 sub + i % 4.
 // A wave of 32 columns reads LDS half as often a column; one of 16 needs half of the registers,
 // which is what puts two waves on a SIMD at head_dim 256 (one of 32 columns takes 77 us where two of
-// 16 take 60). At head_dim 128 both fit, and 32 columns win: 907 us against 1190.
+// 16 take 60; with float32 rows 2048 over 8000, 32 / 8 heads, 1050 where they take 757). At head_dim
+// 128 both fit, and 32 columns win: 907 us against 1190. With float32 rows there, which take twice
+// the queries and weights, 16 win up to 8K (2048 rows 86 us for 106, 12 sequences of 256 rows 242
+// for 271, 512 rows over 8000 134 for 135), 32 beyond (2048 over 32000 1516 for 1653): 16 it is.
 //
 // The loop is pipelined by one cache block: the next block's scores go through the matrix cores
 // among this one's weights and its product with V, so that neither unit waits for the other.
@@ -1040,10 +1043,16 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
 
 // Joins the shares of the column groups that have more than one, in their order. A launch of its
 // own: a group's partial results are 64 to 128 KB a share, too many for the last block to
-// arrive alone. Blocks of threads: (KV head, column group) by 32 columns.
+// arrive alone. Blocks of threads: (KV head, column group) by as many columns as 256 threads take
+// at once, four channels each (with 32 columns a block, four to eight rounds of dependent loads:
+// 1250 rows over 8930 positions of one head of 256 took 67 us, not 39).
+template <int HD>
+constexpr int JOIN_COLS = HD == 64 ? 16 : HD == 256 ? 4 : 8;
+
 template <int HD, int DT, int COLS>
 __global__ __launch_bounds__(256) void k_fp8_attn_join(SpFp8Attn A) {
     constexpr int ROW = HD + 4, PER = HD / 4;
+    static_assert(JOIN_COLS<HD> * PER <= 256 && COLS % JOIN_COLS<HD> == 0);
     typedef typename SpFp8Elem<DT>::T T;
     const int h = blockIdx.x % A.H;
     Share sh;
@@ -1052,40 +1061,38 @@ __global__ __launch_bounds__(256) void k_fp8_attn_join(SpFp8Attn A) {
     if (!slot_fits(A, slot0 + (long long)(sh.n_split - 1) * A.H, COLS)) return;
     const int c0 = sh.ct * COLS, n_cols = min(sh.n_new * A.G - c0, COLS);
     const bool aligned = (uintptr_t)A.out % (4 * sizeof(T)) == 0 && A.out_stride % 4 == 0;
-    for (int at = threadIdx.x; at < 32 * PER; at += 256) {
-        const int c = blockIdx.y * 32 + at / PER, d = at % PER * 4;
-        if (c >= n_cols) return;
-        const float *src = A.part + (slot0 * COLS + c) * ROW;
-        const long long step = (long long)A.H * COLS * ROW;
-        float M = -INFINITY, L = 0.0f;
-        f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int v0 = 0; v0 < sh.n_split; v0 += 8) {
-            Two ml[8];
-            f4 part[8];
+    const int c = blockIdx.y * JOIN_COLS<HD> + threadIdx.x / PER, d = threadIdx.x % PER * 4;
+    if ((int)threadIdx.x >= JOIN_COLS<HD> * PER || c >= n_cols) return;
+    const float *src = A.part + (slot0 * COLS + c) * ROW;
+    const long long step = (long long)A.H * COLS * ROW;
+    float M = -INFINITY, L = 0.0f;
+    f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int v0 = 0; v0 < sh.n_split; v0 += 8) {
+        Two ml[8];
+        f4 part[8];
 #pragma unroll
-            for (int v = 0; v < 8; v++) {
-                const float *rec = src + min(v0 + v, sh.n_split - 1) * step;
-                ml[v] = *reinterpret_cast<const Two *>(rec + HD);
-                part[v] = *reinterpret_cast<const f4 *>(rec + d);
-            }
-#pragma unroll
-            for (int v = 0; v < 8; v++)
-                if (v0 + v < sh.n_split) {
-                    const float Mn = fmaxf(M, ml[v].x), a = weight(M, Mn), b = weight(ml[v].x, Mn);
-                    L = L * a + ml[v].y * b;
-                    x = x * a + part[v] * b;
-                    M = Mn;
-                }
+        for (int v = 0; v < 8; v++) {
+            const float *rec = src + min(v0 + v, sh.n_split - 1) * step;
+            ml[v] = *reinterpret_cast<const Two *>(rec + HD);
+            part[v] = *reinterpret_cast<const f4 *>(rec + d);
         }
-        const int nn = c0 + c, head = h * A.G + nn % A.G;
-        const long long row = (long long)sh.r0 + nn / A.G;
-        const float r = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = L == 0.0f ? 0.0f : x[j] * r;
-        store4<DT>(A.out, row * A.out_stride + (long long)head * HD + d, x, aligned);
-        if (A.lse && d == 0)
-            A.lse[row * A.H * A.G + head] = L == 0.0f ? -INFINITY : (M - P_TOP + __log2f(L)) * 0.69314718055994531f;
+        for (int v = 0; v < 8; v++)
+            if (v0 + v < sh.n_split) {
+                const float Mn = fmaxf(M, ml[v].x), a = weight(M, Mn), b = weight(ml[v].x, Mn);
+                L = L * a + ml[v].y * b;
+                x = x * a + part[v] * b;
+                M = Mn;
+            }
     }
+    const int nn = c0 + c, head = h * A.G + nn % A.G;
+    const long long row = (long long)sh.r0 + nn / A.G;
+    const float r = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[j] = L == 0.0f ? 0.0f : x[j] * r;
+    store4<DT>(A.out, row * A.out_stride + (long long)head * HD + d, x, aligned);
+    if (A.lse && d == 0)
+        A.lse[row * A.H * A.G + head] = L == 0.0f ? -INFINITY : (M - P_TOP + __log2f(L)) * 0.69314718055994531f;
 }
 
 template <int HD, int DT, int NW, int CG>
@@ -1108,23 +1115,26 @@ hipError_t launch(const SpFp8Attn &A, hipStream_t s) {
 
 template <int HD, int DT>
 hipError_t launch_wide(const SpFp8Attn &A, hipStream_t s) {
-    constexpr int CW = HD == 256 && DT != SP_DTYPE_F32 ? 16 : 32, NW = HD == 256 && DT == SP_DTYPE_F32 ? 4 : 8;
+    constexpr int CW = HD == 256 || (HD == 128 && DT == SP_DTYPE_F32) ? 16 : 32, NW = 8;
     constexpr int COLS = CW * NW;
     SpFp8Attn a = A;
     a.target = min(A.target, 256);
     const long long groups = (long long)A.s.n_rows * A.G / COLS + A.s.n_seq;
     // With a block for each CU sharing gains nothing. Below that a group is shared out where the
     // others leave CUs idle, and a second launch joins the shares.
-    const bool share = groups * A.H < a.target;
-    a.least = share ? 4 : 1 << 28;
+    // (No sequence's rows see more than `most` cache blocks; up to 4 * least are not shared out.)
+    constexpr int LEAST = 4;
+    const long long most = A.window > 0 ? min((long long)A.s.stride, ((long long)A.s.n_rows + A.window + 126) / 64) : A.s.stride;
+    const bool share = groups * A.H < a.target && most > 4 * LEAST;
+    a.least = share ? LEAST : 1 << 28;
     const long long blocks = (groups + (share ? (a.target + A.H - 1) / A.H : 0)) * A.H;
     if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
     void *args[] = {&a};
     const hipError_t e = hipLaunchKernel((const void *)k_fp8_attn_wide<HD, DT, NW, CW>, dim3((unsigned)blocks), dim3(NW * 64),
                                          args, (size_t)HD * 512, s);
     if (e != hipSuccess || !share) return e;
-    return hipLaunchKernel((const void *)k_fp8_attn_join<HD, DT, COLS>, dim3((unsigned)(groups * A.H), COLS / 32), dim3(256), args,
-                           0, s);
+    return hipLaunchKernel((const void *)k_fp8_attn_join<HD, DT, COLS>, dim3((unsigned)(groups * A.H), COLS / JOIN_COLS<HD>),
+                           dim3(256), args, 0, s);
 }
 
 template <int HD, int DT>
@@ -1134,15 +1144,23 @@ hipError_t launch_dt(const SpFp8Attn &A, hipStream_t s) {
     // 4.5K, 32 columns each: head_dim 256 48 us with 16 and 80 with 32, fp32 rows at 128 26 and 45).
     constexpr int CG = HD == 256 || DT == SP_DTYPE_F32 ? 1 : 2;
     const long long columns = (long long)A.s.n_rows * A.G;  // of each KV head
-    // The kernel for many rows takes a cache block over 256 columns at once (128 at head_dim 256), this
-    // one over 32 (16) and reads it again for the next. Measured, few rows / many, 32 / 8 heads of 128:
-    //   columns a sequence   64            128           256           512          1024
-    //   1 sequence at 8K     27 / 41 us                  30 / 51       41 / 50      61 / 63
-    //   3 at 2 to 8K                                     42 / 49       78 / 61
-    //   12 at 1 to 4.5K      32 / 48       54 / 51       75 / 67
-    // 16 / 8 heads of 256, 1 at 8K: 256 columns 51 / 61, 512 75 / 69; 12 at 1 to 4.5K: 64 68 / 63.
-    constexpr int MANY = HD == 256 ? 512 : 1024;
-    if (A.s.row && columns >= MANY && columns >= MANY / 8 * (long long)A.s.n_seq) return launch_wide<HD, DT>(A, s);
+    // The kernel for many rows takes a cache block over 256 columns at once (128 in waves of 16), this
+    // one over 32 or 16 and reads it again for the next. Measured, few rows / many in us, 8 KV heads,
+    // 4 query heads each, bf16 (f32); batches are ragged, with two thirds of the columns named:
+    //   columns a sequence            64         128        256               512                1024
+    //   head_dim 128, 1 at 8K                    24 / 29    30 / 36 (33/37)   41 / 43 (50/52)    60 / 60
+    //                 1 at 32K                   42 / 46    64 / 63 (93/85)   109 / 96 (163/137)
+    //                 12 at 1 to 4.5K 32 / 47    53 / 51 (62/61)  74 / 69 (104/101)
+    //   head_dim 64,  1 at 8K                    17 / 23    21 / 28 (24/32)   30 / 32 (35/39)    45 / 43 (66/56)
+    //                 1 at 32K                   30 / 36    47 / 43 (62/56)   79 / 63 (110/88)
+    //                 12 at 1 to 4.5K 22 / 35    39 / 37 (42/45)  52 / 48 (70/62)
+    //   head_dim 256, 1 at 8K         29 / 29    36 / 36 (40/46)  50 / 43 (61/60)   73 / 61 (99/91)
+    //                 1 at 32K        59 / 50    85 / 66    142 / 101 (178/146)
+    //                 12 at 1 to 4.5K 68 / 58    92 / 74 (109/112)  149 / 119 (180/181)
+    //                 24, 40 alike    102 / 131, 122 / 137    202 / 173 (40)
+    constexpr bool F32 = DT == SP_DTYPE_F32;
+    constexpr int MANY = HD < 256 ? 512 : F32 ? 256 : 128, EACH = F32 ? 128 : 64;
+    if (A.s.row && columns >= MANY && columns >= EACH * (long long)A.s.n_seq) return launch_wide<HD, DT>(A, s);
     if (columns > 16ll * A.s.n_seq) return launch<HD, DT, NW, CG>(A, s);
     return launch<HD, DT, NW, 1>(A, s);
 }
