@@ -64,6 +64,7 @@ struct SpFp8Attn {
     int *counters;  // SP_FP8_SLOTS, one per partial result, zero between calls
     int target;     // CUs; the launch makes it the blocks that fill them
     int least;      // fewest cache blocks of a share (the launch's choice)
+    float join;     // rounds in which a block of threads joins shares (the launch's)
 };
 
 hipError_t sp_fp8_launch_write(const SpFp8Copy &A, int hd, int dtype, hipStream_t s);

@@ -90,6 +90,14 @@ __device__ __forceinline__ int shares_of(int nb, int R, int least) {
     return nb <= 4 * least ? 1 : (nb + R - 1) / R;
 }
 
+// Fewest cache blocks of a share: what makes `target` of them, but where few groups are cut into
+// many shares no less than costs least. n blocks in n / R shares take the time of R / 8 blocks, a wave
+// each, and then of n / R shares' partial results, eight loaded at once, in A.join rounds.
+__device__ __forceinline__ int first_share(const SpFp8Attn &A, float T, float mean, int least) {
+    const float even = min(T / (float)A.target * 1.002f, 0x1p24f);  // (2^24 blocks: a whole table row)
+    return max(max((int)even + 1, (int)__builtin_sqrtf(min(mean, 0x1p24f) * A.join)), least);
+}
+
 // The work is divided on the device, so that lengths may change under a captured call. With T
 // the blocks that all column groups see, a column group of n blocks gets ceil(n / R) shares,
 // R the first of R0, 5/4 R0, 3/2 R0 and 2 R0, R0 > T / target, that makes at most `target`
@@ -104,7 +112,7 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
     if (n_seq == 1) {  // nothing to search, and no exchange between lanes
         const Extent e = extent(A, 0, cols);
         const float T = (float)e.ct * (float)e.nb * (float)A.H;
-        const int R0 = max((int)min(T / (float)A.target * 1.002f, 0x1p24f) + 1, least);  // (2^24 blocks: a whole table row)
+        const int R0 = first_share(A, T, (float)e.nb, least);
         int R = 2 * R0;
         for (int k = 2; k >= 0; k--) {
             const int r = R0 + k * R0 / 4;
@@ -116,16 +124,17 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
         return !e.bad && item < e.ct * ns;
     }
     const Extent e0 = extent(A, lane, cols);  // kept: up to 64 sequences are read once
-    float T = (float)e0.ct * (float)e0.nb;
+    float T = (float)e0.ct * (float)e0.nb, groups = (float)e0.ct;
     bool bad = e0.bad;
     for (int i0 = 64; i0 < n_seq; i0 += 64) {
         const Extent e = extent(A, i0 + lane, cols);
         T += (float)e.ct * (float)e.nb;
+        groups += (float)e.ct;
         bad = bad || e.bad;
     }
     if (__any(bad)) return false;  // the grid was made for rows that ascend
     T = wave_sum(T) * (float)A.H;
-    const int R0 = max((int)min(T / (float)A.target * 1.002f, 0x1p24f) + 1, least);  // (2^24 blocks: a whole table row)
+    const int R0 = first_share(A, T, T / fmaxf(wave_sum(groups) * (float)A.H, 1.0f), least);
     float n[3] = {0.0f, 0.0f, 0.0f};
     for (int i0 = 0; i0 < n_seq; i0 += 64) {
         const Extent e = i0 ? extent(A, i0 + lane, cols) : e0;
@@ -1108,6 +1117,8 @@ hipError_t launch(const SpFp8Attn &A, hipStream_t s) {
     if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
     const int cols = A.s.row ? COLS : (A.G < COLS ? A.G : COLS);
     const size_t lds = (size_t)NW * cols * (HD + 4) * sizeof(float);
+    const long long each = A.s.row ? ((long long)A.s.n_rows * A.G + A.s.n_seq - 1) / A.s.n_seq : A.G;
+    a.join = (float)min(each, (long long)COLS) * (HD / 2) / (NW * 64);
     void *args[] = {&a};
     const void *f = (const void *)k_fp8_attn<HD, DT, NW, CG>;
     return hipLaunchKernel(f, dim3((unsigned)blocks), dim3(NW * 64), args, lds, s);
@@ -1122,11 +1133,14 @@ hipError_t launch_wide(const SpFp8Attn &A, hipStream_t s) {
     const long long groups = (long long)A.s.n_rows * A.G / COLS + A.s.n_seq;
     // With a block for each CU sharing gains nothing. Below that a group is shared out where the
     // others leave CUs idle, and a second launch joins the shares.
-    // (No sequence's rows see more than `most` cache blocks; up to 4 * least are not shared out.)
-    constexpr int LEAST = 4;
+    // (No sequence's rows see more than `most` cache blocks; up to 4 * LEAST are not shared out. Waves
+    // of 16 columns take two blocks a share: 512 rows over 768 positions of one head of 256 20 us for 34;
+    // of 32 they are the slower ones, 1024 rows from position 0 of 8 heads of 128 44 us for 40.)
+    constexpr int LEAST = CW == 16 ? 2 : 4;
     const long long most = A.window > 0 ? min((long long)A.s.stride, ((long long)A.s.n_rows + A.window + 126) / 64) : A.s.stride;
     const bool share = groups * A.H < a.target && most > 4 * LEAST;
     a.least = share ? LEAST : 1 << 28;
+    a.join = 0.0f;
     const long long blocks = (groups + (share ? (a.target + A.H - 1) / A.H : 0)) * A.H;
     if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
     void *args[] = {&a};
@@ -1145,22 +1159,31 @@ hipError_t launch_dt(const SpFp8Attn &A, hipStream_t s) {
     constexpr int CG = HD == 256 || DT == SP_DTYPE_F32 ? 1 : 2;
     const long long columns = (long long)A.s.n_rows * A.G;  // of each KV head
     // The kernel for many rows takes a cache block over 256 columns at once (128 in waves of 16), this
-    // one over 32 or 16 and reads it again for the next. Measured, few rows / many in us, 8 KV heads,
-    // 4 query heads each, bf16 (f32); batches are ragged, with two thirds of the columns named:
-    //   columns a sequence            64         128        256               512                1024
-    //   head_dim 128, 1 at 8K                    24 / 29    30 / 36 (33/37)   41 / 43 (50/52)    60 / 60
-    //                 1 at 32K                   42 / 46    64 / 63 (93/85)   109 / 96 (163/137)
-    //                 12 at 1 to 4.5K 32 / 47    53 / 51 (62/61)  74 / 69 (104/101)
-    //   head_dim 64,  1 at 8K                    17 / 23    21 / 28 (24/32)   30 / 32 (35/39)    45 / 43 (66/56)
-    //                 1 at 32K                   30 / 36    47 / 43 (62/56)   79 / 63 (110/88)
-    //                 12 at 1 to 4.5K 22 / 35    39 / 37 (42/45)  52 / 48 (70/62)
-    //   head_dim 256, 1 at 8K         29 / 29    36 / 36 (40/46)  50 / 43 (61/60)   73 / 61 (99/91)
-    //                 1 at 32K        59 / 50    85 / 66    142 / 101 (178/146)
-    //                 12 at 1 to 4.5K 68 / 58    92 / 74 (109/112)  149 / 119 (180/181)
-    //                 24, 40 alike    102 / 131, 122 / 137    202 / 173 (40)
+    // one over 32 or 16 and reads it again for the next. What decides is how many columns there are over
+    // all KV heads (a few blocks of threads with many columns each leave the chip idle) and how many a
+    // sequence has (columns that none has are worked through). The longer the context the better for
+    // the other, but the host does not know it. Measured, few rows / many in us, one sequence:
+    //   columns x heads              4096        8192        16384       32768
+    //   head_dim 64     from 0       8 / 10      8 / 13      15 / 18     33 / 28
+    //                   over 8K      30 / 32     45 / 43
+    //   head_dim 128    from 0       11 / 14     12 / 18     24 / 25     51 / 40
+    //                   over 8K      41 / 43     60 / 60
+    //                   over 32K     109 / 96
+    //     one head, two from 0       15 / 22     23 / 32
+    //     one head, two over 8K      42 / 43     59 / 56
+    //     float32 rows  from 0                   16 / 17     34 / 26     74 / 43
+    //                   over 8K      50 / 52
+    //   head_dim 256    from 0       11 / 15     20 / 20     44 / 29     103 / 48
+    //                   over 8K      73 / 61     138 / 95
+    //     one head, two over 8K      74 / 60     130 / 93
+    //     float32 rows  from 0                   25 / 31     52 / 46     122 / 74
+    //                   over 8K      99 / 91
+    // Twelve sequences of 1 to 4.5K, 8 heads, 42 / 84 / 168 columns each: head_dim 64 22 / 35, 39 / 37,
+    // 52 / 48; 128 32 / 47, 53 / 51, 74 / 69, float32 rows -, 62 / 61, 104 / 101; 256 68 / 58, 92 / 74,
+    // 149 / 119; 24 and 40 sequences of 256 with 42 columns 102 / 131, 122 / 137.
     constexpr bool F32 = DT == SP_DTYPE_F32;
-    constexpr int MANY = HD < 256 ? 512 : F32 ? 256 : 128, EACH = F32 ? 128 : 64;
-    if (A.s.row && columns >= MANY && columns >= EACH * (long long)A.s.n_seq) return launch_wide<HD, DT>(A, s);
+    constexpr int MANY = HD == 256 ? 4096 : HD == 128 && F32 ? 8192 : 12288, EACH = F32 ? 128 : 64;
+    if (A.s.row && columns * A.H >= MANY && columns >= EACH * (long long)A.s.n_seq) return launch_wide<HD, DT>(A, s);
     if (columns > 16ll * A.s.n_seq) return launch<HD, DT, NW, CG>(A, s);
     return launch<HD, DT, NW, 1>(A, s);
 }

@@ -533,6 +533,145 @@ def test_blocks_past_4_gib():
     P.dev.free()
 
 
+# ---- rows enough for the kernel that takes a block over many columns (columns of all KV heads) ----
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("window", [0, 77])
+def test_many_columns(hd, dtype, window):
+    rng = np.random.default_rng(hd + 9)
+    P = Pair(hd, 4, 20)
+    lens, news = [1, 0, 500, 129, 65, 63], [1, 0, 437, 64, 0, 70]  # the last: more rows than positions
+    P.fill(rng, tables(rng, lens, 20, extra=1), lens, "f32", 0.5)
+    row = np.concatenate([[0], np.cumsum(news)]).tolist()
+    for group, scale, kw in ((6, 1 / math.sqrt(hd), {}), (7, -0.3, dict(pad=3, shift=1)), (6, 0.0, dict(pad=8))):
+        P.batch(P.table, lens, row, row[-1] + 3)
+        P.check_attend(dtype, queries(rng, P, 4 * group, dtype), scale, window, **kw)
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_many_columns_shared_out(hd, dtype):
+    rng = np.random.default_rng(hd + 1)
+    P = Pair(hd, 2, 80)
+    lens, news = [2500, 40, 700, 0], [450, 1, 0, 0]
+    P.fill(rng, tables(rng, lens, 80, extra=1), lens, "f32", 0.5)
+    row = np.concatenate([[0], np.cumsum(news)]).tolist()
+    for window, pad in ((0, 0), (1500, 1)):
+        P.batch(P.table, lens, row, row[-1] + 2)
+        q = queries(rng, P, 28, dtype)
+        a = P.check_attend(dtype, q, 1 / math.sqrt(hd), window, pad=pad)
+    b = P.attend(dtype, q, 1 / math.sqrt(hd), window, pad=pad)
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+def test_many_columns_of_many_sequences():
+    rng = np.random.default_rng(14)
+    lens = [40 + (i * 31) % 60 for i in range(70)]
+    lens[68] = 1900
+    P = Pair(64, 4, 190)
+    table = tables(rng, lens, 190)
+    P.fill(rng, table, lens)
+    P.batch(table, lens, [33 * i for i in range(71)])
+    for dtype in ("bf16", "f32"):
+        P.check_attend(dtype, queries(rng, P, 16, dtype), 0.2)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+def test_many_columns_over_holes(hd):
+    rng = np.random.default_rng(12)
+    P = Pair(hd, 8, 12)
+    lens = [640, 300]
+    P.fill(rng, tables(rng, lens, 12, extra=-1), [576, 256])
+    t = [list(x) for x in P.table]
+    t[0] = t[0][:9] + [-1]
+    t[0][3], t[0][8] = -1, 99
+    t[1] = [12, -5, 1 << 30, t[1][2]] + [-1]
+    P.batch(t, lens, [0, 500, 790])
+    for dtype, window in (("f16", 150), ("bf16", 0), ("f32", 333)):
+        P.check_attend(dtype, queries(rng, P, 16, dtype), 0.1, window=window)
+    P.batch([[-1, -1], [-1, 12]], [500, 400], [0, 500, 900])  # nothing to see at all
+    P.check_attend("f16", queries(rng, P, 16, "f16"), 0.1)
+
+
+@pytest.mark.parametrize("kind", ["v", "k", "q"])
+def test_many_columns_scales_far_apart(kind):
+    rng = np.random.default_rng(2)
+    for hd in (64, 128):
+        P = Pair(hd, 1, 10)
+        P.batch([[0, 1, 2, 3, 4, 5]], [384], [0, 384])
+        k, v = P.rows(rng, "f32", 0.0), P.rows(rng, "f32", 0.0)
+        k *= 0.1
+        for j, e in enumerate((30, -35, 0, 35, -30, 4)):
+            (v if kind == "v" else k)[64 * j:64 * j + 64] *= 2.0 ** (e if kind == "v" else e / 8 - 4)
+        if kind == "v":
+            k[64:128] += 1.0
+        P.write("f32", k, v)
+        q = torch.from_numpy(np.abs(rng.standard_normal((384, 32, hd))))
+        scale = 0.5 * 64 / hd
+        if kind == "q":
+            q = q / q.abs().amax(-1, keepdim=True) * 2.0 ** 60
+            scale *= 2.0 ** -57
+        for dtype in ("f32", "bf16"):
+            P.check_attend(dtype, q.to(TORCH[dtype]), scale)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_many_columns_not_finite(hd):
+    """Queries that are not finite stay in their rows, what was written as such in masked places
+    does not show."""
+    rng = np.random.default_rng(8)
+    P = Pair(hd, 4, 8)
+    row = [0, 200, 330]
+    P.batch(tables(rng, [250, 130], 8), [250, 130], [0, 250, 380])
+    k, v = P.rows(rng, "f32", 0.3), P.rows(rng, "f32", 0.3)
+    for x in (k, v):
+        x[:20], x[20:30], x[240:250] = float("inf"), float("nan"), 3e38
+    P.write("f32", k, v)
+    P.batch(P.table, [240, 130], row)
+    for dtype in ("f32", "bf16"):
+        q = queries(rng, P, 40, dtype)
+        good = P.check_attend(dtype, q, 0.1, window=10)
+        bad = q.clone()
+        bad[1, 1, 3] = float("nan")
+        bad[0, 2, 5] = float("inf")
+        got = P.attend(dtype, bad, 0.1, window=10)
+        same = np.ones(q.shape[:2], bool)
+        same[1, 1] = same[0, 2] = False
+        assert np.array_equal(got[0][same], good[0][same]) and np.array_equal(got[1][same], good[1][same])
+        assert np.isnan(got[0][1, 1]).all() and np.isnan(got[1][1, 1])
+        assert not np.isfinite(got[0][0, 2]).any()
+
+
+def test_captured_chunk_of_many_columns():
+    """One graph of a chunk's attention, its shares joined by a second launch, replayed over more
+    of a sequence that is there already."""
+    rng = np.random.default_rng(34)
+    P = Pair(64, 2, 80)
+    table = tables(rng, [4000], 80)
+    new, n_q = 130, 96
+    P.fill(rng, table, [4000])
+    P.batch(table, [1500], [0, new])
+    q = queries(rng, P, n_q, "bf16").cuda()
+    out, lse = torch.zeros_like(q), torch.zeros(new, n_q, device="cuda")
+
+    def step(stream):
+        S.check(S.lib().sp_hip_fp8_attn_prefill(P.dev.ref, 0, P.b.ref, q.data_ptr(), n_q * 64, n_q, S.DTYPE_BF16, 0.125,
+                                                0, out.data_ptr(), n_q * 64, lse.data_ptr(), stream), "a")
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(cur())
+    for length in (1630, 200, 3900):
+        P.set_lens([length])
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = P.check_attend("bf16", q.cpu(), 0.125)
+        assert np.array_equal(out.double().cpu().numpy(), eager[0])
+        assert np.array_equal(lse.double().cpu().numpy(), eager[1])
+
+
 # ---- as a server uses them ----
 
 def test_a_prompt_then_steps_then_proposals():
