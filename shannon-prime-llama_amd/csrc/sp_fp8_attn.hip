@@ -86,23 +86,27 @@ __device__ __forceinline__ Extent extent(const SpFp8Attn &A, int i, int cols) {
     }
     return e;
 }
-__device__ __forceinline__ int shares_of(int nb, int R, int least) {
-    return nb <= 4 * least ? 1 : (nb + R - 1) / R;
+__device__ __forceinline__ int shares_of(int nb, int R, int alone) {
+    return nb <= alone ? 1 : (nb + R - 1) / R;
 }
 
 // Fewest cache blocks of a share: what makes `target` of them, but where few groups are cut into
 // many shares no less than costs least. n blocks in n / R shares take the time of R / 8 blocks, a wave
-// each, and then of n / R shares' partial results, eight loaded at once, in A.join rounds.
-__device__ __forceinline__ int first_share(const SpFp8Attn &A, float T, float mean, int least) {
+// each, and then of n / R shares' partial results, eight loaded at once, in A.join rounds: R is the
+// root of n A.join (16 rows over 32000 positions of two heads of 128 take 36 us, where `target` shares
+// took 50; four rows of one head 23 for 43). alone: blocks up to which a group is not shared out.
+__device__ __forceinline__ int first_share(const SpFp8Attn &A, float T, float mean, int least, int &alone) {
     const float even = min(T / (float)A.target * 1.002f, 0x1p24f);  // (2^24 blocks: a whole table row)
-    return max(max((int)even + 1, (int)__builtin_sqrtf(min(mean, 0x1p24f) * A.join)), least);
+    const int cheap = (int)__builtin_sqrtf(min(mean, 0x1p24f) * A.join);
+    alone = max(4 * least, 2 * cheap);
+    return max(max((int)even + 1, cheap), least);
 }
 
 // The work is divided on the device, so that lengths may change under a captured call. With T
 // the blocks that all column groups see, a column group of n blocks gets ceil(n / R) shares,
 // R the first of R0, 5/4 R0, 3/2 R0 and 2 R0, R0 > T / target, that makes at most `target`
-// shares, if one does. R is at least `least`, and up to four times that is not shared out: a
-// share's own waves join their results in LDS, which costs less than the stores, the count and
+// shares, if one does. R is at least `least`, and up to four times that (or `alone`) is not shared out:
+// a share's own waves join their results in LDS, which costs less than the stores, the count and
 // the loads (three memory latencies) that join shares. Groups of two or more shares (n > R, so
 // ceil(n / R) < 2 n / R) have at most 2 T / R < 2 target shares, which bounds the partial
 // results. by_group: `item` counts column groups, and their first shares are found.
@@ -112,13 +116,14 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
     if (n_seq == 1) {  // nothing to search, and no exchange between lanes
         const Extent e = extent(A, 0, cols);
         const float T = (float)e.ct * (float)e.nb * (float)A.H;
-        const int R0 = first_share(A, T, (float)e.nb, least);
+        int alone;
+        const int R0 = first_share(A, T, (float)e.nb, least, alone);
         int R = 2 * R0;
         for (int k = 2; k >= 0; k--) {
             const int r = R0 + k * R0 / 4;
-            if ((float)shares_of(e.nb, r, least) * (float)e.ct * (float)A.H <= (float)A.target) R = r;
+            if ((float)shares_of(e.nb, r, alone) * (float)e.ct * (float)A.H <= (float)A.target) R = r;
         }
-        const int ns = shares_of(e.nb, R, least);
+        const int ns = shares_of(e.nb, R, alone);
         if (by_group) item *= ns;
         out = Share{0, e.a, e.b - e.a, e.len - (e.b - e.a), e.ct - 1 - item / ns, item % ns, ns, item};
         return !e.bad && item < e.ct * ns;
@@ -134,12 +139,13 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
     }
     if (__any(bad)) return false;  // the grid was made for rows that ascend
     T = wave_sum(T) * (float)A.H;
-    const int R0 = first_share(A, T, T / fmaxf(wave_sum(groups) * (float)A.H, 1.0f), least);
+    int alone;
+    const int R0 = first_share(A, T, T / fmaxf(wave_sum(groups) * (float)A.H, 1.0f), least, alone);
     float n[3] = {0.0f, 0.0f, 0.0f};
     for (int i0 = 0; i0 < n_seq; i0 += 64) {
         const Extent e = i0 ? extent(A, i0 + lane, cols) : e0;
 #pragma unroll
-        for (int k = 0; k < 3; k++) n[k] += (float)e.ct * (float)shares_of(e.nb, R0 + k * R0 / 4, least);
+        for (int k = 0; k < 3; k++) n[k] += (float)e.ct * (float)shares_of(e.nb, R0 + k * R0 / 4, alone);
     }
     int R = 2 * R0;
 #pragma unroll
@@ -148,7 +154,7 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
     int slots = 0;
     for (int i0 = 0; i0 < n_seq; i0 += 64) {
         const Extent e = i0 ? extent(A, i0 + lane, cols) : e0;
-        const int ns = shares_of(e.nb, R, least), mine = by_group ? e.ct : e.ct * ns, sum = sp_fp8_scan(mine, lane);
+        const int ns = shares_of(e.nb, R, alone), mine = by_group ? e.ct : e.ct * ns, sum = sp_fp8_scan(mine, lane);
         const int part = ns > 1 ? e.ct * ns : 0, psum = sp_fp8_scan(part, lane);
         const unsigned long long past = __ballot(sum > item);
         if (past) {
@@ -575,8 +581,8 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 // within a factor of two and their unit always, so that the second part keeps its bits.
 //
 // Bound by the matrix cores and, beside them, by power: 2048 rows over 32768 positions, 32 / 8 heads
-// of 128, take 890 us in a row of calls (1.2 PFLOP/s; a large bf16 matrix product reaches 1.19 to 1.24, by
-// card) and 960 alone, the matrix cores busy 51% of the cycles; the same loop with nothing but its matrix
+// of 128, take 886 to 918 us by card in a row of calls (1.16 to 1.20 PFLOP/s; a large bf16 matrix product reaches 1.19 to
+// 1.24) and 960 alone, the matrix cores busy 51% of the cycles; the same loop with nothing but its matrix
 // instructions takes 595 us at a clock of 1.7 GHz. 2048 rows in a window of 1024, 16 / 8 heads of
 // 256: 59 us under the tracer, 52 in a run of calls (0.66 PFLOP/s), 18 blocks a column group with
 // 11 us before the first; LDS reads, the codes' conversion and the weights each hide a fifth of the rest.
