@@ -1188,7 +1188,10 @@ hipError_t launch_dt(const SpFp8Attn &A, hipStream_t s) {
     // 52 / 48; 128 32 / 47, 53 / 51, 74 / 69, float32 rows -, 62 / 61, 104 / 101; 256 68 / 58, 92 / 74,
     // 149 / 119; 24 and 40 sequences of 256 with 42 columns 102 / 131, 122 / 137.
     constexpr bool F32 = DT == SP_DTYPE_F32;
-    constexpr int MANY = HD == 256 ? 4096 : HD == 128 && F32 ? 8192 : 12288, EACH = F32 ? 128 : 64;
+    // Up to a column group of this kernel's on each CU it is the better one over short contexts and no
+    // worse over 8K; past that it takes a second turn (300 rows over 16000, head_dim 128: 186 / 107).
+    // At head_dim 256, where it reads more, the other from there on.
+    constexpr int MANY = 256 * 16 * CG + (HD == 256 ? 0 : 1), EACH = F32 ? 128 : 64;
     if (A.s.row && columns * A.H >= MANY && columns >= EACH * (long long)A.s.n_seq) return launch_wide<HD, DT>(A, s);
     if (columns > 16ll * A.s.n_seq) return launch<HD, DT, NW, CG>(A, s);
     return launch<HD, DT, NW, 1>(A, s);
