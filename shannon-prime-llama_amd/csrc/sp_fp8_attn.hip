@@ -35,6 +35,13 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr float P_TOP = 14.0f;  // log2 of the largest weight
 
+// A score further than this from 0 has the maximum taken off first, which is exact at the maximum, and
+// P_TOP added then. Taken together they are rounded where a float counts in 2 or more (from 2^24 on):
+// the largest weight becomes 2^16, which is no fp16 number. Below, rounding them costs less than the
+// score's own last bit. (Always in two steps: 40.5 us for 39.7 with 32 rows of each of 12 sequences at
+// head_dim 64, 32 / 8 heads.)
+constexpr float FAR_SCORE = 0x1p18f;
+
 // Eight codes (two dwords) as fp16.
 __device__ __forceinline__ h8 to_half(unsigned a, unsigned b) {
     const h2 x = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false);
@@ -223,7 +230,7 @@ __device__ __forceinline__ void finish(const SpFp8Attn &A, long long row, int he
     out[0] = SpFp8Elem<DT>::put(l == 0.0f ? 0.0f : o0 * r);
     out[1] = SpFp8Elem<DT>::put(l == 0.0f ? 0.0f : o1 * r);
     if (A.lse && d == 0)
-        A.lse[row * A.H * A.G + head] = l == 0.0f ? -INFINITY : (m - P_TOP + __log2f(l)) * 0.69314718055994531f;
+        A.lse[row * A.H * A.G + head] = l == 0.0f ? -INFINITY : (m + (__log2f(l) - P_TOP)) * 0.69314718055994531f;
 }
 
 // Whether a partial result has its place (always: see find_share).
@@ -468,7 +475,15 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
                         top = fmaxf(top, x);
                     }
                 const float m_new = fmaxf(m[y], column_max(top));
-                const float ref = m_new == -INFINITY ? 0.0f : m_new - P_TOP;
+                float ref = m_new == -INFINITY ? 0.0f : m_new;
+                if (__any(fabsf(ref) > FAR_SCORE)) {
+#pragma unroll
+                    for (int n = 0; n < 4; n++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) s[y][n][i] -= ref;
+                    ref = 0.0f;
+                }
+                ref -= P_TOP;
                 const float alpha = weight(m[y], m_new);
                 float sum = 0.0f;
 #pragma unroll

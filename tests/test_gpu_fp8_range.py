@@ -1,0 +1,79 @@
+"""The 8-bit block cache's attention over the range of scores that its calls accept, against the
+numpy form in 64 bits.
+
+With kq_scale the float nearest to ln 2 a score counts in powers of two, so that scores which are
+whole numbers are exact in the kernels (fp32 holds every product and sum below: each is a multiple of
+the last bit that a float of its size has) and exact in the numpy form with ln 2 itself. What is then
+left of fp8_ref.bounds is its part that does not come from the scores."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import fp8_ref as R
+from test_gpu_fp8_cache import TORCH, Pair
+
+pytestmark = pytest.mark.gpu
+
+LN2 = float(np.float32(math.log(2)))
+assert np.float32(LN2) * np.float32(1.4426950408889634) == 1.0  # the factor of the kernels' exponents
+KE = 8  # K's values count in 2^KE, so that fp16 queries reach large scores
+
+# M * 2^(E - 7) is the smallest of the large scores, with M in [128, 240): fp32 counts in 2^(E - 23) there
+TOPS = [(131, 19), (128, 20), (160, 25), (200, 25), (176, 26), (160, 27), (150, 29)]
+
+
+def step_of(E):
+    """Distance of the scores: a float's last bit there, at least 1 (a weight half as large)."""
+    return max(2.0 ** (E - 23), 1.0)
+
+
+def check(P, dtype, q, window=0):
+    """P.check_attend for scores that are exact."""
+    out, lse = P.attend(dtype, q, LN2, window)
+    want, wlse, reach, steep = P.ref.attend(0, P.table, P.lens, P.row, P.n_rows, q.double().numpy(), math.log(2), window)
+    tol, ltol = R.bounds(dtype, P.hd, max(P.lens), want, reach, 0 * steep)
+    assert np.isfinite(out).all() and np.isfinite(lse).all(), "a finite row came out infinite or NaN"
+    d, dl = np.abs(out - want), np.abs(lse - wlse)
+    assert (d <= tol).all(), (float((d - tol).max()), float(d.max()))
+    assert (dl <= ltol + 2.0 ** -23 * np.abs(wlse)).all(), float((dl - 2.0 ** -23 * np.abs(wlse)).max())
+
+
+def fill(P, rng, length, grade, large=lambda block: np.full(block.shape, 256.0)):
+    """K: channel 0 makes a score large (by block), channel 1 grades it; V: strength by block."""
+    block = np.arange(length) // 64
+    k = np.zeros((length, 1, P.hd))
+    k[:, 0, 0], k[:, 0, 1] = large(block), grade(block, np.arange(length))
+    v = rng.standard_normal((length, 1, P.hd)) * 2.0 ** ((block * 5) % 13 - 6.0)[:, None, None]
+    P.batch([rng.permutation(P.n_blocks).tolist()], [length], [0, length])
+    P.write("f32", torch.from_numpy(k * 2.0 ** KE).float(), torch.from_numpy(v).float())
+
+
+def large_queries(n, n_q, hd, M, E, sign, dtype):
+    """Row r, head h: score (M + (r + h) % 14) 2^(E - 7) of channel 0's 256, one step for each of channel 1's 1."""
+    q = np.zeros((n, n_q, hd))
+    rh = np.arange(n)[:, None] + np.arange(n_q)[None]
+    q[..., 0] = sign * (M + rh % 14) * 2.0 ** (E - 7 - 8 - KE)
+    q[..., 1] = step_of(E) * 2.0 ** -KE
+    t = torch.from_numpy(q).to(TORCH[dtype])
+    assert (t.double().numpy() == q).all()
+    return t
+
+
+GRADES = {"within": lambda block, t: (t * 7) % 4 + (t % 64 == 17), "rising": lambda block, t: np.minimum(block // 4, 15)}
+
+
+@pytest.mark.parametrize("length", [300, 2560])  # 2560: in shares, joined
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("M,E", TOPS)
+def test_large_scores(M, E, sign, length):
+    """The kernel for few rows: one row, a few, and more than 16 columns a wave."""
+    rng = np.random.default_rng(E)
+    for hd, grade in ((64, "within"), (256, "rising")):
+        P = Pair(hd, 1, (length + 63) // 64)
+        fill(P, rng, length, GRADES[grade])
+        for dtype in ("f16", "bf16", "f32"):
+            for row, n_q in ((None, 3), ([0, 4], 3), ([0, 9], 4)):
+                P.batch(P.table, [length], row)
+                check(P, dtype, large_queries(P.n_rows, n_q, hd, M, E, sign, dtype))
