@@ -820,10 +820,12 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     V o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = V{};
-    // m: the reference; off = W_TOP - m, 0 while m is -inf; the output's unit is 2^ev_now
+    // m: the reference; off = W_TOP - m (huge: -m), 0 while m is -inf; the output's unit is 2^ev_now
     float m = -INFINITY, off = 0.0f, l = 0.0f;
     int ev_now = 0;
-    bool huge = false;  // the fused difference of a score and the reference would not be 0 where they are equal
+    // a column's reference is past FAR_SCORE: the fused difference of a score and the reference would not
+    // be 0 where they are equal, and the constants added to the reference would be rounded
+    bool huge = false;
     // of the block whose weights come next: score scale, exponent offset, its part in l
     float cs = 0.0f, shift = 0.0f, lmul = 1.0f;
     h8 p[NP][NH];
@@ -911,7 +913,9 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     const auto settle = [&](const Facts &f, float top, V(&s)[RB]) __attribute__((always_inline)) {
         // never 0: a masked score stays -inf when it is multiplied
         cs = fmaxf(cscale * sp_fp8_pow2(f.ek), 0x1p-126f);
-        const bool raise = __builtin_fmaf(top, cs, off) > (m == -INFINITY ? -INFINITY : W_TOP + W_SLACK);
+        // (huge: whatever is past the reference raises it, since what is up to half a float's step past it may
+        // be rounded to a whole one)
+        const bool raise = __builtin_fmaf(top, cs, off) > (m == -INFINITY ? -INFINITY : huge ? 0.0f : W_TOP + W_SLACK);
         float scale = 1.0f;
         bool rescale = false;
         if (f.ev > ev_now || f.ev < ev_now - W_FOLD) {
@@ -926,20 +930,22 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
             l *= alpha;
             scale *= alpha;
             m = m_new;
-            off = m == -INFINITY ? 0.0f : W_TOP - m;
             rescale = true;
-            huge = __any(fabsf(m) > 0x1p18f && m > -INFINITY);
+            huge = __any(fabsf(m) > FAR_SCORE && m > -INFINITY);
+            off = m == -INFINITY ? 0.0f : (huge ? 0.0f : W_TOP) - m;
         }
-        if (huge) {  // the reference was rounded: round the scores as it was
+        shift = off;
+        if (huge) {  // the reference was rounded: round the scores as it was, and take it off first
 #pragma unroll
-            for (int i = 0; i < NE; i++) s[i / VL][i % VL] *= cs;
+            for (int i = 0; i < NE; i++) s[i / VL][i % VL] = s[i / VL][i % VL] * cs + off;
             cs = 1.0f;
+            shift = W_TOP;
         }
         if (rescale) {
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] *= scale;
         }
-        shift = off + (float)(f.ev - ev_now);
+        shift += (float)(f.ev - ev_now);
         lmul = sp_fp8_pow2(ev_now - f.ev);
     };
     const std::true_type yes;
@@ -1057,7 +1063,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
                 else store4<DT>(out, ch, x, aligned);
             }
         if (A.lse && sub == 0)
-            A.lse[row * A.H * A.G + head] = l == 0.0f ? -INFINITY : (m - W_TOP + __log2f(l)) * 0.69314718055994531f;
+            A.lse[row * A.H * A.G + head] = l == 0.0f ? -INFINITY : (m + (__log2f(l) - W_TOP)) * 0.69314718055994531f;
     }
     if (!through) return;
     lds_barrier();

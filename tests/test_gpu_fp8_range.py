@@ -77,3 +77,33 @@ def test_large_scores(M, E, sign, length):
             for row, n_q in ((None, 3), ([0, 4], 3), ([0, 9], 4)):
                 P.batch(P.table, [length], row)
                 check(P, dtype, large_queries(P.n_rows, n_q, hd, M, E, sign, dtype))
+
+
+@pytest.mark.parametrize("length", [300, 2560])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("M,E", TOPS)
+def test_large_scores_of_many_columns(M, E, sign, length):
+    """The kernel for many rows, its waves of 32 columns and of 16."""
+    rng = np.random.default_rng(E)
+    for hd in (64, 256):
+        P = Pair(hd, 1, (length + 63) // 64)
+        fill(P, rng, length, GRADES["within"])
+        for dtype in ("bf16", "f32"):
+            n = {(64, "bf16"): 129, (64, "f32"): 65}.get((hd, dtype), 65)  # 8256 columns, else 4160
+            P.batch(P.table, [length], [0, n])
+            check(P, dtype, large_queries(n, 64, hd, M, E, sign, dtype))
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("M,E", [(128, 20), (160, 25), (160, 27)])
+def test_scores_small_then_large(M, E, sign):
+    """Blocks without channel 0 among blocks with it: the maximum jumps up, or from far below 0 to near it."""
+    rng = np.random.default_rng(E)
+    for hd in (64,):
+        P = Pair(hd, 1, 12)
+        fill(P, rng, 700, GRADES["within"], lambda block: np.where(np.isin(block, (0, 1, 5, 8)), 0.0, 256.0))
+        for dtype in ("bf16", "f32"):
+            for row, n_q in ((None, 3), ([0, 9], 4), ([0, 600], 16)):
+                for window in (0, 100):
+                    P.batch(P.table, [700], row)
+                    check(P, dtype, large_queries(P.n_rows, n_q, hd, M, E, sign, dtype), window)
