@@ -602,6 +602,8 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 // 256: 59 us under the tracer, 52 in a run of calls (0.66 PFLOP/s), 18 blocks a column group with
 // 11 us before the first; LDS reads, the codes' conversion and the weights each hide a fifth of the rest.
 typedef float f16x __attribute__((ext_vector_type(16)));
+template <int DT>
+constexpr float WIDE_TOP = DT == SP_DTYPE_F32 ? 14.0f : 12.0f;  // W_TOP
 
 // LDS written before is seen after, by the whole block; loads from memory stay in flight.
 __device__ __forceinline__ void lds_barrier() {
@@ -645,7 +647,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     constexpr int KE = CW == 32 ? 16 : 32;  // channels of a score step
     constexpr bool SPLIT2 = DT == SP_DTYPE_F32;
     constexpr int NH = SPLIT2 ? 2 : 1;
-    constexpr float W_TOP = SPLIT2 ? 14.0f : 12.0f, W_SLACK = SPLIT2 ? 1.0f : 3.0f;
+    constexpr float W_TOP = WIDE_TOP<DT>, W_SLACK = SPLIT2 ? 1.0f : 3.0f;
     constexpr int W_FOLD = SPLIT2 ? 0 : 8;
     constexpr int KP = (HD * 4 + HT - 1) / HT;  // K pieces of 16 codes a thread (half the threads)
     constexpr int VP = (HD * 2 + HT - 1) / HT;  // pairs of V pieces (the other half)
@@ -1034,8 +1036,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
         const long long slot = (long long)sh.slot * A.H + h;
         if (active && slot_fits(A, slot, COLS)) {
             float *dst = A.part + (slot * COLS + mycol) * ROW;
-            // the maximum whose weight would be 2^P_TOP
-            if (sub == 0) *reinterpret_cast<Two *>(dst + HD) = Two{m + (P_TOP - W_TOP), l};
+            if (sub == 0) *reinterpret_cast<Two *>(dst + HD) = Two{m, l};
 #pragma unroll
             for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -1128,7 +1129,7 @@ __global__ __launch_bounds__(256) void k_fp8_attn_join(SpFp8Attn A) {
     for (int j = 0; j < 4; j++) x[j] = L == 0.0f ? 0.0f : x[j] * r;
     store4<DT>(A.out, row * A.out_stride + (long long)head * HD + d, x, aligned);
     if (A.lse && d == 0)
-        A.lse[row * A.H * A.G + head] = L == 0.0f ? -INFINITY : (M - P_TOP + __log2f(L)) * 0.69314718055994531f;
+        A.lse[row * A.H * A.G + head] = L == 0.0f ? -INFINITY : (M + (__log2f(L) - WIDE_TOP<DT>)) * 0.69314718055994531f;
 }
 
 template <int HD, int DT, int NW, int CG>

@@ -95,11 +95,24 @@ def test_large_scores_of_many_columns(M, E, sign, length):
 
 
 @pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("M,E", TOPS)
+def test_large_scores_in_rising_shares(M, E, sign):
+    """The shares of the kernel for many rows have maxima of their own, a step or more apart."""
+    rng = np.random.default_rng(E)
+    for hd in (64, 256):
+        P = Pair(hd, 1, 40)
+        fill(P, rng, 2560, GRADES["rising"])
+        P.batch(P.table, [2560], [0, 129 if hd == 64 else 65])
+        for dtype in ("f16", "bf16", "f32"):
+            check(P, dtype, large_queries(P.n_rows, 64, hd, M, E, sign, dtype))
+
+
+@pytest.mark.parametrize("sign", [1, -1])
 @pytest.mark.parametrize("M,E", [(128, 20), (160, 25), (160, 27)])
 def test_scores_small_then_large(M, E, sign):
     """Blocks without channel 0 among blocks with it: the maximum jumps up, or from far below 0 to near it."""
     rng = np.random.default_rng(E)
-    for hd in (64,):
+    for hd in (64, 128):
         P = Pair(hd, 1, 12)
         fill(P, rng, 700, GRADES["within"], lambda block: np.where(np.isin(block, (0, 1, 5, 8)), 0.0, 256.0))
         for dtype in ("bf16", "f32"):
