@@ -57,7 +57,7 @@ struct SpFp8Attn {
     long long q_stride, out_stride;
     int H, G;  // KV heads, query heads per KV head
     int window;
-    float c;   // kq_scale * log2(e), not negative
+    float c;   // kq_scale * log2(e) / 2, not negative (half: a float whatever kq_scale is)
     int negate;
     float *part;    // partial results: part_rows rows of hd + 4 floats
     int part_rows;

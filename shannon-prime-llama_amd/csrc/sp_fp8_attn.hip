@@ -62,6 +62,12 @@ __device__ __forceinline__ float column_sum(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
+// A.c 2^e, at most the largest float. kq_scale, the query's exponent and the block's are put together in
+// one step: two of them may multiply to more than a float holds where all three are an ordinary scale.
+__device__ __forceinline__ float score_scale(const SpFp8Attn &A, int e) {
+    return fminf(__builtin_amdgcn_ldexpf(A.c, e), 0x1.fffffep127f);
+}
+
 // Results that all lanes agree on are taken into scalar registers (readfirstlane, readlane), so
 // that what follows from them is scalar too.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -390,7 +396,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
     }
     if (mine > 0) start();
     h8 q[CG][NC][NH];
-    float cscale[CG];
+    int qe[CG];  // scores count in 2^(qe + the block's exponent) * A.c
 #pragma unroll
     for (int y = 0; y < CG; y++) {
         float top = 0.0f;
@@ -402,7 +408,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
         int e = (__float_as_int(top) >> 23) - 127 - 14;
         e = top == 0.0f || !(top < INFINITY) ? 0 : max(e, -126);
         const float down = A.negate ? -sp_fp8_pow2(-e) : sp_fp8_pow2(-e);
-        cscale[y] = A.c * sp_fp8_pow2(e);
+        qe[y] = e + 1;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -433,7 +439,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
         for (int k = 0; k < count; k++) {
             const int t = t0 + w + NW * (base + k);
             const bool none = __builtin_amdgcn_readlane(blk, k) < 0;
-            const float kscale = sp_fp8_pow2(sp_fp8_exponent(__builtin_amdgcn_readlane(ekb, k)));
+            const int ek = sp_fp8_exponent(__builtin_amdgcn_readlane(ekb, k));
             f4 s[CG][4];
 #pragma unroll
             for (int y = 0; y < CG; y++)
@@ -461,7 +467,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
             h8 p[CG][2][NH];
 #pragma unroll
             for (int y = 0; y < CG; y++) {
-                const float cs = cscale[y] * kscale;
+                const float cs = score_scale(A, qe[y] + ek);
                 float top = -INFINITY;
                 // positions of this block that the column sees, counted from the lane's first: (before, upto]
                 const int lane0 = t * 64 + 4 * g, upto = none ? -1 : pos[y] - lane0, before = from[y] - lane0;
@@ -764,7 +770,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     const int wlast = min(w * CW + CW - 1, n_cols - 1);
     const int wpos0 = sh.first + (c0 + w * CW) / A.G, wpos1 = sh.first + (c0 + wlast) / A.G;
     h8 q[NS][NH];
-    float cscale;
+    int qe;  // scores count in 2^(qe + the block's exponent) * A.c
     {
         // Rows of 16-bit types go through LDS, in 16-byte pieces: loaded as they lie, and read
         // back by column with a row's pieces turned around so that 16 columns' reads meet no bank
@@ -804,7 +810,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
         int e = (__float_as_int(top) >> 23) - 127 - 14;
         e = top == 0.0f || !(top < INFINITY) ? 0 : max(e, -126);
         const float down = A.negate ? -sp_fp8_pow2(-e) : sp_fp8_pow2(-e);
-        cscale = A.c * sp_fp8_pow2(e);
+        qe = e + 1;
 #pragma unroll
         for (int s = 0; s < NS; s++) {
             eight(s, x);
@@ -914,7 +920,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     // the reference and the output's unit for a block with largest score `top` (this lane's)
     const auto settle = [&](const Facts &f, float top, V(&s)[RB]) __attribute__((always_inline)) {
         // never 0: a masked score stays -inf when it is multiplied
-        cs = fmaxf(cscale * sp_fp8_pow2(f.ek), 0x1p-126f);
+        cs = fmaxf(score_scale(A, qe + f.ek), 0x1p-126f);
         // (huge: whatever is past the reference raises it, since what is up to half a float's step past it may
         // be rounded to a whole one)
         const bool raise = __builtin_fmaf(top, cs, off) > (m == -INFINITY ? -INFINITY : huge ? 0.0f : W_TOP + W_SLACK);

@@ -187,7 +187,7 @@ int attend(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *b, 
     A.H = H;
     A.G = n_q / H;
     A.window = window >= MAX_ROWS ? 0 : window;  // no position is that far
-    A.c = fabsf(kq_scale) * 1.4426950408889634f;
+    A.c = fabsf(kq_scale) * 0.72134752044448170f;
     A.negate = kq_scale < 0.0f;
     A.part = pv->ws[which].part;
     A.counters = pv->ws[which].counters;

@@ -120,3 +120,29 @@ def test_scores_small_then_large(M, E, sign):
                 for window in (0, 100):
                     P.batch(P.table, [700], row)
                     check(P, dtype, large_queries(P.n_rows, n_q, hd, M, E, sign, dtype), window)
+
+
+def test_scales_whose_product_is_past_a_float():
+    """Finite scores from factors whose scales multiply to more, or whose kq_scale does with log2 e."""
+    rng = np.random.default_rng(3)
+    k = torch.from_numpy(rng.standard_normal((300, 1, 64))).float()
+    k[:, 0, 0] = 0.0
+    v = torch.from_numpy(rng.standard_normal((300, 1, 64))).float()
+    for ke in (45, -27, -40):
+        P = Pair(64, 1, 6)
+        P.batch([[3, 0, 1, 2, 5]], [300], [0, 300])
+        P.write("f32", k * 2.0 ** ke, v)
+        for dtype in ("f32", "bf16"):
+            for row, n_q in ((None, 3), ([0, 9], 4), ([0, 300], 32)):
+                P.batch(P.table, [300], row)
+                q = torch.from_numpy(rng.standard_normal((P.n_rows, n_q, 64))).to(TORCH[dtype])
+                first = torch.zeros_like(q)
+                first[..., 0] = 2.0 ** 126  # meets zeros alone
+                P.check_attend(dtype, q * 0.0, 3.2e38)
+                P.check_attend(dtype, first, 0.125)
+                P.check_attend(dtype, first, -(2.0 ** 120))
+                if ke == -27:  # scores near 1
+                    P.check_attend(dtype, q * 2.0 ** -101, 3.2e38)
+                    P.check_attend(dtype, q * 2.0 ** 122, 2.0 ** -96)
+                if ke == -40:  # scores near 2^104
+                    P.check_attend(dtype, q * 2.0 ** 110, 2.0 ** 34)
