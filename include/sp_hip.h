@@ -23,7 +23,7 @@ extern "C" {
 
 #define SP_DTYPE_F32 0
 #define SP_DTYPE_F16 1
-#define SP_DTYPE_BF16 2   /* the 8-bit block cache's calls only */
+#define SP_DTYPE_BF16 2   /* the 8-bit block cache only; the spectral caches refuse it */
 
 /* ======================================================================== */
 /* Ship cache  (sp_cuda_cache_t, shannon_prime_cuda.h:29-46)                */

@@ -331,6 +331,14 @@ extern "C" uint16_t sp_f32_to_f16(float f) {
     return (uint16_t)(sign | keep);
 }
 
+// The spectral caches' rows are fp32 or fp16. Every call that takes a dtype asks before anything else:
+// the launches take what is not fp16 for fp32, twice the bytes of a bf16 row.
+static bool rows_ok(int dtype, const char *who) {
+    if (dtype == SP_DT_F32 || dtype == SP_DT_F16) return true;
+    set_err("%s: dtype %d (SP_DTYPE_F32 or SP_DTYPE_F16)", who, dtype);
+    return false;
+}
+
 // ===========================================================================
 // generic codec entry points
 // ===========================================================================
@@ -338,6 +346,7 @@ extern "C" int sp_hip_ship_encode(const sp_band_config_t *bc, const int *d_order
                                   const void *d_src, int src_dtype, long long src_outer,
                                   long long src_inner, void *d_dst, long long dst_outer,
                                   int n_outer, int n_inner, void *stream) {
+    if (!rows_ok(src_dtype, "encode")) return -1;
     if (!bc || !d_src || !d_dst || n_outer < 0 || n_inner < 0) { set_err("encode: bad args"); return -1; }
     SpPlan P;
     if (sp_build_plan(bc, bc->head_dim, vht2_norm, -1, &P)) { set_err("encode: bad band config"); return -1; }
@@ -350,6 +359,7 @@ extern "C" int sp_hip_ship_decode(const sp_band_config_t *bc, const int *d_order
                                   int max_bands, const void *d_src, long long src_outer,
                                   void *d_dst, int dst_dtype, long long dst_outer,
                                   long long dst_inner, int n_outer, int n_inner, void *stream) {
+    if (!rows_ok(dst_dtype, "decode")) return -1;
     if (!bc || !d_src || !d_dst || n_outer < 0 || n_inner < 0) { set_err("decode: bad args"); return -1; }
     SpPlan P;
     if (sp_build_plan(bc, bc->head_dim, vht2_norm, max_bands, &P)) { set_err("decode: bad band config"); return -1; }
@@ -364,6 +374,7 @@ extern "C" int sp_hip_ship_encode_generic(const sp_band_config_t *bc, const int 
                                           long long src_outer, long long src_inner, void *d_dst,
                                           long long dst_outer, int n_outer, int n_inner,
                                           void *stream) {
+    if (!rows_ok(src_dtype, "encode_generic")) return -1;
     SpPlan P;
     if (!bc || sp_build_plan(bc, bc->head_dim, vht2_norm, -1, &P)) return -1;
     return hip_ok(sp_launch_ship_encode_generic(P, d_order, d_src, src_dtype, src_outer, src_inner,
@@ -376,6 +387,7 @@ extern "C" int sp_hip_ship_decode_generic(const sp_band_config_t *bc, const int 
                                           long long src_outer, void *d_dst, int dst_dtype,
                                           long long dst_outer, long long dst_inner, int n_outer,
                                           int n_inner, void *stream) {
+    if (!rows_ok(dst_dtype, "decode_generic")) return -1;
     SpPlan P;
     if (!bc || sp_build_plan(bc, bc->head_dim, vht2_norm, max_bands, &P)) return -1;
     return hip_ok(sp_launch_ship_decode_generic(P, d_order, (const unsigned char *)d_src, src_outer,
@@ -605,6 +617,7 @@ extern "C" void sp_hip_read_v_batch_f16(const sp_hip_cache_t *cc, int l, int h, 
 
 extern "C" int sp_hip_write_layer(sp_hip_cache_t *cc, int layer, int start_pos, int n_tok,
                                   const void *d_k, const void *d_v, long long row_stride, int dtype) {
+    if (!rows_ok(dtype, "write_layer")) return -1;
     if (!slot_ok(cc, layer, 0, start_pos, n_tok)) { set_err("write_layer: bad layer/pos"); return -1; }
     const int H = cc->config.n_heads_kv, hd = cc->config.head_dim;
     if (row_stride < (long long)H * hd) { set_err("write_layer: row_stride"); return -1; }
@@ -629,6 +642,7 @@ extern "C" int sp_hip_write_layer(sp_hip_cache_t *cc, int layer, int start_pos, 
 
 extern "C" int sp_hip_read_layer(const sp_hip_cache_t *cc, int layer, int start_pos, int n_tok,
                                  void *d_k, void *d_v, long long row_stride, int dtype, int max_bands) {
+    if (!rows_ok(dtype, "read_layer")) return -1;
     if (!slot_ok(cc, layer, 0, start_pos, n_tok)) { set_err("read_layer: bad layer/pos"); return -1; }
     const int H = cc->config.n_heads_kv, hd = cc->config.head_dim;
     if (row_stride < (long long)H * hd) { set_err("read_layer: row_stride"); return -1; }
@@ -808,6 +822,7 @@ extern "C" int sp_hip_calibrate_end(sp_hip_cache_t *cc, int *var_order_out, int 
 
 extern "C" int sp_hip_write_all(sp_hip_cache_t *cc, int start_pos, int n_pos, const void *d_k,
                                 const void *d_v, int dtype) {
+    if (!rows_ok(dtype, "write_all")) return -1;
     if (!slot_ok(cc, 0, 0, start_pos, n_pos)) { set_err("write_all: bad pos"); return -1; }
     const int n_slots = cc->config.n_layers * cc->config.n_heads_kv, hd = cc->config.head_dim;
     ShipPriv *pv = (ShipPriv *)cc->priv;
@@ -832,6 +847,7 @@ extern "C" int sp_hip_write_all(sp_hip_cache_t *cc, int start_pos, int n_pos, co
 
 extern "C" int sp_hip_read_all(const sp_hip_cache_t *cc, int start_pos, int n_pos, void *d_k, void *d_v,
                                int dtype, int max_bands) {
+    if (!rows_ok(dtype, "read_all")) return -1;
     if (!slot_ok(cc, 0, 0, start_pos, n_pos)) { set_err("read_all: bad pos"); return -1; }
     const int n_slots = cc->config.n_layers * cc->config.n_heads_kv, hd = cc->config.head_dim;
     ShipPriv *pv = (ShipPriv *)cc->priv;
@@ -1198,6 +1214,7 @@ static bool sq_slot_ok(const sp_hip_sqfree_cache_t *cc, int layer, int head, int
 
 extern "C" int sp_hip_sqfree_write_batch(sp_hip_sqfree_cache_t *cc, int is_v, int layer, int head,
                                          int start_pos, int n_pos, const void *d_src, int dtype) {
+    if (!rows_ok(dtype, "sqfree write")) return -1;
     if (!sq_slot_ok(cc, layer, head, start_pos, n_pos) || !d_src) { set_err("sqfree write: bad args"); return -1; }
     SqPriv *pv = (SqPriv *)cc->priv;
     const SpSqGeo G = sq_geo(cc, is_v);
@@ -1211,6 +1228,7 @@ extern "C" int sp_hip_sqfree_write_batch(sp_hip_sqfree_cache_t *cc, int is_v, in
 
 extern "C" int sp_hip_sqfree_read_batch(const sp_hip_sqfree_cache_t *cc, int is_v, int layer, int head,
                                         int start_pos, int n_pos, void *d_dst, int dtype) {
+    if (!rows_ok(dtype, "sqfree read")) return -1;
     if (!sq_slot_ok(cc, layer, head, start_pos, n_pos) || !d_dst) { set_err("sqfree read: bad args"); return -1; }
     SqPriv *pv = (SqPriv *)cc->priv;
     const SpSqGeo G = sq_geo(cc, is_v);
@@ -1224,6 +1242,7 @@ extern "C" int sp_hip_sqfree_read_batch(const sp_hip_sqfree_cache_t *cc, int is_
 
 extern "C" int sp_hip_sqfree_write_layer(sp_hip_sqfree_cache_t *cc, int layer, int start_pos, int n_tok,
                                          const void *d_k, const void *d_v, long long row_stride, int dtype) {
+    if (!rows_ok(dtype, "sqfree write_layer")) return -1;
     if (!sq_slot_ok(cc, layer, 0, start_pos, n_tok)) { set_err("sqfree write_layer: bad layer/pos"); return -1; }
     const int H = cc->config.n_heads_kv, hd = cc->config.head_dim;
     if (row_stride < (long long)H * hd) { set_err("sqfree write_layer: row_stride"); return -1; }
@@ -1251,6 +1270,7 @@ extern "C" int sp_hip_sqfree_write_layer(sp_hip_sqfree_cache_t *cc, int layer, i
 
 extern "C" int sp_hip_sqfree_read_layer(const sp_hip_sqfree_cache_t *cc, int layer, int start_pos, int n_tok,
                                         void *d_k, void *d_v, long long row_stride, int dtype) {
+    if (!rows_ok(dtype, "sqfree read_layer")) return -1;
     if (!sq_slot_ok(cc, layer, 0, start_pos, n_tok)) { set_err("sqfree read_layer: bad layer/pos"); return -1; }
     const int H = cc->config.n_heads_kv, hd = cc->config.head_dim;
     if (row_stride < (long long)H * hd) { set_err("sqfree read_layer: row_stride"); return -1; }
@@ -1552,6 +1572,7 @@ static bool hier_slot_ok(const sp_hip_hier_cache_t *hc, int layer, int head, int
 
 extern "C" int sp_hip_hier_write_batch(sp_hip_hier_cache_t *hc, int is_v, int layer, int head, int start_pos,
                                        int n_pos, const void *d_src, int dtype) {
+    if (!rows_ok(dtype, "hier write")) return -1;
     if (!hier_slot_ok(hc, layer, head, start_pos, n_pos) || !d_src) { set_err("hier write: bad args"); return -1; }
     const int slot = layer * hc->config.n_heads_kv + head;
     const SpHierGeo G = hier_geo(hc, slot);
@@ -1563,6 +1584,7 @@ extern "C" int sp_hip_hier_write_batch(sp_hip_hier_cache_t *hc, int is_v, int la
 
 extern "C" int sp_hip_hier_read_batch(const sp_hip_hier_cache_t *hc, int is_v, int layer, int head, int start_pos,
                                       int n_pos, void *d_dst, int dtype) {
+    if (!rows_ok(dtype, "hier read")) return -1;
     if (!hier_slot_ok(hc, layer, head, start_pos, n_pos) || !d_dst) { set_err("hier read: bad args"); return -1; }
     const int slot = layer * hc->config.n_heads_kv + head;
     const SpHierGeo G = hier_geo(hc, slot);
@@ -1575,6 +1597,7 @@ extern "C" int sp_hip_hier_read_batch(const sp_hip_hier_cache_t *hc, int is_v, i
 
 extern "C" int sp_hip_hier_write_layer(sp_hip_hier_cache_t *hc, int layer, int start_pos, int n_tok,
                                        const void *d_k, const void *d_v, long long row_stride, int dtype) {
+    if (!rows_ok(dtype, "hier write_layer")) return -1;
     if (!hier_slot_ok(hc, layer, 0, start_pos, n_tok) ||
         (long long)(layer + 1) * hc->config.n_heads_kv > hc->n_slots) { set_err("hier write_layer: bad layer/pos"); return -1; }
     const int H = hc->config.n_heads_kv, hd = hc->config.head_dim;
@@ -1600,6 +1623,7 @@ extern "C" int sp_hip_hier_write_layer(sp_hip_hier_cache_t *hc, int layer, int s
 
 extern "C" int sp_hip_hier_read_layer(const sp_hip_hier_cache_t *hc, int layer, int start_pos, int n_tok,
                                       void *d_k, void *d_v, long long row_stride, int dtype) {
+    if (!rows_ok(dtype, "hier read_layer")) return -1;
     if (!hier_slot_ok(hc, layer, 0, start_pos, n_tok) ||
         (long long)(layer + 1) * hc->config.n_heads_kv > hc->n_slots) { set_err("hier read_layer: bad layer/pos"); return -1; }
     const int H = hc->config.n_heads_kv, hd = hc->config.head_dim;
