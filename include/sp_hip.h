@@ -483,7 +483,10 @@ typedef struct {
     int            n_rows;        /* rows of the call's tensors */
 } sp_hip_fp8_batch_t;
 
-/* 0 or -1 (sp_hip_last_error). The memory is cleared: a fresh block holds zeros. */
+/* 0 or -1 (sp_hip_last_error). The memory is cleared: a fresh block holds zeros. Beside the codes
+ * (2 * n_layers * n_blocks * n_heads_kv * 64 * head_dim bytes) and their scales init takes the
+ * workspaces of both kinds of attention calls: 40, 59, 78 or 85 MB at head_dim 64, 96, 128 or
+ * 256, whatever the cache's size. */
 int  sp_hip_fp8_cache_init(sp_hip_fp8_cache_t *c, const sp_config_t *cfg, int n_blocks, void *stream);
 void sp_hip_fp8_cache_free(sp_hip_fp8_cache_t *c);
 
@@ -509,7 +512,9 @@ int  sp_hip_fp8_read(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_ba
  * r*q_stride + n*head_dim in d_q and r*out_stride + n*head_dim in d_out, both of `dtype`;
  * query head n reads KV head n / (n_q / n_heads_kv), any number per KV head.
  *   d_out = softmax(kq_scale * q . K) V      d_lse [n_rows][n_q] fp32 (may be NULL): the log
- * of the sum of exp(kq_scale * q . K). A row that sees nothing gets zeros and -infinity.
+ * of the sum of exp(kq_scale * q . K). A row that sees nothing gets zeros and -infinity. Scores
+ * are fp32: they may be of any size that a float holds (times log2 e), and so may kq_scale; of a
+ * query row nothing finer than about 2^-39 of its largest entry is seen.
  * The call's own positions are read from the cache: write them first. decode takes one row
  * per sequence (d_row NULL), prefill any number.
  * Their workspaces belong to the cache and are allocated by init: a decode and a prefill call on

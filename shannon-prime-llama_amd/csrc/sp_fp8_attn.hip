@@ -13,8 +13,11 @@
 // the weights' operand layout, so nothing passes through LDS inside the loop.
 //
 // Precision. q is scaled by a power of two that puts its row's largest entry in [2^14, 2^15)
-// and rounded to fp16: exact for fp16 and bf16 rows (entries below 2^-39 of the row's largest
-// lose bits). An fp32 row is split into two fp16 parts (22 bits). The weights are counted from
+// and rounded to fp16, whose last bit is 2^-24 or more, 2^-39 of the row's largest entry (2^-38 with one
+// next to 2^15). A bf16 row is exact but for its entries below 2^-31 of the largest, which lose bits and
+// vanish at 2^-39; an fp16 row is exact but, where its largest is 2^15 or more, for a last bit of 2^-24.
+// An fp32 row is split into two fp16 parts (22 bits, of entries below 2^-17 of the largest fewer, down
+// to the same last bit). The weights are counted from
 // 2^14 at the maximum, so that those of 2^-28 of it are still normal fp16 numbers, and rounded
 // to fp16 (half a step, 2^-11, beside the 2^-11 and 2^-8 of an fp16 or bf16 result) or, for fp32
 // results, split in two. Sums, maxima and the running output are fp32. The running output counts in
@@ -592,7 +595,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 // The loop is pipelined by one cache block: the next block's scores go through the matrix cores
 // among this one's weights and its product with V, so that neither unit waits for the other.
 //
-// The running maximum is a reference that is raised only when a score passes it by 2^W_SLACK
+// The running maximum is a reference that is raised only when a score passes it by W_SLACK
 // (the weights, 2^W_TOP at the reference, then still fit fp16), so that the output is rescaled
 // a few times in a whole sequence and no exchange between lanes is needed in the others. The
 // output counts in units of the strongest V scale of late; a block whose scale is up to
@@ -602,8 +605,8 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 // within a factor of two and their unit always, so that the second part keeps its bits.
 //
 // Bound by the matrix cores and, beside them, by power: 2048 rows over 32768 positions, 32 / 8 heads
-// of 128, take 886 to 918 us by card in a row of calls (1.16 to 1.20 PFLOP/s; a large bf16 matrix product reaches 1.19 to
-// 1.24) and 960 alone, the matrix cores busy 51% of the cycles; the same loop with nothing but its matrix
+// of 128, take 886 to 928 us by card in a row of calls (1.15 to 1.20 PFLOP/s; a large bf16 matrix product reaches 1.19 to
+// 1.24) and 930 to 960 alone, the matrix cores busy 51% of the cycles; the same loop with nothing but its matrix
 // instructions takes 595 us at a clock of 1.7 GHz. 2048 rows in a window of 1024, 16 / 8 heads of
 // 256: 59 us under the tracer, 52 in a run of calls (0.66 PFLOP/s), 18 blocks a column group with
 // 11 us before the first; LDS reads, the codes' conversion and the weights each hide a fifth of the rest.
@@ -1198,27 +1201,36 @@ hipError_t launch_dt(const SpFp8Attn &A, hipStream_t s) {
     // sequence has (columns that none has are worked through). The longer the context the better for
     // the other, but the host does not know it. Measured, few rows / many in us, one sequence:
     //   columns x heads              4096        8192        16384       32768
-    //   head_dim 64     from 0       8 / 10      8 / 13      15 / 18     33 / 28
-    //                   over 8K      30 / 32     45 / 43
-    //   head_dim 128    from 0       11 / 14     12 / 18     24 / 25     51 / 40
-    //                   over 8K      41 / 43     60 / 60
-    //                   over 32K     109 / 96
+    //   head_dim 64     from 0       8 / 10      9 / 13      16 / 18     33 / 28
+    //                   over 8K      31 / 32     46 / 43     86 / 65
+    //     float32 rows  from 0       7 / 13      11 / 17     23 / 24     51 / 41
+    //                   over 8K      36 / 40     67 / 58     126 / 89
+    //   head_dim 96     from 0       9 / 12      10 / 16     20 / 22     43 / 37
+    //                   over 8K      37 / 39     53 / 54     100 / 81
+    //     float32 rows  from 0       9 / 17      15 / 22     30 / 33     66 / 53
+    //                   over 8K      45 / 50     83 / 72     157 / 117
+    //   head_dim 128    from 0       11 / 14     12 / 18     24 / 25     52 / 40
+    //                   over 8K      43 / 44     62 / 60     114 / 90
+    //                   over 32K     118 / 96    194 / 160
     //     one head, two from 0       15 / 22     23 / 32
     //     one head, two over 8K      42 / 43     59 / 56
-    //     float32 rows  from 0                   16 / 17     34 / 26     74 / 43
-    //                   over 8K      50 / 52
-    //   head_dim 256    from 0       11 / 15     20 / 20     44 / 29     103 / 48
-    //                   over 8K      73 / 61     138 / 95
+    //     float32 rows  from 0       10 / 14     17 / 18     35 / 26     76 / 43
+    //                   over 8K      52 / 52     100 / 83    180 / 145
+    //   head_dim 256    from 0       11 / 15     21 / 20     44 / 30     102 / 49
+    //                   over 8K      76 / 61     141 / 100   268 / 171
     //     one head, two over 8K      74 / 60     130 / 93
-    //     float32 rows  from 0                   25 / 31     52 / 46     122 / 74
-    //                   over 8K      99 / 91
+    //     float32 rows  from 0       13 / 22     25 / 31     52 / 46     120 / 75
+    //                   over 8K      94 / 91     178 / 149   326 / 252
     // Twelve sequences of 1 to 4.5K, 8 heads, 42 / 84 / 168 columns each: head_dim 64 22 / 35, 39 / 37,
     // 52 / 48; 128 32 / 47, 53 / 51, 74 / 69, float32 rows -, 62 / 61, 104 / 101; 256 68 / 58, 92 / 74,
     // 149 / 119; 24 and 40 sequences of 256 with 42 columns 102 / 131, 122 / 137.
     constexpr bool F32 = DT == SP_DTYPE_F32;
-    // Up to a column group of this kernel's on each CU it is the better one over short contexts and no
-    // worse over 8K; past that it takes a second turn (300 rows over 16000, head_dim 128: 186 / 107).
-    // At head_dim 256, where it reads more, the other from there on.
+    // Up to a column group of this kernel's on each CU (8192 columns; 4096 in waves of 16) it is the
+    // better one over short contexts and within 7% of the other over 8K; past that it takes a second turn
+    // (300 rows over 16000, head_dim 128: 188 / 116), and the other is taken, though it is up to 2 us slower
+    // (7 with float32 rows) where such a call starts at position 0: it saves 9 to 40 over 8K. At head_dim
+    // 256, where this one reads more, the other from 4096 on: 4 us slower from 0 (float32 rows 9), 15 (3)
+    // faster over 8K.
     constexpr int MANY = 256 * 16 * CG + (HD == 256 ? 0 : 1), EACH = F32 ? 128 : 64;
     if (A.s.row && columns * A.H >= MANY && columns >= EACH * (long long)A.s.n_seq) return launch_wide<HD, DT>(A, s);
     if (columns > 16ll * A.s.n_seq) return launch<HD, DT, NW, CG>(A, s);
