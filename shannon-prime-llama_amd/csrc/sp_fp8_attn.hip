@@ -44,6 +44,7 @@ constexpr float P_TOP = 14.0f;  // log2 of the largest weight
 // score's own last bit. (Always in two steps: 40.5 us for 39.7 with 32 rows of each of 12 sequences at
 // head_dim 64, 32 / 8 heads.)
 constexpr float FAR_SCORE = 0x1p18f;
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > FAR_SCORE && fabsf(m) < INFINITY; }
 
 // Eight codes (two dwords) as fp16.
 __device__ __forceinline__ h8 to_half(unsigned a, unsigned b) {
@@ -485,12 +486,14 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
                     }
                 const float m_new = fmaxf(m[y], column_max(top));
                 float ref = m_new == -INFINITY ? 0.0f : m_new;
-                if (__any(fabsf(ref) > FAR_SCORE)) {
+                const bool far = is_far(m_new);
+                if (__any(far)) {  // (a column that is not stays as it is beside others)
+                    const float first = far ? ref : 0.0f;
 #pragma unroll
                     for (int n = 0; n < 4; n++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) s[y][n][i] -= ref;
-                    ref = 0.0f;
+                        for (int i = 0; i < 4; i++) s[y][n][i] -= first;
+                    ref -= first;
                 }
                 ref -= P_TOP;
                 const float alpha = weight(m[y], m_new);
@@ -831,12 +834,13 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     V o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = V{};
-    // m: the reference; off = W_TOP - m (huge: -m), 0 while m is -inf; the output's unit is 2^ev_now
-    float m = -INFINITY, off = 0.0f, l = 0.0f;
+    // m: the reference; off = W_TOP - m (far: -m), 0 while m is -inf; most: what a score and off
+    // may come to before the reference is raised; the output's unit is 2^ev_now
+    float m = -INFINITY, off = 0.0f, most = -INFINITY, l = 0.0f;
     int ev_now = 0;
-    // a column's reference is past FAR_SCORE: the fused difference of a score and the reference would not
+    // the column's reference is past FAR_SCORE: the fused difference of a score and the reference would not
     // be 0 where they are equal, and the constants added to the reference would be rounded
-    bool huge = false;
+    bool far = false;
     // of the block whose weights come next: score scale, exponent offset, its part in l
     float cs = 0.0f, shift = 0.0f, lmul = 1.0f;
     h8 p[NP][NH];
@@ -924,9 +928,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
     const auto settle = [&](const Facts &f, float top, V(&s)[RB]) __attribute__((always_inline)) {
         // never 0: a masked score stays -inf when it is multiplied
         cs = fmaxf(score_scale(A, qe + f.ek), 0x1p-126f);
-        // (huge: whatever is past the reference raises it, since what is up to half a float's step past it may
-        // be rounded to a whole one)
-        const bool raise = __builtin_fmaf(top, cs, off) > (m == -INFINITY ? -INFINITY : huge ? 0.0f : W_TOP + W_SLACK);
+        const bool raise = __builtin_fmaf(top, cs, off) > most;
         float scale = 1.0f;
         bool rescale = false;
         if (f.ev > ev_now || f.ev < ev_now - W_FOLD) {
@@ -942,11 +944,14 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn_wide(SpFp8Attn A) {
             scale *= alpha;
             m = m_new;
             rescale = true;
-            huge = __any(fabsf(m) > FAR_SCORE && m > -INFINITY);
-            off = m == -INFINITY ? 0.0f : (huge ? 0.0f : W_TOP) - m;
+            far = is_far(m);
+            off = m == -INFINITY ? 0.0f : (far ? 0.0f : W_TOP) - m;
+            // (far: whatever is past the reference raises it, since what is less than half a float's step past
+            // it may be rounded to a whole one)
+            most = m == -INFINITY ? -INFINITY : far ? 0.0f : W_TOP + W_SLACK;
         }
         shift = off;
-        if (huge) {  // the reference was rounded: round the scores as it was, and take it off first
+        if (far) {  // the reference was rounded: round the scores as it was, and take it off first
 #pragma unroll
             for (int i = 0; i < NE; i++) s[i / VL][i % VL] = s[i / VL][i % VL] * cs + off;
             cs = 1.0f;

@@ -146,3 +146,30 @@ def test_scales_whose_product_is_past_a_float():
                     P.check_attend(dtype, q * 2.0 ** 122, 2.0 ** -96)
                 if ke == -40:  # scores near 2^104
                     P.check_attend(dtype, q * 2.0 ** 110, 2.0 ** 34)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_neighbours_of_infinite_and_large_queries(dtype):
+    """Rows beside one whose query is infinite, or whose scores are past 2^25, are bit for bit what they
+    are beside an ordinary one (few rows; one sequence, so that the shares are the same)."""
+    rng = np.random.default_rng(12)
+    for hd, length in ((64, 300), (256, 2560)):
+        P = Pair(hd, 1, (length + 63) // 64)
+        P.fill(rng, [list(range(P.n_blocks))], [length], "f32", 0.3)
+        for row, n_q in ((None, 4), ([0, 9], 4)):
+            P.batch(P.table, [length], row)
+            q = torch.from_numpy(rng.standard_normal((P.n_rows, n_q, hd))).to(TORCH[dtype])
+            good = P.check_attend(dtype, q, 0.11)
+            for much in (float("inf"), -float("inf"), 3e4):  # past 2^25 at the larger scale
+                scale = 0.11 if math.isinf(much) else 2.0 ** 11
+                bad = q * (0.11 / scale) if scale != 0.11 else q.clone()
+                want = good if scale == 0.11 else P.attend(dtype, bad, scale)
+                bad[0, 1] = 0.0
+                bad[0, 1, 5] = much
+                got = P.attend(dtype, bad, scale)
+                others = np.ones(q.shape[:2], bool)
+                others[0, 1] = False
+                assert np.array_equal(got[0][others], want[0][others]), much
+                assert np.array_equal(got[1][others], want[1][others]), much
+                if math.isinf(much):
+                    assert not np.isfinite(got[0][0, 1]).any()
