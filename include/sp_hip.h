@@ -473,7 +473,10 @@ typedef struct {
  *
  * A position is in the cache if it is not negative and its table entry exists and lies in
  * [0, n_blocks). Others (a length past the table, an entry of -1) are never accessed: write
- * passes over them, read gives zeros, attention leaves them out. */
+ * passes over them, read gives zeros, attention leaves them out.
+ *
+ * Batches of more threads than a launch counts (32 bits: about 2^23 sequences, in attention 2^23
+ * groups of 16 to 256 query rows over all KV heads) are refused. */
 typedef struct {
     int            n_seq;
     int            table_stride;  /* entries of a table row */

@@ -77,6 +77,10 @@ inline int sp_fp8_prefill_rows(int hd) { return 512 * (hd == 256 ? 128 : 256); }
 
 #define SP_FP8_SLOTS 1024
 
+// A launch's threads along its first axis are counted in 32 bits.
+#define SP_FP8_MOST_THREADS 0xffffffffll
+#define SP_FP8_COPY_THREADS 256  // of a block of write or read
+
 __device__ __forceinline__ int sp_fp8_floor64(int x) { return x >> 6; }  // arithmetic: toward -inf
 
 // Rows and length of sequence i, whatever the arrays hold: 0 <= r0 <= r1 <= n_rows,

@@ -39,7 +39,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 constexpr float P_TOP = 14.0f;  // log2 of the largest weight
 
 // A score further than this from 0 has the maximum taken off first, which is exact at the maximum, and
-// P_TOP added then. Taken together they are rounded where a float counts in 2 or more (from 2^24 on):
+// P_TOP added then. Taken together they are rounded where a float counts in 4 or more (from 2^25 on):
 // the largest weight becomes 2^16, which is no fp16 number. Below, rounding them costs less than the
 // score's own last bit. (Always in two steps: 40.5 us for 39.7 with 32 rows of each of 12 sequences at
 // head_dim 64, 32 / 8 heads.)
@@ -1156,7 +1156,7 @@ hipError_t launch(const SpFp8Attn &A, hipStream_t s) {
                                      : (long long)A.s.n_seq * ((A.G + COLS - 1) / COLS);
     // shares: one per group, and at most target more over all KV heads
     const long long blocks = (groups + (a.target + A.H - 1) / A.H) * A.H;
-    if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
+    if (blocks * (NW * 64) > SP_FP8_MOST_THREADS) return hipErrorInvalidValue;
     const int cols = A.s.row ? COLS : (A.G < COLS ? A.G : COLS);
     const size_t lds = (size_t)NW * cols * (HD + 4) * sizeof(float);
     const long long each = A.s.row ? ((long long)A.s.n_rows * A.G + A.s.n_seq - 1) / A.s.n_seq : A.G;
@@ -1184,7 +1184,7 @@ hipError_t launch_wide(const SpFp8Attn &A, hipStream_t s) {
     a.least = share ? LEAST : 1 << 28;
     a.join = 0.0f;
     const long long blocks = (groups + (share ? (a.target + A.H - 1) / A.H : 0)) * A.H;
-    if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
+    if (blocks * (NW * 64) > SP_FP8_MOST_THREADS) return hipErrorInvalidValue;
     void *args[] = {&a};
     const hipError_t e = hipLaunchKernel((const void *)k_fp8_attn_wide<HD, DT, NW, CW>, dim3((unsigned)blocks), dim3(NW * 64),
                                          args, (size_t)HD * 512, s);

@@ -94,7 +94,7 @@ __device__ __forceinline__ unsigned recode(unsigned w, float down) {
     return pack4(x[0], x[1], x[2], x[3]);
 }
 
-constexpr int NT = 256;
+constexpr int NT = SP_FP8_COPY_THREADS;
 
 template <int HD, int DT>
 __global__ __launch_bounds__(NT) void k_fp8_write(SpFp8Copy A) {

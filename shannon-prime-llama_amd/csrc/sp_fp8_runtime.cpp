@@ -132,7 +132,10 @@ int copy_rows(const sp_hip_fp8_cache_t *c, int layer, const sp_hip_fp8_batch_t *
     const hipStream_t s = (hipStream_t)(stream ? stream : c->stream);
     if (!stream_ok(c, s, who)) return -1;
     if (b->n_rows == 0 || b->n_seq == 0 || (!k && !v)) return 0;
-    if (((long long)b->n_rows / 64 + 2ll * b->n_seq) > 0x7fffffffll) { sp_set_error("%s: too many rows", who); return -1; }
+    if (((long long)b->n_rows / 64 + 2ll * b->n_seq) * SP_FP8_COPY_THREADS > SP_FP8_MOST_THREADS) {
+        sp_set_error("%s: too many rows or sequences", who);
+        return -1;
+    }
     const OnDevice on(((const Fp8Priv *)c->priv)->device);
     if (!on.ok()) { sp_set_error("%s: the cache's device", who); return -1; }
     if (k) A.side[0] = layer_side(c, layer, false);
