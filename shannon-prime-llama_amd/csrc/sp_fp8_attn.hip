@@ -608,7 +608,7 @@ __global__ __launch_bounds__(NW * 64) void k_fp8_attn(SpFp8Attn A) {
 // within a factor of two and their unit always, so that the second part keeps its bits.
 //
 // Bound by the matrix cores and, beside them, by power: 2048 rows over 32768 positions, 32 / 8 heads
-// of 128, take 886 to 928 us by card in a row of calls (1.15 to 1.20 PFLOP/s; a large bf16 matrix product reaches 1.19 to
+// of 128, take 886 to 935 us by card in a row of calls (1.14 to 1.20 PFLOP/s; a large bf16 matrix product reaches 1.19 to
 // 1.24) and 930 to 960 alone, the matrix cores busy 51% of the cycles; the same loop with nothing but its matrix
 // instructions takes 595 us at a clock of 1.7 GHz. 2048 rows in a window of 1024, 16 / 8 heads of
 // 256: 59 us under the tracer, 52 in a run of calls (0.66 PFLOP/s), 18 blocks a column group with
