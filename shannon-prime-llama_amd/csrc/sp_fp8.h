@@ -118,6 +118,43 @@ __device__ __forceinline__ int sp_fp8_scan(int v, int lane) {
     return v + (lane < 16 ? 0 : lane < 32 ? a : lane < 48 ? b : c);
 }
 
+// The (sequence, cache block) pair of a grid index: sequence, block index in the sequence and
+// the call's rows of it. False: no such pair. Every lane of a wave agrees, in scalar registers.
+__device__ __forceinline__ bool sp_fp8_pair(const SpFp8Seqs &S, int p, int lane, int &seq, int &j, int &r0, int &first,
+                                            int &last) {
+    if (!S.row || S.n_seq == 1) {  // nothing to search
+        seq = S.row ? 0 : p;
+        int r1, len;
+        sp_fp8_seq(S, seq, r0, r1, len);
+        first = len - (r1 - r0);
+        last = len - 1;
+        j = sp_fp8_floor64(first) + (S.row ? p : 0);
+        return r1 > r0 && j <= sp_fp8_floor64(last);
+    }
+    for (int i0 = 0; i0 < S.n_seq; i0 += 64) {
+        const int i = i0 + lane;
+        int a = 0, b = 0, len = 0, n = 0;
+        if (i < S.n_seq) {
+            sp_fp8_seq(S, i, a, b, len);
+            if (b > a) n = sp_fp8_floor64(len - 1) - sp_fp8_floor64(len - (b - a)) + 1;
+        }
+        const int sum = sp_fp8_scan(n, lane);
+        const unsigned long long past = __ballot(sum > p);
+        if (past) {
+            const int l = __ffsll(past) - 1;
+            const auto of = [l](int v) { return __builtin_amdgcn_readlane(v, l); };
+            seq = i0 + l;
+            r0 = of(a);
+            first = of(len) - (of(b) - r0);
+            last = of(len) - 1;
+            j = sp_fp8_floor64(first) + p - (of(sum) - of(n));
+            return true;
+        }
+        p -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
 template <int DT>
 struct SpFp8Elem;
 template <>

@@ -28,43 +28,6 @@ using sp_fp8::u4;
 using sp_fp8::load4;
 using sp_fp8::store4;
 
-// The (sequence, cache block) pair of a grid index: sequence, block index in the sequence and
-// the call's rows of it. False: no such pair. Every lane of a wave agrees, in scalar registers.
-__device__ __forceinline__ bool pair_of(const SpFp8Seqs &S, int p, int lane, int &seq, int &j, int &r0, int &first,
-                                        int &last) {
-    if (!S.row || S.n_seq == 1) {  // nothing to search
-        seq = S.row ? 0 : p;
-        int r1, len;
-        sp_fp8_seq(S, seq, r0, r1, len);
-        first = len - (r1 - r0);
-        last = len - 1;
-        j = sp_fp8_floor64(first) + (S.row ? p : 0);
-        return r1 > r0 && j <= sp_fp8_floor64(last);
-    }
-    for (int i0 = 0; i0 < S.n_seq; i0 += 64) {
-        const int i = i0 + lane;
-        int a = 0, b = 0, len = 0, n = 0;
-        if (i < S.n_seq) {
-            sp_fp8_seq(S, i, a, b, len);
-            if (b > a) n = sp_fp8_floor64(len - 1) - sp_fp8_floor64(len - (b - a)) + 1;
-        }
-        const int sum = sp_fp8_scan(n, lane);
-        const unsigned long long past = __ballot(sum > p);
-        if (past) {
-            const int l = __ffsll(past) - 1;
-            const auto of = [l](int v) { return __builtin_amdgcn_readlane(v, l); };
-            seq = i0 + l;
-            r0 = of(a);
-            first = of(len) - (of(b) - r0);
-            last = of(len) - 1;
-            j = sp_fp8_floor64(first) + p - (of(sum) - of(n));
-            return true;
-        }
-        p -= __builtin_amdgcn_readlane(sum, 63);
-    }
-    return false;
-}
-
 // Byte of (position t, channel d) in a tile; t and d multiples of 4 give a dword's first byte
 // for K (channels d..d+3 of t) and, with t the quad's first position, for V (d's positions).
 template <int HD>
@@ -105,7 +68,7 @@ __global__ __launch_bounds__(NT) void k_fp8_write(SpFp8Copy A) {
     const SpFp8Side side = A.side[is_v];
     if (!side.codes) return;
     int seq, j, r0, first, last;
-    if (!pair_of(A.s, blockIdx.x, lane, seq, j, r0, first, last)) return;
+    if (!sp_fp8_pair(A.s, blockIdx.x, lane, seq, j, r0, first, last)) return;
     // the call's positions in this cache block: [lo, hi) of its 64
     const int lo = max(first - j * 64, 0), hi = min(last + 1 - j * 64, 64);
     const void *rows = A.rows[is_v];
@@ -233,7 +196,7 @@ __global__ __launch_bounds__(NT) void k_fp8_read(SpFp8Copy A) {
     const SpFp8Side side = A.side[is_v];
     if (!side.codes) return;
     int seq, j, r0, first, last;
-    if (!pair_of(A.s, blockIdx.x, lane, seq, j, r0, first, last)) return;
+    if (!sp_fp8_pair(A.s, blockIdx.x, lane, seq, j, r0, first, last)) return;
     const int blk = sp_fp8_block(A.s, seq, j);
     const int lo = max(first - j * 64, 0), hi = min(last + 1 - j * 64, 64);
     const long long row0 = (long long)r0 + ((long long)j * 64 - first);
