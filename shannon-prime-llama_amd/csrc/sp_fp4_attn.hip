@@ -1,0 +1,278 @@
+// sp_fp4_attn.hip -- attention over the 4-bit block cache (sp_block_attn.h): its codes as operands, and
+// which kernel a call takes.
+//
+// E2M1 codes times a power of two are exact in fp16 as long as the power stays in its range. A
+// block's codes are converted relative to its largest exponent, which is then the block's scale
+// for the loop (that of the 8-bit cache): exact for values down to 2^-23 of the block's largest
+// scale, below that rounded at 2^-24 of it.
+#include "sp_block_attn.h"
+#include "sp_fp4.h"
+
+namespace {
+
+using namespace sp_block;
+using sp_fp4::eight;
+using sp_fp4::Largest;
+using sp_fp4::relative;
+
+// The float with exponent byte b of `rel` (b known where this is expanded).
+__device__ __forceinline__ float power(unsigned rel, int b) {
+    return __int_as_float((b == 3 ? rel >> 1 : rel << (23 - 8 * b)) & 0x7f800000);
+}
+// Two codes: byte b of w.
+__device__ __forceinline__ h2 two(unsigned w, float scale, int b) {
+    return b == 0 ? sp_fp4::two<0>(w, scale) : b == 1 ? sp_fp4::two<1>(w, scale) : b == 2 ? sp_fp4::two<2>(w, scale)
+                                                                                          : sp_fp4::two<3>(w, scale);
+}
+
+struct Fp4 {
+    // A block in a wave's registers. K: lane (r, g) has plane 4 c + g of quad Q(r). V: lane (r, g) has
+    // quads 4 i + g of plane r (head_dim 64: half of plane r / 2; 96: lanes past plane 11 repeat it, and
+    // their rows of the output are dropped; 256: planes r and 16 + r).
+    template <int HD>
+    struct Few {
+        static constexpr int NC = HD / 32, PV = HD == 256 ? 2 : 1, CH = HD == 64 ? 4 : 8, ND = PV * CH, AT_ONCE = 2;
+        u4 kr[NC], vr[PV][4], vs[PV];
+        unsigned ks[NC];
+        static __device__ __forceinline__ int plane(int r, int x) { return HD == 64 ? r >> 1 : HD == 96 ? min(r, 11) : 16 * x + r; }
+        __device__ __forceinline__ void look_up(const SpFp8Attn &, long long) {}
+        __device__ __forceinline__ void load_k(const SpFp8Side &S, long long tile, int lane) {
+            const int r = lane & 15, g = lane >> 4;
+            const uint8_t *p = S.codes + tile * sp_fp4_tile(HD) + g * 256 + (4 * (r & 3) + (r >> 2)) * 16;
+            const uint8_t *e = S.exps + tile * sp_fp4_exps(HD) + r * 4;
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                kr[c] = *reinterpret_cast<const u4 *>(p + c * 1024);
+                ks[c] = *reinterpret_cast<const unsigned *>(e + c * 64);
+            }
+        }
+        __device__ __forceinline__ void load_v(const SpFp8Side &S, long long tile, int lane) {
+            const int r = lane & 15, g = lane >> 4;
+            const uint8_t *p = S.codes + tile * sp_fp4_tile(HD) + g * 16, *e = S.exps + tile * sp_fp4_exps(HD) + g * 16;
+#pragma unroll
+            for (int x = 0; x < PV; x++) {
+                const int n = plane(r, x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) vr[x][i] = *reinterpret_cast<const u4 *>(p + n * 256 + i * 64);
+                vs[x] = *reinterpret_cast<const u4 *>(e + (n >> 2) * 64);
+            }
+        }
+        // the block's largest exponent; from here on ks and vs are relative to it
+        __device__ __forceinline__ int k_exponent(int) {
+            Largest m;
+#pragma unroll
+            for (int c = 0; c < NC; c++) m.add(ks[c]);
+            const int top = uniform(sp_fp4::row_max(m.get()));  // the same in all four rows
+#pragma unroll
+            for (int c = 0; c < NC; c++) ks[c] = relative(ks[c], top);
+            return top - 127;
+        }
+        __device__ __forceinline__ int v_exponent(int) {
+            Largest m;
+#pragma unroll
+            for (int x = 0; x < PV; x++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) m.add(vs[x][i]);
+            const int top = sp_fp4::wave_max(m.get());
+#pragma unroll
+            for (int x = 0; x < PV; x++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) vs[x][i] = relative(vs[x][i], top);
+            if (HD == 64) {
+                const int half = (threadIdx.x & 1) * 16;
+#pragma unroll
+                for (int i = 0; i < 4; i++) vr[0][i] >>= half;
+            }
+            return top - 127;
+        }
+        // row blocks 2 u and 2 u + 1 of step c
+        __device__ __forceinline__ void k_rows(int c, int u, h8 &a, h8 &b) const {
+            a = eight(kr[c][2 * u], power(ks[c], 2 * u));
+            b = eight(kr[c][2 * u + 1], power(ks[c], 2 * u + 1));
+        }
+        // channels d and d + 1: one byte of each of the lane's sixteen positions, turned
+        __device__ __forceinline__ void v_rows(int d, h8 (&a)[AT_ONCE][2]) const {
+            const int x = d / CH, byte = d % CH / 2;
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                h2 c[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) c[k] = two(vr[x][2 * s + k / 4][k % 4], power(vs[x][2 * s + k / 4], k % 4), byte);
+#pragma unroll
+                for (int o = 0; o < 2; o++)
+                    a[o][s] = h8{c[0][o], c[1][o], c[2][o], c[3][o], c[4][o], c[5][o], c[6][o], c[7][o]};
+            }
+        }
+        // position of value i of row block n, from the lane's first; its step and place among V's operands
+        static constexpr __device__ __forceinline__ int at(int n, int i) { return 16 * i + n; }
+        static constexpr __device__ __forceinline__ int step(int, int i) { return i / 2; }
+        static constexpr __device__ __forceinline__ int place(int n, int i) { return i % 2 * 4 + n; }
+        static __device__ __forceinline__ void put(float *rec, const f4 (&o)[ND], int g, float unit) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = 4 * g + i;
+                if (HD == 96 && r >= 12) break;
+#pragma unroll
+                for (int d = 0; d < ND; d += 4)
+                    *reinterpret_cast<f4 *>(rec + d / CH * 128 + r * CH + d % CH) =
+                        f4{o[d][i], o[d + 1][i], o[d + 2][i], o[d + 3][i]} * unit;
+            }
+        }
+    };
+
+    // A block on its way into LDS: half of the threads bring K, half V.
+    // A piece of K is a quad of a plane: one operand row of eight channels for each of its positions.
+    // A piece of V is half of a plane's channels for the eight positions that a lane of the product has
+    // in one step: four operand rows. Rows are put where the eight lanes that write at once, and
+    // the lanes that read, meet no bank twice: at CW 32 the low two bits of a row's place are
+    // turned by the next two but one, at CW 16 the lowest by the fourth, and row blocks lie two
+    // places further apart.
+    template <int HD, int NT, int CW>
+    struct Wide {
+        static constexpr int HT = NT / 2, NW = NT / 64;
+        static constexpr int NS = CW == 32 ? HD / 16 : HD / 32, NP = CW == 32 ? 4 : 2, PAD = CW == 32 ? 0 : 2;
+        static constexpr int PIECES = 2 * HD, PER = (PIECES + HT - 1) / HT;
+        // fp16 eights: of a block's place in LDS, and of a row block of it
+        static constexpr int K_ROW = NS * 64 + PAD, K_PLACE = 64 / CW * K_ROW;
+        static constexpr int V_ROW = NP * 64 + PAD, V_PLACE = HD / CW * V_ROW;
+        static constexpr int LDS = 2 * (K_PLACE + V_PLACE) * 16, BYTES = LDS + 64 * 4;
+        static_assert(64 % NW == 0);
+        struct Raw {
+            u4 x[2 * PER];
+            unsigned e[2 * PER];
+        };
+        static constexpr __device__ __forceinline__ int at(int lane) { return lane ^ ((lane >> 3) & (CW == 32 ? 3 : 1)); }
+        static __device__ __forceinline__ bool mine(int x) { return PER * HT == PIECES || x < PIECES; }
+        // The largest exponents of the 64 blocks that the lanes have: each wave finds those of its share
+        // of them, coalesced, and all meet in LDS.
+        static __device__ __forceinline__ void look_up(const SpFp8Attn &A, int h, int blk, int w, int lane, int *area, int &ekb,
+                                                       int &evb) {
+            constexpr int EACH = 64 / NW, DW = sp_fp4_exps(HD) / 4, TWICE = DW > 64 ? 2 : 1;
+            unsigned ke[EACH][TWICE], ve[EACH][TWICE];
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                const int b = max(__builtin_amdgcn_readlane(blk, w * EACH + i), 0);
+                const long long tile = ((long long)b * A.H + h) * DW;
+#pragma unroll
+                for (int t = 0; t < TWICE; t++) {
+                    const int x = min(lane + t * 64, DW - 1);
+                    ke[i][t] = reinterpret_cast<const unsigned *>(A.k.exps)[tile + x];
+                    ve[i][t] = reinterpret_cast<const unsigned *>(A.v.exps)[tile + x];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                Largest k, v;
+#pragma unroll
+                for (int t = 0; t < TWICE; t++) {
+                    k.add(ke[i][t]);
+                    v.add(ve[i][t]);
+                }
+                const int both = sp_fp4::wave_max(k.get()) | sp_fp4::wave_max(v.get()) << 8;
+                if (lane == 0) area[w * EACH + i] = both;
+            }
+            lds_barrier();
+            ekb = area[lane] & 255;
+            evb = area[lane] >> 8;
+        }
+        static __device__ __forceinline__ void fetch_k(const SpFp8Side &S, long long tile, int st, Raw &raw) {
+            const uint8_t *p = S.codes + tile * sp_fp4_tile(HD), *e = S.exps + tile * sp_fp4_exps(HD);
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int x = st + i * HT, q = x & 15;  // x = (plane, quad)
+                if (!mine(x)) continue;
+                raw.x[i] = *reinterpret_cast<const u4 *>(p + x * 16);
+                raw.e[i] = *reinterpret_cast<const unsigned *>(e + (x >> 6) * 64 + (q & 3) * 16 + (q >> 2) * 4);
+            }
+        }
+        // x = (plane / 4, step, lane group, plane % 4, half): its first quad (the second is HOP further)
+        static constexpr int HOP = CW == 32 ? 2 : 4;
+        static __device__ __forceinline__ int quad(int x) {
+            const int y = (x >> 3) & 7;
+            return CW == 32 ? (y >> 1) * 4 + (y & 1) : (y >> 2) * 8 + (y & 3);
+        }
+        static __device__ __forceinline__ void fetch_v(const SpFp8Side &S, long long tile, int st, Raw &raw) {
+            const uint8_t *p = S.codes + tile * sp_fp4_tile(HD), *e = S.exps + tile * sp_fp4_exps(HD);
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int x = st + i * HT, q = quad(x), n = (x >> 6) * 4 + ((x >> 1) & 3);
+                if (!mine(x)) continue;
+#pragma unroll
+                for (int o = 0; o < 2; o++) {
+                    const int qo = q + o * HOP;
+                    raw.x[2 * i + o] = *reinterpret_cast<const u4 *>(p + n * 256 + qo * 16);
+                    raw.e[2 * i + o] = *reinterpret_cast<const unsigned *>(e + (x >> 6) * 64 + (qo & 3) * 16 + (qo >> 2) * 4);
+                }
+            }
+        }
+        static __device__ __forceinline__ void stage_k(Raw &raw, int st, int top, h8 *to) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int x = st + i * HT, q = x & 15, n = x >> 4;
+                if (!mine(x)) continue;
+                const unsigned rel = relative(raw.e[i], top + 127);
+                // its first position's lane and row block
+                const int lane = CW == 32 ? (n & 1) * 32 + 4 * (q & 7) : (n & 3) * 16 + 4 * (q & 3);
+                h8 *d = to + (CW == 32 ? (q >> 3) * K_ROW + (n >> 1) * 64 : (q >> 2) * K_ROW + (n >> 2) * 64);
+#pragma unroll
+                for (int b = 0; b < 4; b++) d[at(lane + b)] = eight(raw.x[i][b], power(rel, b));
+            }
+        }
+        static __device__ __forceinline__ void stage_v(Raw &raw, int st, int top, h8 *to) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int x = st + i * HT, y = (x >> 3) & 7, n = (x >> 6) * 4 + ((x >> 1) & 3), half = x & 1;
+                if (!mine(x)) continue;
+                h2 c[2][8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const unsigned w = raw.x[2 * i + k / 4][k % 4] >> (16 * half);
+                    const float scale = power(relative(raw.e[2 * i + k / 4], top + 127), k % 4);
+                    c[0][k] = two(w, scale, 0);
+                    c[1][k] = two(w, scale, 1);
+                }
+                const int lane = CW == 32 ? (y & 1) * 32 + 8 * (n & 3) + 4 * half : (y & 3) * 16 + 8 * (n & 1) + 4 * half;
+                h8 *d = to + (CW == 32 ? (n >> 2) * V_ROW + (y >> 1) * 64 : (n >> 1) * V_ROW + (y >> 2) * 64);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const h2 *a = c[j / 2];
+                    const int o = j % 2;
+                    d[at(lane + j)] = h8{a[0][o], a[1][o], a[2][o], a[3][o], a[4][o], a[5][o], a[6][o], a[7][o]};
+                }
+            }
+        }
+    };
+};
+
+template <int HD, int DT>
+hipError_t launch_dt(const SpFp8Attn &A, hipStream_t s) {
+    constexpr int NW = HD == 256 ? 4 : 8;
+    constexpr int CG = HD == 256 || DT == SP_DTYPE_F32 ? 1 : 2;
+    const long long columns = (long long)A.s.n_rows * A.G;  // of each KV head
+    constexpr int MANY = 256 * 16 * CG + (HD == 256 ? 0 : 1), EACH = DT == SP_DTYPE_F32 ? 128 : 64;
+    if (A.s.row && columns * A.H >= MANY && columns >= EACH * (long long)A.s.n_seq) return launch_wide<Fp4, HD, DT>(A, s);
+    if (columns > 16ll * A.s.n_seq) return launch<Fp4, HD, DT, NW, CG>(A, s);
+    return launch<Fp4, HD, DT, NW, 1>(A, s);
+}
+
+template <int HD>
+hipError_t launch_hd(const SpFp8Attn &A, int dtype, hipStream_t s) {
+    switch (dtype) {
+        case SP_DTYPE_F32: return launch_dt<HD, SP_DTYPE_F32>(A, s);
+        case SP_DTYPE_F16: return launch_dt<HD, SP_DTYPE_F16>(A, s);
+        case SP_DTYPE_BF16: return launch_dt<HD, SP_DTYPE_BF16>(A, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t sp_fp4_launch_attn(const SpFp8Attn &A, int hd, int dtype, hipStream_t s) {
+    switch (hd) {
+        case 64: return launch_hd<64>(A, dtype, s);
+        case 96: return launch_hd<96>(A, dtype, s);
+        case 128: return launch_hd<128>(A, dtype, s);
+        case 256: return launch_hd<256>(A, dtype, s);
+    }
+    return hipErrorInvalidValue;
+}
