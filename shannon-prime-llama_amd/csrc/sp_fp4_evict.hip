@@ -224,10 +224,15 @@ hipError_t launch_weigh(const SpFp4Weigh &A, int dtype, hipStream_t s) {
 // ---------------------------------------------------------------------------
 // evict
 // ---------------------------------------------------------------------------
-// Which positions stay: one block of threads for each (sequence, KV head) finds the weight of the last
-// one that stays by three counts of its bits from the top (11, 11 and 10), then writes the kept
-// positions in order: each wave counts its run of the positions, and with the counts of the
-// waves before it knows where its own go.
+// Which positions stay: one block of threads for each (sequence, KV head) finds the key (the weight's
+// bits, in order) of the last one that stays, by counts of eleven of its bits at a time from the top
+// of the range that the keys have (attention weights span few of a float's octaves: bits above the
+// range would put them into few bins, where lanes that meet take turns: 13 us for 2 with 32768
+// positions). Then it writes the kept positions in order: each wave counts its run of the
+// positions, and with the counts of the waves before it knows where its own go.
+//
+// A wave's run is consecutive, and a lane has four neighbours of each 256 positions. The keys are made
+// once and kept in LDS where it holds them; those of longer sequences are made again for each pass.
 constexpr int SN = SP_FP4_EVICT_THREADS;
 
 // Order of weights as unsigned numbers: NaN below all, -0 as 0.
@@ -235,124 +240,206 @@ __device__ __forceinline__ unsigned key_of(float w) {
     const unsigned u = __float_as_uint(w + 0.0f);
     return w != w ? 0u : (u >> 31) ? ~u : u | 0x80000000u;
 }
+constexpr unsigned NO_KEY = 0xffffffffu;  // of a position that stays whatever its weight, and of places that have none
 
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+#define SP_MAX(ctrl) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true))
+    SP_MAX(0x128);  // row_ror 8, 4, 2, 1
+    SP_MAX(0x124);
+    SP_MAX(0x122);
+    SP_MAX(0x121);
+#undef SP_MAX
+    return max(max((unsigned)__builtin_amdgcn_readlane((int)v, 0), (unsigned)__builtin_amdgcn_readlane((int)v, 16)),
+               max((unsigned)__builtin_amdgcn_readlane((int)v, 32), (unsigned)__builtin_amdgcn_readlane((int)v, 48)));
+}
+
+constexpr int MOST_KEYS = 36 * 1024;  // that LDS holds beside the counts
+
+// AT_ONCE: loads of a lane that are made together.
+template <bool HELD, int AT_ONCE>
 __global__ __launch_bounds__(SN) void k_fp4_select(SpFp4Evict A) {
-    constexpr int NW = SN / 64, BINS = 2048;
+    constexpr int NW = SN / 64, BITS = 11, BINS = 1 << BITS;
+    extern __shared__ __align__(16) unsigned keys[];
     __shared__ int bins[BINS];
     __shared__ int wave_n[NW], wave_t[NW];
-    __shared__ int found_bin, found_above;
+    __shared__ unsigned wave_hi[NW], wave_lo[NW];
+    __shared__ int found_bin, found_above, found_here;
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int h = blockIdx.x % A.H, seq = blockIdx.x / A.H;
     int a, b, n;
     sp_fp8_seq(A.s, seq, a, b, n);
+    n = uniform(n);
     int *kept = A.kept + ((long long)seq * A.H + h) * A.keep;
     if (n <= A.keep) {
         for (int j = tid; j < A.keep; j += SN) kept[j] = j < n ? j : -1;
         return;
     }
-    int bad = 0;
-    for (int j = tid; j < (n + 63) >> 6; j += SN) bad |= sp_fp8_block(A.s, seq, j) < 0;
+    if (n > (long long)A.s.stride * 64) {
+        for (int j = tid; j < A.keep; j += SN) kept[j] = -1;
+        return;
+    }
+    // wave w has positions [p0, p1), a lane the p0 + 256 i + 4 lane + (0 .. 3)
+    const int run = ((n + 4 * SN - 1) / (4 * SN)) * 256, p0 = min(w * run, n), p1 = min(p0 + run, n);
+    const int *table = A.s.table + (long long)seq * A.s.stride;
+    const int last = ((n + 63) >> 6) - 1, behind = n - A.recent;
+    int bad = 0;  // a block that is missing
+    // keys from memory: of positions p + 256 i + 4 lane + (0 .. 3)
+    const auto make = [&](int p, uint4 (&key)[AT_ONCE]) __attribute__((always_inline)) {
+        int blk[AT_ONCE];
+        float4 weight[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) blk[i] = table[min((p + i * 256 + 4 * lane) >> 6, last)];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            bad |= blk[i] < 0 || blk[i] >= A.s.n_blocks;
+            weight[i] = *reinterpret_cast<const float4 *>(
+                A.weight + ((long long)min(max(blk[i], 0), A.s.n_blocks - 1) * A.H + h) * 64 + (4 * lane & 63));
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            const int at = p + i * 256 + 4 * lane;
+            const auto one = [&](int k, float x) { return at + k < A.first || at + k >= behind ? NO_KEY : key_of(x); };
+            key[i] = uint4{one(0, weight[i].x), one(1, weight[i].y), one(2, weight[i].z), one(3, weight[i].w)};
+        }
+    };
+    // the lane's keys in order, four at a time: f(their first position, key, key, key, key)
+    const auto each = [&](auto f) __attribute__((always_inline)) {
+        if constexpr (HELD) {
+#pragma unroll 2
+            for (int p = p0; p < p1; p += 256) {
+                const uint4 k = *reinterpret_cast<const uint4 *>(keys + p + 4 * lane);
+                f(p + 4 * lane, k.x, k.y, k.z, k.w);
+            }
+        } else {
+            for (int p = p0; p < p1; p += 256 * AT_ONCE) {
+                uint4 k[AT_ONCE];
+                make(p, k);
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; i++)
+                    if (p + i * 256 < p1) f(p + i * 256 + 4 * lane, k[i].x, k[i].y, k[i].z, k[i].w);
+            }
+        }
+    };
+    // ---- the keys' range ----
+    unsigned hi = 0, lo = 0;  // largest key + 1, complement of the least (0: no key)
+    for (int p = p0; p < p1; p += 256 * AT_ONCE) {
+        uint4 k[AT_ONCE];
+        make(p, k);
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; i++) {
+            hi = max(max(hi, max(k[i].x + 1, k[i].y + 1)), max(k[i].z + 1, k[i].w + 1));
+            lo = max(max(lo, max(~k[i].x, ~k[i].y)), max(~k[i].z, ~k[i].w));
+            if (HELD && p + i * 256 < p1) *reinterpret_cast<uint4 *>(keys + p + i * 256 + 4 * lane) = k[i];
+        }
+    }
+    hi = wave_umax(hi);
+    lo = wave_umax(lo);
+    for (int k = tid; k < BINS; k += SN) bins[k] = 0;
+    if (lane == 0) {
+        wave_hi[w] = hi;
+        wave_lo[w] = lo;
+    }
     if (__syncthreads_or(bad)) {
         for (int j = tid; j < A.keep; j += SN) kept[j] = -1;
         return;
     }
-    const int lo = A.first, hi = n - A.recent;  // of these `need` stay
-    const int need = A.keep - A.first - A.recent;
-    const int *table = A.s.table + (long long)seq * A.s.stride;
-    const auto key_at = [&](int p) { return key_of(A.weight[((long long)table[p >> 6] * A.H + h) * 64 + (p & 63)]); };
-    // keys of `limit` and more stay, of those that equal it `ties` if exact
-    unsigned limit = 0xffffffffu;
-    int ties = 0;
-    bool exact = true;
-    if (need > 0) {
-        int want = need;  // of the keys that agree with `limit` in the bits above `shift`
-        unsigned prefix = 0;
-        int shift = 32;
-        for (int pass = 0; pass < 3; pass++) {
-            const int bits = pass < 2 ? 11 : 10, down = shift - bits;
+    hi = wave_umax(lane < NW ? wave_hi[lane] : 0u);
+    lo = wave_umax(lane < NW ? wave_lo[lane] : 0u);
+    const unsigned least = ~lo;
+    // ---- the key of the last that stays: of those in [limit, limit + 2^shift) `want` stay ----
+    int want = A.keep - A.first - A.recent, here = n - A.first - A.recent;
+    unsigned limit = least;
+    int shift = want && hi > least + 1 ? 32 - __clz(hi - 1 - least) : 0;
+    for (bool fresh = true; shift > 0; fresh = false) {
+        const int down = max(shift - BITS, 0);
+        // (no key but NO_KEY is past it: with 32 bits the range ends there)
+        const unsigned span = shift == 32 ? NO_KEY - limit : 1u << shift;
+        if (!fresh) {
             for (int k = tid; k < BINS; k += SN) bins[k] = 0;
             __syncthreads();
-            for (int p = lo + tid; p < hi; p += SN) {
-                const unsigned key = key_at(p);
-                if (pass == 0 || key >> shift == prefix) atomicAdd(&bins[(key >> down) & ((1 << bits) - 1)], 1);
-            }
-            __syncthreads();
-            // sums from the top: thread 0 has the two highest bins
-            const int top = (1 << bits) - 1 - 2 * tid;
-            const int c1 = top >= 0 ? bins[top] : 0, c0 = top >= 1 ? bins[top - 1] : 0;
-            const int sum = sp_fp8_scan(c0 + c1, lane);
-            if (lane == 63) wave_n[w] = sum;
-            __syncthreads();
-            int before = sum - c0 - c1;
-            for (int k = 0; k < w; k++) before += wave_n[k];
-            if (before < want && before + c0 + c1 >= want) {
-                const bool second = before + c1 < want;
-                found_bin = second ? top - 1 : top;
-                found_above = second ? before + c1 : before;
-            }
-            __syncthreads();
-            prefix = prefix << bits | (unsigned)found_bin;
-            want -= found_above;
-            shift = down;
-            const int here = bins[found_bin];
-            __syncthreads();
-            if (here == want) {  // all of them stay
-                exact = false;
-                break;
-            }
         }
-        limit = prefix << shift;
-        ties = exact ? want : 0;
+        const auto count = [&](unsigned k) __attribute__((always_inline)) {
+            if (k - limit < span && k != NO_KEY) atomicAdd(&bins[(k - limit) >> down], 1);
+        };
+        each([&](int, unsigned k0, unsigned k1, unsigned k2, unsigned k3) __attribute__((always_inline)) {
+            count(k0);
+            count(k1);
+            count(k2);
+            count(k3);
+        });
+        __syncthreads();
+        // sums from the top: thread 0 has the two highest bins
+        const int top = BINS - 1 - 2 * tid, c1 = bins[top], c0 = bins[top - 1];
+        const int sum = sp_fp8_scan(c0 + c1, lane);
+        if (lane == 63) wave_n[w] = sum;
+        __syncthreads();
+        int before = sum - c0 - c1;
+        for (int k = 0; k < w; k++) before += wave_n[k];
+        if (before < want && before + c0 + c1 >= want) {
+            const bool second = before + c1 < want;
+            found_bin = second ? top - 1 : top;
+            found_above = second ? before + c1 : before;
+            found_here = second ? c0 : c1;
+        }
+        __syncthreads();
+        limit += (unsigned)found_bin << down;
+        want -= found_above;
+        here = found_here;
+        shift = down;
+        if (here == want) break;  // all of them stay
     }
-    // ---- in order: wave w has positions [w * run, (w + 1) * run) ----
-    const int run = ((n + SN - 1) / SN) * 64, p0 = w * run, p1 = min(p0 + run, n);
-    // 2: stays, 1: equals the limit, 0: goes
-    const auto verdict = [&](int p) {
-        if (p < lo || p >= hi) return 2;
-        if (need == 0) return 0;
-        const unsigned key = key_at(p);
-        return key > limit || (!exact && key == limit) ? 2 : key == limit ? 1 : 0;
-    };
-    int n_stay = 0, n_tie = 0;
-    for (int p = p0; p < p1; p += 64) {
-        const int v = p + lane < p1 ? verdict(p + lane) : 0;
-        n_stay += __popcll(__ballot(v == 2));
-        n_tie += __popcll(__ballot(v == 1));
-    }
-    __syncthreads();
-    if (lane == 0) {
+    // Keys from `over` on stay; but of those that equal the limit, where they are more than are wanted, the
+    // first `want`. (None wanted, and none between: `over` is NO_KEY alone.)
+    const bool tied = here != want && want > 0;
+    const unsigned over = want == 0 ? NO_KEY : tied ? limit + 1 : limit;
+    int n_stay = 0, n_tie = 0;  // of this lane, then of the wave
+    each([&](int p, unsigned k0, unsigned k1, unsigned k2, unsigned k3) __attribute__((always_inline)) {
+        n_stay += (k0 >= over && p < p1) + (k1 >= over && p + 1 < p1) + (k2 >= over && p + 2 < p1) + (k3 >= over && p + 3 < p1);
+        if (tied) n_tie += (k0 == limit) + (k1 == limit) + (k2 == limit) + (k3 == limit);
+    });
+    n_stay = sp_fp8_scan(n_stay, lane);
+    n_tie = sp_fp8_scan(n_tie, lane);
+    if (lane == 63) {
         wave_n[w] = n_stay;
         wave_t[w] = n_tie;
     }
     __syncthreads();
-    int at = 0, tied = 0;  // kept before this wave's run, and ties met
+    int at = 0, met = 0;  // kept before this wave's run, and keys at the limit met
     for (int k = 0; k < w; k++) {
-        at += wave_n[k] + max(min(wave_t[k], ties - tied), 0);
-        tied += wave_t[k];
+        at += wave_n[k] + max(min(wave_t[k], want - met), 0);
+        met += wave_t[k];
     }
-    const unsigned long long below = (1ull << lane) - 1;
-    for (int p = p0; p < p1; p += 64) {
-        const int v = p + lane < p1 ? verdict(p + lane) : 0;
-        const unsigned long long t = __ballot(v == 1);
-        const bool stays = v == 2 || (v == 1 && tied + __popcll(t & below) < ties);
-        const unsigned long long s = __ballot(stays);
-        const int j = at + __popcll(s & below);
-        if (stays && j < A.keep) kept[j] = p + lane;
-        at += __popcll(s);
-        tied += __popcll(t);
-    }
+    each([&](int p, unsigned k0, unsigned k1, unsigned k2, unsigned k3) __attribute__((always_inline)) {
+        bool stays[4] = {k0 >= over && p < p1, k1 >= over && p + 1 < p1, k2 >= over && p + 2 < p1, k3 >= over && p + 3 < p1};
+        if (tied) {
+            const int mine = (k0 == limit) + (k1 == limit) + (k2 == limit) + (k3 == limit), sum = sp_fp8_scan(mine, lane);
+            int t = met + sum - mine;
+            const unsigned k[4] = {k0, k1, k2, k3};
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (k[i] == limit) stays[i] = t++ < want;
+            met += __builtin_amdgcn_readlane(sum, 63);
+        }
+        const int mine = stays[0] + stays[1] + stays[2] + stays[3], sum = sp_fp8_scan(mine, lane);
+        int j = at + sum - mine;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (stays[i] && j < A.keep) kept[j] = p + i;
+            j += stays[i];
+        }
+        at += __builtin_amdgcn_readlane(sum, 63);
+    });
 }
 
-// Rows to their new places: one block of threads for each (sequence, KV head, side, 32 channels) goes up
-// the places. A row never moves up, so a place's row lies at or behind it: a round that
-// has loaded its rows may store them, whatever the rounds before and behind do.
-constexpr int MN = SP_FP4_EVICT_THREADS;
-constexpr int MOVES = 8;  // dwords of a thread a round: 2048 places
-
-__global__ __launch_bounds__(MN) void k_fp4_move(SpFp4Evict A) {
-    constexpr int ROUND = MN / 4 * MOVES;
-    const int tid = threadIdx.x, plane = tid >> 8, lane = tid & 255;
-    const int h = blockIdx.x % A.H, seq = blockIdx.x / A.H, is_v = blockIdx.y & 1, G = blockIdx.y >> 1;
+// Rows to their new places: a block of threads for each (sequence, KV head, side) and PLANES planes of
+// eight channels goes up the places. A row never moves up, so a place's row lies at or behind it:
+// a round that has loaded its rows may store them, whatever the rounds before and behind do. A
+// round is so large (NT places, ROUND of a thread) that most calls take one.
+template <int NT, int PLANES, int ROUND>
+__global__ __launch_bounds__(NT) void k_fp4_move(SpFp4Evict A) {
+    constexpr int PLACES = NT * ROUND;
+    const int tid = threadIdx.x;
+    const int h = blockIdx.x % A.H, seq = blockIdx.x / A.H, is_v = blockIdx.y & 1, n0 = (blockIdx.y >> 1) * PLANES;
     int a, b, n;
     sp_fp8_seq(A.s, seq, a, b, n);
     if (n <= A.keep) return;
@@ -360,42 +447,63 @@ __global__ __launch_bounds__(MN) void k_fp4_move(SpFp4Evict A) {
     if (kept[0] < 0) return;  // a block is missing
     const SpFp8Side side = A.side[is_v];
     const int *table = A.s.table + (long long)seq * A.s.stride;
-    const int tile = A.NC * 1024, exps = A.NC * 64;
-    const bool with_exp = plane == 0, with_weight = plane == 1 && is_v == 0 && G == 0;
-    for (int j0 = 0; j0 < A.keep; j0 += ROUND) {
-        unsigned code[MOVES];
-        int exp[MOVES];
-        float weight[MOVES];
-        bool moves[MOVES];
+    const int tile = A.NC * 256, exps = A.NC * 64;  // dwords of codes, bytes of exponents
+    const bool with_exp = n0 % 4 == 0, with_weight = is_v == 0 && n0 == 0;
+    unsigned *codes = reinterpret_cast<unsigned *>(side.codes) + n0 * 64;
+    uint8_t *exp_plane = side.exps + n0 / 4 * 64;
+    for (int j0 = 0; j0 < A.keep; j0 += PLACES) {
+        int p[ROUND];
+        long long from[ROUND], to[ROUND];  // tiles
 #pragma unroll
-        for (int k = 0; k < MOVES; k++) {
-            const int j = j0 + k * (MN / 4) + lane;
-            const int p = j < A.keep ? kept[j] : j;
-            moves[k] = p != j;
-            if (!moves[k]) continue;
-            const long long at = (long long)table[p >> 6] * A.H + h;
-            code[k] = reinterpret_cast<const unsigned *>(side.codes + at * tile)[(G * 4 + plane) * 64 + (p & 63)];
-            if (with_exp) exp[k] = side.exps[at * exps + G * 64 + sp_fp4_place(p & 63)];
-            if (with_weight) weight[k] = A.weight[at * 64 + (p & 63)];
+        for (int k = 0; k < ROUND; k++) {
+            const int j = j0 + k * NT + tid;
+            p[k] = j < A.keep ? kept[j] : j;
+        }
+#pragma unroll
+        for (int k = 0; k < ROUND; k++) {
+            const int j = j0 + k * NT + tid;
+            from[k] = to[k] = 0;
+            if (p[k] == j) continue;
+            from[k] = (long long)table[p[k] >> 6] * A.H + h;
+            to[k] = (long long)table[j >> 6] * A.H + h;
+        }
+        unsigned code[ROUND][PLANES];
+        uint8_t e[ROUND];
+        float weight[ROUND];
+#pragma unroll
+        for (int k = 0; k < ROUND; k++) {
+            const int j = j0 + k * NT + tid;
+            if (p[k] == j) continue;
+#pragma unroll
+            for (int x = 0; x < PLANES; x++) code[k][x] = codes[from[k] * tile + x * 64 + (p[k] & 63)];
+            if (with_exp) e[k] = exp_plane[from[k] * exps + sp_fp4_place(p[k] & 63)];
+            if (with_weight) weight[k] = A.weight[from[k] * 64 + (p[k] & 63)];
         }
         // what this round loads is in registers before any of it is stored over
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < MOVES; k++) {
-            if (!moves[k]) continue;
-            const int j = j0 + k * (MN / 4) + lane;
-            const long long at = (long long)table[j >> 6] * A.H + h;
-            reinterpret_cast<unsigned *>(side.codes + at * tile)[(G * 4 + plane) * 64 + (j & 63)] = code[k];
-            if (with_exp) side.exps[at * exps + G * 64 + sp_fp4_place(j & 63)] = (uint8_t)exp[k];
-            if (with_weight) A.weight[at * 64 + (j & 63)] = weight[k];
+        for (int k = 0; k < ROUND; k++) {
+            const int j = j0 + k * NT + tid;
+            if (p[k] == j) continue;
+#pragma unroll
+            for (int x = 0; x < PLANES; x++) codes[to[k] * tile + x * 64 + (j & 63)] = code[k][x];
+            if (with_exp) exp_plane[to[k] * exps + sp_fp4_place(j & 63)] = e[k];
+            if (with_weight) A.weight[to[k] * 64 + (j & 63)] = weight[k];
         }
     }
     // behind the last place nothing counts in its block's largest exponent
     const int tail = A.keep & 63;
-    if (tail == 0) return;
+    if (tail == 0 || !with_exp) return;
     const int t = tail + tid;
-    if (t < 64) side.exps[((long long)table[A.keep >> 6] * A.H + h) * exps + G * 64 + sp_fp4_place(t)] = SP_FP4_LEAST;
+    if (t < 64) exp_plane[((long long)table[A.keep >> 6] * A.H + h) * exps + sp_fp4_place(t)] = SP_FP4_LEAST;
+}
+
+template <int NT, int PLANES, int ROUND>
+hipError_t launch_move(const SpFp4Evict &A, hipStream_t s) {
+    void *args[] = {const_cast<SpFp4Evict *>(&A)};
+    return hipLaunchKernel((const void *)k_fp4_move<NT, PLANES, ROUND>, dim3((unsigned)(A.H * A.s.n_seq), (unsigned)(2 * A.NC * 4 / PLANES)),
+                           dim3(NT), args, 0, s);
 }
 
 }  // namespace
@@ -412,7 +520,15 @@ hipError_t sp_fp4_launch_weigh(const SpFp4Weigh &A, int hd, int dtype, hipStream
 
 hipError_t sp_fp4_launch_evict(const SpFp4Evict &A, hipStream_t s) {
     void *args[] = {const_cast<SpFp4Evict *>(&A)};
-    const hipError_t e = hipLaunchKernel((const void *)k_fp4_select, dim3((unsigned)(A.H * A.s.n_seq)), dim3(SN), args, 0, s);
+    // no sequence is longer than its table row
+    const long long most = ((long long)A.s.stride * 64 + 255) / 256 * 256;
+    const bool held = most <= MOST_KEYS;
+    const void *select = !held ? (const void *)k_fp4_select<false, 4>
+                       : most <= 8 * SN ? (const void *)k_fp4_select<true, 2> : (const void *)k_fp4_select<true, 8>;
+    const hipError_t e = hipLaunchKernel(select, dim3((unsigned)(A.H * A.s.n_seq)), dim3(SN), args, held ? (size_t)most * 4 : 0, s);
     if (e != hipSuccess) return e;
-    return hipLaunchKernel((const void *)k_fp4_move, dim3((unsigned)(A.H * A.s.n_seq), (unsigned)(2 * A.NC)), dim3(MN), args, 0, s);
+    // Many sequences and KV heads: blocks of 256 threads with four planes and 1024 places a round. Few, with more
+    // places: blocks of 1024 threads with one plane and 8192 places.
+    const long long groups = (long long)A.H * A.s.n_seq * 2 * A.NC;
+    return groups < 256 && A.keep > 1024 ? launch_move<1024, 1, 8>(A, s) : launch_move<256, 4, 4>(A, s);
 }
