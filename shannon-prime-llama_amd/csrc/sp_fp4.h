@@ -48,7 +48,7 @@ struct SpFp4Weigh {
     long long q_stride;
     int H, G;
     int window;
-    float c;  // |kq_scale| / 2
+    float c;  // |kq_scale| * log2(e) / 2
     int negate;
     int cus;
 };

@@ -24,25 +24,65 @@ __device__ __forceinline__ float power(unsigned rel, int b) {
 // eight consecutive blocks of a sequence. Columns (row, query head) pass by in stages: the block of
 // threads brings them into LDS as operands, and each wave takes them 16 at a time. The weights are
 // summed over columns in the registers that the scores come in, and over the 16 lanes at the end.
+//
+// Queries of 16-bit types are operands as they are, with K in their type: no maximum to look for, no
+// conversion. K counts relative to the block's largest exponent, for bf16 2^-12 of that, so that no
+// sum of finite queries passes a float. fp32 queries are scaled by a power of two and split in two
+// fp16 parts, as in attention.
 constexpr int WN = 512;  // threads
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
-template <int HD, int DT>
-__global__ __launch_bounds__(WN) void k_fp4_weigh(SpFp4Weigh A, int items) {
+// Four or sixteen bytes a lane from memory to LDS: lane l's to the l-th place from `to`. The wave waits for
+// them as for loads.
+typedef __attribute__((address_space(1))) void Global;
+typedef __attribute__((address_space(3))) void Shared;
+__device__ __forceinline__ void to_lds16(const void *from, void *to) { __builtin_amdgcn_global_load_lds((Global *)from, (Shared *)to, 16, 0, 0); }
+__device__ __forceinline__ void to_lds4(const void *from, void *to) { __builtin_amdgcn_global_load_lds((Global *)from, (Shared *)to, 4, 0, 0); }
+
+template <int DT>
+struct Operand {
+    typedef h8 V;
+    static constexpr int DOWN = 0;
+    static __device__ __forceinline__ V codes(unsigned w, float scale) { return eight(w, scale); }
+    static __device__ __forceinline__ f4 mma(V a, V b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Operand<SP_DTYPE_BF16> {
+    typedef b8 V;
+    static constexpr int DOWN = 12;
+    static __device__ __forceinline__ V codes(unsigned w, float scale) {
+        const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1),
+                   c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
+        return b8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+    static __device__ __forceinline__ f4 mma(V a, V b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// DIRECT (16-bit rows at multiples of 16 bytes): a stage's pieces go from memory to LDS past the registers,
+// a wave's 16 bytes a lane as one operand, while the stage before is worked on.
+template <int HD, int DT, bool DIRECT>
+__global__ __launch_bounds__(WN, HD == 256 || (HD == 128 && !DIRECT) ? 2 : 4) void k_fp4_weigh(SpFp4Weigh A, int items) {
+    typedef Operand<DT> Op;
+    typedef typename Op::V V;
     constexpr int NC = HD / 32, NW = WN / 64;
     constexpr int LP = HD == 64 ? 8 : HD == 256 ? 32 : 16;  // threads of a column (96: twelve of them have a part)
-    constexpr int CS = WN / LP, CG = CS / 16;               // columns of a stage, groups of 16
     constexpr bool SPLIT2 = DT == SP_DTYPE_F32;
     constexpr int NH = SPLIT2 ? 2 : 1;
+    constexpr int PER = HD == 64 || DIRECT ? 2 : 1;                          // columns of a thread in a stage
+    constexpr int CS = DIRECT ? (HD == 256 ? 64 : 128) : PER * WN / LP;      // columns of a stage
+    constexpr int BUF = CS / 16 * NC * NH * 64;                              // eights of a stage
     typedef typename SpFp8Elem<DT>::T T;
+    typedef T T8 __attribute__((ext_vector_type(8)));
     struct Column {
         float lse;  // +inf: adds nothing
         int qe;     // scores count in 2^(qe + the block's exponent) * A.c
-        int pos, from;
     };
-    __shared__ __align__(16) h8 qs[2][CG * NC * NH * 64];
-    __shared__ Column col_of[2][CS];
+    __shared__ __align__(16) V qs[(DIRECT ? 2 : 1) * BUF];
+    __shared__ Column col_of[DIRECT ? 1 : CS];
+    __shared__ float lse_of[DIRECT ? 2 * CS : 1];
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int h = blockIdx.y, r = lane & 15, g = lane >> 4;
+    const bool aligned = (uintptr_t)A.q % sizeof(T8) == 0 && A.q_stride % 8 == 0;
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
         // ---- the sequence, and eight blocks of those that its rows see ----
         int seq = -1, r0 = 0, n_new = 0, first = 0, j0 = 0, left = item;
@@ -71,10 +111,93 @@ __global__ __launch_bounds__(WN) void k_fp4_weigh(SpFp4Weigh A, int items) {
         const int t = j0 + w, n_cols = n_new * A.G;
         const int blk = uniform(t <= (first + n_new - 1) >> 6 ? sp_fp8_block(A.s, seq, t) : -1);
         const long long tile = (long long)max(blk, 0) * A.H + h;
-        // ---- K of this wave's block ----
-        u4 kr[NC];
-        unsigned ks[NC];
+        // ---- columns: this thread's eight entries of some, into LDS ----
+        const auto direct = [&](int c0, int buf) __attribute__((always_inline)) {
+            const int here = min(n_cols - c0, CS);
+            for (int f = w; f < (here + 15) / 16 * NC; f += NW) {  // fragments: 16 columns, 32 channels
+                const int n = c0 + min(f / NC * 16 + r, here - 1);
+                const T *src = reinterpret_cast<const T *>(A.q) + (long long)(r0 + n / A.G) * A.q_stride +
+                               (long long)(h * A.G + n % A.G) * HD + f % NC * 32 + g * 8;
+                to_lds16(src, qs + buf * BUF + f * 64);
+            }
+            for (int c = w * 64; c < here; c += WN) {
+                const int n = c0 + min(c + lane, here - 1);
+                to_lds4(A.lse + (long long)(r0 + n / A.G) * A.H * A.G + h * A.G + n % A.G, lse_of + buf * CS + c);
+            }
+        };
+        const int mine = tid / LP, part = tid % LP;
+        const auto stage = [&](int c0) __attribute__((always_inline)) {
+            T8 raw[PER];
+            float lse[PER];
+#pragma unroll
+            for (int y = 0; y < PER; y++) {
+                const int n = c0 + y * (WN / LP) + mine;
+                raw[y] = T8{};
+                lse[y] = INFINITY;
+                if (n >= n_cols) continue;
+                const int row = r0 + n / A.G, head = h * A.G + n % A.G;
+                lse[y] = A.lse[(long long)row * A.H * A.G + head];
+                if (part >= HD / 8) continue;
+                const T *src = reinterpret_cast<const T *>(A.q) + (long long)row * A.q_stride + (long long)head * HD + part * 8;
+                if (aligned) {
+                    raw[y] = *reinterpret_cast<const T8 *>(src);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) raw[y][k] = src[k];
+                }
+            }
+#pragma unroll
+            for (int y = 0; y < PER; y++) {
+                if (c0 + y * (WN / LP) >= n_cols) break;
+                const int c = y * (WN / LP) + mine;
+                // not: rows that see nothing, and those whose scores are no numbers
+                bool finite = true;
+#pragma unroll
+                for (int k = 0; k < 8; k++) finite = finite && fabsf(SpFp8Elem<DT>::get(raw[y][k])) < INFINITY;
+                const unsigned long long odd = __ballot(!finite) >> (lane & ~(LP - 1));
+                const bool active = fabsf(lse[y]) < INFINITY && (odd & ((1ull << LP) - 1)) == 0;
+                V q[NH];
+                int qe = 1;
+                if constexpr (!SPLIT2) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) q[0][k] = active ? raw[y][k] : (T)0.0f;
+                } else {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) top = fmaxf(top, fabsf(raw[y][k]));
+#pragma unroll
+                    for (int s = LP / 2; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+                    int e = (__float_as_int(top) >> 23) - 127 - 14;
+                    e = top == 0.0f || !active ? 0 : max(e, -126);
+                    const float down = sp_fp8_pow2(-e);
+                    qe = e + 1;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const float v = active ? raw[y][k] * down : 0.0f;
+                        const _Float16 hi = (_Float16)v;
+                        q[0][k] = hi;
+                        q[NH - 1][k] = (_Float16)(v - (float)hi);
+                    }
+                }
+                if (part < HD / 8) {
+                    V *d = qs + ((c >> 4) * NC + (part >> 2)) * NH * 64 + (part & 3) * 16 + (c & 15);
+#pragma unroll
+                    for (int k = 0; k < NH; k++) d[k * 64] = q[k];
+                }
+                if (part == 0) {
+                    Column to;
+                    to.lse = active ? lse[y] : INFINITY;
+                    to.qe = qe;
+                    col_of[c] = to;
+                }
+            }
+        };
+        // ---- K of this wave's block, relative to its largest exponent, as in attention ----
+        int top;
+        V ka[NC][4];
         {
+            u4 kr[NC];
+            unsigned ks[NC];
             const uint8_t *p = A.k.codes + tile * sp_fp4_tile(HD) + g * 256 + (4 * (r & 3) + (r >> 2)) * 16;
             const uint8_t *e = A.k.exps + tile * sp_fp4_exps(HD) + r * 4;
 #pragma unroll
@@ -82,84 +205,55 @@ __global__ __launch_bounds__(WN) void k_fp4_weigh(SpFp4Weigh A, int items) {
                 kr[c] = *reinterpret_cast<const u4 *>(p + c * 1024);
                 ks[c] = *reinterpret_cast<const unsigned *>(e + c * 64);
             }
+            if constexpr (DIRECT) direct(0, 0);
+            else stage(0);
+            Largest m;
+#pragma unroll
+            for (int c = 0; c < NC; c++) m.add(ks[c]);
+            top = uniform(sp_fp4::row_max(m.get()));
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const unsigned rel = relative(ks[c], top + Op::DOWN);
+#pragma unroll
+                for (int n = 0; n < 4; n++) ka[c][n] = Op::codes(kr[c][n], power(rel, n));
+            }
         }
-        // ---- columns: this thread's eight entries of one ----
-        const int mine = tid / LP, part = tid % LP;
-        float x[8];
-        const auto load = [&](int c0) __attribute__((always_inline)) {
-            const int n = c0 + mine;
-#pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = 0.0f;
-            if (n < n_cols && part < HD / 8) {
-                const bool aligned = (uintptr_t)A.q % (4 * sizeof(T)) == 0 && A.q_stride % 4 == 0;
-                load8<DT>(reinterpret_cast<const T *>(A.q) + (long long)(r0 + n / A.G) * A.q_stride +
-                              (long long)(h * A.G + n % A.G) * HD + part * 8, aligned, x);
-            }
-        };
-        const auto put = [&](int c0, int to) __attribute__((always_inline)) {
-            const int n = c0 + mine, tk = n / A.G;
-            float top = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; k++) top = x[k] != x[k] ? INFINITY : fmaxf(top, fabsf(x[k]));
-#pragma unroll
-            for (int s = LP / 2; s; s >>= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
-            float lse = INFINITY;
-            if (n < n_cols) lse = A.lse[(long long)(r0 + tk) * A.H * A.G + h * A.G + n % A.G];
-            // rows that see nothing, and those whose scores are no numbers
-            const bool active = n < n_cols && fabsf(lse) < INFINITY && top < INFINITY;
-            int e = (__float_as_int(top) >> 23) - 127 - 14;
-            e = top == 0.0f || !active ? 0 : max(e, -126);
-            const float down = A.negate ? -sp_fp8_pow2(-e) : sp_fp8_pow2(-e);
-            h8 q[NH];
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const float v = active ? x[k] * down : 0.0f;
-                const _Float16 hi = (_Float16)v;
-                q[0][k] = hi;
-                if (SPLIT2) q[NH - 1][k] = (_Float16)(v - (float)hi);
-            }
-            if (part < HD / 8) {
-                h8 *d = qs[to] + ((mine >> 4) * NC + (part >> 2)) * NH * 64 + (part & 3) * 16 + (mine & 15);
-#pragma unroll
-                for (int k = 0; k < NH; k++) d[k * 64] = q[k];
-            }
-            if (part == 0) {
-                Column c;
-                c.lse = active ? lse : INFINITY;
-                c.qe = e + 1;
-                c.pos = active ? first + tk : -1;
-                c.from = A.window > 0 ? c.pos - A.window : -1;
-                col_of[to][mine] = c;
-            }
-        };
-        load(0);
-        // relative to the block's largest exponent, as in attention
-        Largest m;
-#pragma unroll
-        for (int c = 0; c < NC; c++) m.add(ks[c]);
-        const int top = uniform(sp_fp4::row_max(m.get()));
-#pragma unroll
-        for (int c = 0; c < NC; c++) ks[c] = relative(ks[c], top);
-        h8 ka[NC][4];
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int n = 0; n < 4; n++) ka[c][n] = eight(kr[c][n], power(ks[c], n));
         f4 acc[4];
 #pragma unroll
         for (int n = 0; n < 4; n++) acc[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        int at = 0;
-        for (int c0 = 0; c0 < n_cols; c0 += CS, at ^= 1) {
-            put(c0, at);
-            lds_barrier();  // (two places: a stage is written after all have read the one before the last)
-            if (c0 + CS < n_cols) load(c0 + CS);
+        // whether every column sees all of this block: nothing then depends on a column's position
+        const bool all = t * 64 + 63 <= first && (A.window <= 0 || t * 64 > first + n_new - 1 - A.window);
+        const auto units = [&](int qe) {  // of the scores, times log2 e
+            const float up = fminf(__builtin_amdgcn_ldexpf(A.c, qe + top + Op::DOWN - 127), 0x1.fffffep127f);
+            return A.negate ? -up : up;
+        };
+        const float cs1 = units(1);
+        int buf = 0;
+        for (int c0 = 0; c0 < n_cols; c0 += CS) {
+            if constexpr (DIRECT) {
+                // this stage is there, and all have read the one that the next goes over
+                __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                lds_barrier();
+                buf = c0 / CS & 1;
+                if (c0 + CS < n_cols) direct(c0 + CS, buf ^ 1);
+            } else {
+                if (c0) {
+                    lds_barrier();  // all have read the stage before
+                    stage(c0);
+                }
+                lds_barrier();
+            }
             if (blk < 0) continue;
-            for (int y = 0; y < CG && c0 + y * 16 < n_cols; y++) {
-                const int n0 = c0 + y * 16, n1 = min(n0 + 15, n_cols - 1);
-                const int pos0 = first + n0 / A.G, pos1 = first + n1 / A.G;
-                if (t * 64 > pos1 || (A.window > 0 && t * 64 + 63 <= pos0 - A.window)) continue;
-                const Column col = col_of[at][y * 16 + r];
-                const h8 *qy = qs[at] + y * NC * NH * 64 + lane;
+#pragma unroll 1
+            for (int y = 0; y < CS / 16 && c0 + y * 16 < n_cols; y++) {
+                const int n0 = c0 + y * 16;
+                bool open = all;
+                if (!all) {
+                    const int pos0 = first + n0 / A.G, pos1 = first + min(n0 + 15, n_cols - 1) / A.G;
+                    if (t * 64 > pos1 || (A.window > 0 && t * 64 + 63 <= pos0 - A.window)) continue;
+                    open = t * 64 + 63 <= pos0 && (A.window <= 0 || t * 64 > pos1 - A.window);
+                }
+                const V *qy = qs + buf * BUF + y * NC * NH * 64 + lane;
                 f4 s[4];
 #pragma unroll
                 for (int n = 0; n < 4; n++) s[n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -167,22 +261,45 @@ __global__ __launch_bounds__(WN) void k_fp4_weigh(SpFp4Weigh A, int items) {
                 for (int c = 0; c < NC; c++)
 #pragma unroll
                     for (int k = 0; k < NH; k++) {
-                        const h8 q = qy[(c * NH + k) * 64];
+                        const V q = qy[(c * NH + k) * 64];
 #pragma unroll
-                        for (int n = 0; n < 4; n++) s[n] = mma(ka[c][n], q, s[n]);
+                        for (int n = 0; n < 4; n++) s[n] = Op::mma(ka[c][n], q, s[n]);
                     }
-                const float cs = fminf(__builtin_amdgcn_ldexpf(A.c, col.qe + top - 127), 0x1.fffffep127f);
-                const bool open = t * 64 + 63 <= pos0 && (A.window <= 0 || t * 64 > pos1 - A.window);
-                const int lane0 = t * 64 + 4 * g, upto = col.pos - lane0, before = col.from - lane0;
+                float lse, cs = cs1;
+                if constexpr (DIRECT) {
+                    lse = lse_of[buf * CS + y * 16 + r];
+                    lse = n0 + r < n_cols && fabsf(lse) < INFINITY ? lse : INFINITY;
+                    // a query that is not finite has no finite score: one of them tells (finite ones have: see above)
+                    const bool odd = !(fabsf(s[0][0]) < INFINITY);
+                    if (__any(odd)) {
+                        lse = odd ? INFINITY : lse;
+#pragma unroll
+                        for (int n = 0; n < 4; n++) s[n] = odd ? f4{0.0f, 0.0f, 0.0f, 0.0f} : s[n];
+                    }
+                } else {
+                    const Column col = col_of[y * 16 + r];
+                    lse = col.lse;
+                    cs = units(col.qe);
+                }
+                // (log2 e and lse are multiplied first: what that rounds off is less than lse's own last bit)
+                lse *= 1.44269504088896341f;
 #pragma unroll
                 for (int n = 0; n < 4; n++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        // the score less lse, rounded once
-                        float d = __builtin_fmaf(s[n][i], cs, -col.lse);
-                        if (!open) d = 16 * i + n <= upto && 16 * i + n > before ? d : -INFINITY;
-                        acc[n][i] += __builtin_amdgcn_exp2f(d * 1.44269504088896341f);
-                    }
+                    for (int i = 0; i < 4; i++) s[n][i] = __builtin_fmaf(s[n][i], cs, -lse);
+                if (__builtin_expect(!open, 0)) {
+                    const int pos = first + (n0 + r) / A.G, lane0 = t * 64 + 4 * g;
+                    const int upto = pos - lane0, before = (A.window > 0 ? pos - A.window : -1) - lane0;
+#pragma unroll
+                    for (int n = 0; n < 4; n++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) s[n][i] = 16 * i + n <= upto && 16 * i + n > before ? s[n][i] : -INFINITY;
+                    __asm__ volatile("" ::: "memory");  // (a branch: else the comparisons are made for every block)
+                }
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[n][i] += __builtin_amdgcn_exp2f(s[n][i]);
             }
         }
         lds_barrier();  // the next item's first stage
@@ -214,9 +331,10 @@ hipError_t launch_weigh(const SpFp4Weigh &A, int dtype, hipStream_t s) {
     const long long most = (long long)A.s.n_seq * ((A.s.stride + 7) / 8);
     int items = (int)(most < (1ll << 30) ? most : 1ll << 30);
     const int wide = (4 * A.cus + A.H - 1) / A.H;
-    const void *f = dtype == SP_DTYPE_F32 ? (const void *)k_fp4_weigh<HD, SP_DTYPE_F32>
-                  : dtype == SP_DTYPE_F16 ? (const void *)k_fp4_weigh<HD, SP_DTYPE_F16>
-                                          : (const void *)k_fp4_weigh<HD, SP_DTYPE_BF16>;
+    const bool direct = dtype != SP_DTYPE_F32 && (uintptr_t)A.q % 16 == 0 && A.q_stride % 8 == 0;
+    const void *f = dtype == SP_DTYPE_F32 ? (const void *)k_fp4_weigh<HD, SP_DTYPE_F32, false>
+                  : dtype == SP_DTYPE_F16 ? (direct ? (const void *)k_fp4_weigh<HD, SP_DTYPE_F16, true> : (const void *)k_fp4_weigh<HD, SP_DTYPE_F16, false>)
+                                          : (direct ? (const void *)k_fp4_weigh<HD, SP_DTYPE_BF16, true> : (const void *)k_fp4_weigh<HD, SP_DTYPE_BF16, false>);
     void *args[] = {const_cast<SpFp4Weigh *>(&A), &items};
     return hipLaunchKernel(f, dim3((unsigned)(items < wide ? items : wide), (unsigned)A.H), dim3(WN), args, 0, s);
 }

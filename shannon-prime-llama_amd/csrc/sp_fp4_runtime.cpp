@@ -141,7 +141,7 @@ extern "C" int sp_hip_fp4_weigh(sp_hip_fp4_cache_t *c, int layer, const sp_hip_f
     A.H = c->config.n_heads_kv;
     A.G = n_q / A.H;
     A.window = window >= MAX_ROWS ? 0 : window;  // no position is that far
-    A.c = fabsf(kq_scale) * 0.5f;
+    A.c = fabsf(kq_scale) * 0.72134752044448170f;
     A.negate = kq_scale < 0.0f;
     A.cus = pv->cus;
     return ok(sp_fp4_launch_weigh(A, c->config.head_dim, dtype, s), who) ? 0 : -1;
