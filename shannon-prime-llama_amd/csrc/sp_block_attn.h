@@ -783,6 +783,8 @@ __global__ __launch_bounds__(NW * 64) void k_attn_wide(SpFp8Attn A) {
     float cs = 0.0f, shift = 0.0f, lmul = 1.0f;
     h8 p[NP][NH];
 
+    const h8 *const kl = kbuf + Blocks::at(lane);
+    const h8 *const vl = vbuf + Blocks::v_at(lane);
     // out^T += V^T p^T for one of the NP steps
     const auto product = [&](auto step, const h8 *vd) __attribute__((always_inline)) {
         constexpr int t = decltype(step)::value;
@@ -791,7 +793,7 @@ __global__ __launch_bounds__(NW * 64) void k_attn_wide(SpFp8Attn A) {
         for (int d0 = 0; d0 < ND; d0 += AT_ONCE) {
             h8 a[AT_ONCE];
 #pragma unroll
-            for (int d = 0; d < AT_ONCE; d++) a[d] = vd[(d0 + d) * Blocks::V_ROW + t * 64];
+            for (int d = 0; d < AT_ONCE; d++) a[d] = vd[(d0 + d) * Blocks::V_ROW + t * Blocks::V_STEP];
 #pragma unroll
             for (int d = 0; d < AT_ONCE; d++)
 #pragma unroll
@@ -908,7 +910,6 @@ __global__ __launch_bounds__(NW * 64) void k_attn_wide(SpFp8Attn A) {
 
     // ---- block 0's scores; K one block ahead of V from here ----
     // Blocks past the last are fetched as block 0 and never used: no turn asks for its place.
-    const h8 *const kl = kbuf + Blocks::at(lane), *const vl = vbuf + Blocks::at(lane);
     V sa[RB], sb[RB];
     if (n > 0) {
         stage(0, 0, stage_v ? f0.ev : f0.ek);

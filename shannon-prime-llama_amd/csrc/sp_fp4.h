@@ -116,8 +116,8 @@ __device__ __forceinline__ int row_max(int v) {
 // And of a wave, in a scalar register.
 __device__ __forceinline__ int wave_max(int v) {
     v = row_max(v);
-    return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
-               max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+    return __builtin_amdgcn_readfirstlane(max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+                                              max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48))));
 }
 
 }  // namespace sp_fp4

@@ -15,9 +15,15 @@ using sp_fp4::eight;
 using sp_fp4::Largest;
 using sp_fp4::relative;
 
-// The float with exponent byte b of `rel` (b known where this is expanded).
-__device__ __forceinline__ float power(unsigned rel, int b) {
-    return __int_as_float((b == 3 ? rel >> 1 : rel << (23 - 8 * b)) & 0x7f800000);
+// The float with exponent byte b of e (b known where this is expanded): the byte, moved, in one instruction.
+__device__ __forceinline__ float byte_power(unsigned e, int b) {
+    float r;
+    const int by = 23;
+    if (b == 0) __asm__("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_0" : "=v"(r) : "v"(by), "v"(e));
+    else if (b == 1) __asm__("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_1" : "=v"(r) : "v"(by), "v"(e));
+    else if (b == 2) __asm__("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_2" : "=v"(r) : "v"(by), "v"(e));
+    else __asm__("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:BYTE_3" : "=v"(r) : "v"(by), "v"(e));
+    return r;
 }
 // Two codes: byte b of w.
 __device__ __forceinline__ h2 two(unsigned w, float scale, int b) {
@@ -87,8 +93,8 @@ struct Fp4 {
         }
         // row blocks 2 u and 2 u + 1 of step c
         __device__ __forceinline__ void k_rows(int c, int u, h8 &a, h8 &b) const {
-            a = eight(kr[c][2 * u], power(ks[c], 2 * u));
-            b = eight(kr[c][2 * u + 1], power(ks[c], 2 * u + 1));
+            a = eight(kr[c][2 * u], byte_power(ks[c], 2 * u));
+            b = eight(kr[c][2 * u + 1], byte_power(ks[c], 2 * u + 1));
         }
         // channels d and d + 1: one byte of each of the lane's sixteen positions, turned
         __device__ __forceinline__ void v_rows(int d, h8 (&a)[AT_ONCE][2]) const {
@@ -97,7 +103,7 @@ struct Fp4 {
             for (int s = 0; s < 2; s++) {
                 h2 c[8];
 #pragma unroll
-                for (int k = 0; k < 8; k++) c[k] = two(vr[x][2 * s + k / 4][k % 4], power(vs[x][2 * s + k / 4], k % 4), byte);
+                for (int k = 0; k < 8; k++) c[k] = two(vr[x][2 * s + k / 4][k % 4], byte_power(vs[x][2 * s + k / 4], k % 4), byte);
 #pragma unroll
                 for (int o = 0; o < 2; o++)
                     a[o][s] = h8{c[0][o], c[1][o], c[2][o], c[3][o], c[4][o], c[5][o], c[6][o], c[7][o]};
@@ -120,56 +126,60 @@ struct Fp4 {
         }
     };
 
-    // A block on its way into LDS: half of the threads bring K, half V.
-    // A piece of K is a quad of a plane: one operand row of eight channels for each of its positions.
-    // A piece of V is half of a plane's channels for the eight positions that a lane of the product has
-    // in one step: four operand rows. Rows are put where the eight lanes that write at once, and
-    // the lanes that read, meet no bank twice: at CW 32 the low two bits of a row's place are
-    // turned by the next two but one, at CW 16 the lowest by the fourth, and row blocks lie two
-    // places further apart.
+    // A block on its way into LDS: half of the threads bring K, half V, in pieces of a quad of a plane. Of K
+    // that is an operand row of eight channels for each of four positions (16 bytes each); of V, half of an operand
+    // row of eight positions for each of eight channels (8 bytes each). Rows are put where the lanes
+    // that write at once meet no bank twice, nor those that read (of a read of 16 bytes a lane these are lanes 0 to 3,
+    // 12 to 15, 20 to 23 and 24 to 27 of each 32, and the others): of K a row's place is turned by other bits of
+    // it, of V steps, upper lanes and row blocks lie apart by what keeps them in different banks.
     template <int HD, int NT, int CW>
     struct Wide {
         static constexpr int HT = NT / 2, NW = NT / 64;
         static constexpr int NS = CW == 32 ? HD / 16 : HD / 32, NP = CW == 32 ? 4 : 2, PAD = CW == 32 ? 0 : 2;
         static constexpr int PIECES = 2 * HD, PER = (PIECES + HT - 1) / HT;
-        // fp16 eights: of a block's place in LDS, and of a row block of it
+        // fp16 eights: of a block's place in LDS, of a row block of it, of a step of V
         static constexpr int K_ROW = NS * 64 + PAD, K_PLACE = 64 / CW * K_ROW;
-        static constexpr int V_ROW = NP * 64 + PAD, V_PLACE = HD / CW * V_ROW;
+        static constexpr int V_STEP = CW == 32 ? 66 : 73, V_ROW = CW == 32 ? 264 : 148, V_PLACE = HD / CW * V_ROW;
         static constexpr int LDS = 2 * (K_PLACE + V_PLACE) * 16, BYTES = LDS + 64 * 4;
         static_assert(64 % NW == 0);
         struct Raw {
-            u4 x[2 * PER];
-            unsigned e[2 * PER];
+            u4 x[PER];
+            unsigned e[PER];
         };
+        // place of lane `lane` of an operand of K, and of one of V
         static constexpr __device__ __forceinline__ int at(int lane) { return lane ^ ((lane >> 3) & (CW == 32 ? 3 : 1)); }
+        static constexpr __device__ __forceinline__ int v_at(int lane) { return lane + (lane >> 5) * (CW == 32 ? 1 : 2); }
         static __device__ __forceinline__ bool mine(int x) { return PER * HT == PIECES || x < PIECES; }
         // The largest exponents of the 64 blocks that the lanes have: each wave finds those of its share
         // of them, coalesced, and all meet in LDS.
         static __device__ __forceinline__ void look_up(const SpFp8Attn &A, int h, int blk, int w, int lane, int *area, int &ekb,
                                                        int &evb) {
-            constexpr int EACH = 64 / NW, DW = sp_fp4_exps(HD) / 4, TWICE = DW > 64 ? 2 : 1;
-            unsigned ke[EACH][TWICE], ve[EACH][TWICE];
+            constexpr int EACH = 64 / NW, DW = sp_fp4_exps(HD) / 4, TWICE = DW > 64 ? 2 : 1, SOME = EACH / TWICE;
+#pragma unroll 1
+            for (int i0 = 0; i0 < EACH; i0 += SOME) {  // (as many loads together as the loop's registers leave room for)
+                unsigned ke[SOME][TWICE], ve[SOME][TWICE];
 #pragma unroll
-            for (int i = 0; i < EACH; i++) {
-                const int b = max(__builtin_amdgcn_readlane(blk, w * EACH + i), 0);
-                const long long tile = ((long long)b * A.H + h) * DW;
+                for (int i = 0; i < SOME; i++) {
+                    const int b = max(__builtin_amdgcn_readlane(blk, w * EACH + i0 + i), 0);
+                    const long long tile = ((long long)b * A.H + h) * DW;
 #pragma unroll
-                for (int t = 0; t < TWICE; t++) {
-                    const int x = min(lane + t * 64, DW - 1);
-                    ke[i][t] = reinterpret_cast<const unsigned *>(A.k.exps)[tile + x];
-                    ve[i][t] = reinterpret_cast<const unsigned *>(A.v.exps)[tile + x];
+                    for (int t = 0; t < TWICE; t++) {
+                        const int x = min(lane + t * 64, DW - 1);
+                        ke[i][t] = reinterpret_cast<const unsigned *>(A.k.exps)[tile + x];
+                        ve[i][t] = reinterpret_cast<const unsigned *>(A.v.exps)[tile + x];
+                    }
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < EACH; i++) {
-                Largest k, v;
+                for (int i = 0; i < SOME; i++) {
+                    Largest k, v;
 #pragma unroll
-                for (int t = 0; t < TWICE; t++) {
-                    k.add(ke[i][t]);
-                    v.add(ve[i][t]);
+                    for (int t = 0; t < TWICE; t++) {
+                        k.add(ke[i][t]);
+                        v.add(ve[i][t]);
+                    }
+                    const int both = sp_fp4::wave_max(k.get()) | sp_fp4::wave_max(v.get()) << 8;
+                    if (lane == 0) area[w * EACH + i0 + i] = both;
                 }
-                const int both = sp_fp4::wave_max(k.get()) | sp_fp4::wave_max(v.get()) << 8;
-                if (lane == 0) area[w * EACH + i] = both;
             }
             lds_barrier();
             ekb = area[lane] & 255;
@@ -185,24 +195,36 @@ struct Fp4 {
                 raw.e[i] = *reinterpret_cast<const unsigned *>(e + (x >> 6) * 64 + (q & 3) * 16 + (q >> 2) * 4);
             }
         }
-        // x = (plane / 4, step, lane group, plane % 4, half): its first quad (the second is HOP further)
-        static constexpr int HOP = CW == 32 ? 2 : 4;
-        static __device__ __forceinline__ int quad(int x) {
-            const int y = (x >> 3) & 7;
-            return CW == 32 ? (y >> 1) * 4 + (y & 1) : (y >> 2) * 8 + (y & 3);
+        // A V piece: its plane and quad; which step of the product, group of lanes and half of an eight that quad is.
+        struct Piece {
+            int n, quad, step, sub, half;
+        };
+        static __device__ __forceinline__ Piece piece(int x) {
+            Piece p;
+            if (CW == 32) {  // x = (plane, quad)
+                p.n = x >> 4;
+                p.quad = x & 15;
+                p.step = p.quad >> 2;
+                p.half = p.quad >> 1 & 1;
+                p.sub = p.quad & 1;
+            } else {  // x = (plane / 4, sub % 2, plane % 2, plane / 2 % 2, sub / 2, step, half)
+                p.n = (x >> 6) * 4 + (x >> 3 & 1) * 2 + (x >> 4 & 1);
+                p.half = x & 1;
+                p.step = x >> 1 & 1;
+                p.sub = (x >> 2 & 1) * 2 + (x >> 5 & 1);
+                p.quad = p.step * 8 + p.half * 4 + p.sub;
+            }
+            return p;
         }
         static __device__ __forceinline__ void fetch_v(const SpFp8Side &S, long long tile, int st, Raw &raw) {
             const uint8_t *p = S.codes + tile * sp_fp4_tile(HD), *e = S.exps + tile * sp_fp4_exps(HD);
 #pragma unroll
             for (int i = 0; i < PER; i++) {
-                const int x = st + i * HT, q = quad(x), n = (x >> 6) * 4 + ((x >> 1) & 3);
+                const int x = st + i * HT;
                 if (!mine(x)) continue;
-#pragma unroll
-                for (int o = 0; o < 2; o++) {
-                    const int qo = q + o * HOP;
-                    raw.x[2 * i + o] = *reinterpret_cast<const u4 *>(p + n * 256 + qo * 16);
-                    raw.e[2 * i + o] = *reinterpret_cast<const unsigned *>(e + (x >> 6) * 64 + (qo & 3) * 16 + (qo >> 2) * 4);
-                }
+                const Piece v = piece(x);
+                raw.x[i] = *reinterpret_cast<const u4 *>(p + v.n * 256 + v.quad * 16);
+                raw.e[i] = *reinterpret_cast<const unsigned *>(e + (v.n >> 2) * 64 + (v.quad & 3) * 16 + (v.quad >> 2) * 4);
             }
         }
         static __device__ __forceinline__ void stage_k(Raw &raw, int st, int top, h8 *to) {
@@ -215,29 +237,29 @@ struct Fp4 {
                 const int lane = CW == 32 ? (n & 1) * 32 + 4 * (q & 7) : (n & 3) * 16 + 4 * (q & 3);
                 h8 *d = to + (CW == 32 ? (q >> 3) * K_ROW + (n >> 1) * 64 : (q >> 2) * K_ROW + (n >> 2) * 64);
 #pragma unroll
-                for (int b = 0; b < 4; b++) d[at(lane + b)] = eight(raw.x[i][b], power(rel, b));
+                for (int b = 0; b < 4; b++) d[at(lane + b)] = eight(raw.x[i][b], byte_power(rel, b));
             }
         }
         static __device__ __forceinline__ void stage_v(Raw &raw, int st, int top, h8 *to) {
+            typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 #pragma unroll
             for (int i = 0; i < PER; i++) {
-                const int x = st + i * HT, y = (x >> 3) & 7, n = (x >> 6) * 4 + ((x >> 1) & 3), half = x & 1;
+                const int x = st + i * HT;
                 if (!mine(x)) continue;
-                h2 c[2][8];
+                const Piece v = piece(x);
+                const unsigned rel = relative(raw.e[i], top + 127);
+                float scale[4];
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const unsigned w = raw.x[2 * i + k / 4][k % 4] >> (16 * half);
-                    const float scale = power(relative(raw.e[2 * i + k / 4], top + 127), k % 4);
-                    c[0][k] = two(w, scale, 0);
-                    c[1][k] = two(w, scale, 1);
-                }
-                const int lane = CW == 32 ? (y & 1) * 32 + 8 * (n & 3) + 4 * half : (y & 3) * 16 + 8 * (n & 1) + 4 * half;
-                h8 *d = to + (CW == 32 ? (n >> 2) * V_ROW + (y >> 1) * 64 : (n >> 1) * V_ROW + (y >> 2) * 64);
+                for (int b = 0; b < 4; b++) scale[b] = byte_power(rel, b);
+                const int lane = v.sub * CW + v.n * 8 % CW;  // of its first channel
+                h4 *d = reinterpret_cast<h4 *>(to + v.n * 8 / CW * V_ROW + v.step * V_STEP + v_at(lane)) + v.half;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const h2 *a = c[j / 2];
-                    const int o = j % 2;
-                    d[at(lane + j)] = h8{a[0][o], a[1][o], a[2][o], a[3][o], a[4][o], a[5][o], a[6][o], a[7][o]};
+                for (int byte = 0; byte < 4; byte++) {
+                    h2 c[4];
+#pragma unroll
+                    for (int b = 0; b < 4; b++) c[b] = two(raw.x[i][b], scale[b], byte);
+#pragma unroll
+                    for (int o = 0; o < 2; o++) d[2 * (2 * byte + o)] = h4{c[0][o], c[1][o], c[2][o], c[3][o]};
                 }
             }
         }

@@ -67,13 +67,14 @@ struct Fp8 {
         static constexpr int NS = CW == 32 ? HD / 16 : HD / 32, NP = CW == 32 ? 4 : 2;
         static constexpr int KP = (HD * 4 + HT - 1) / HT;  // K pieces of 16 codes a thread (half the threads)
         static constexpr int VP = (HD * 2 + HT - 1) / HT;  // pairs of V pieces (the other half)
-        // fp16 eights: of a block's place in LDS, and of a row block of it
-        static constexpr int K_PLACE = TILE / 8, V_PLACE = TILE / 8, K_ROW = NS * 64, V_ROW = NP * 64;
+        // fp16 eights: of a block's place in LDS, of a row block of it, of a step of V
+        static constexpr int K_PLACE = TILE / 8, V_PLACE = TILE / 8, K_ROW = NS * 64, V_ROW = NP * 64, V_STEP = 64;
         static constexpr int LDS = HD * 512, BYTES = LDS;
         struct Raw {
             u4 x[KP > 2 * VP ? KP : 2 * VP];
         };
         static constexpr __device__ __forceinline__ int at(int lane) { return lane; }
+        static constexpr __device__ __forceinline__ int v_at(int lane) { return lane; }
         static __device__ __forceinline__ void look_up(const SpFp8Attn &A, int h, int blk, int, int, int *, int &ekb, int &evb) {
             const long long at = (long long)max(blk, 0) * A.H + h;
             ekb = A.k.exps[at];
