@@ -1085,14 +1085,22 @@ __global__ __launch_bounds__(256) void k_attn_join(SpFp8Attn A) {
         A.lse[row * A.H * A.G + head] = L == 0.0f ? -INFINITY : (M + (__log2f(L) - WIDE_TOP<DT>)) * 0.69314718055994531f;
 }
 
+// No sequence's rows see more cache blocks than this, as far as the host knows.
+inline long long most_blocks(const SpFp8Attn &A) {
+    return A.window > 0 ? min((long long)A.s.stride, ((long long)A.s.n_rows + A.window + 126) / 64) : A.s.stride;
+}
+
+// Column groups of a few-row launch: each sequence's rows times G, in groups of cols.
+inline long long few_groups(const SpFp8Attn &A, int cols) {
+    return A.s.row ? ((long long)A.s.n_rows * A.G) / cols + A.s.n_seq : (long long)A.s.n_seq * ((A.G + cols - 1) / cols);
+}
+
 template <class F, int HD, int DT, int NW, int CG>
 hipError_t launch(const SpFp8Attn &A, hipStream_t s) {
     constexpr int COLS = 16 * CG;
     SpFp8Attn a = A;
     a.target = min(A.target, 256);
-    // column groups: each sequence's rows times G, in groups of COLS
-    const long long groups = A.s.row ? ((long long)A.s.n_rows * A.G) / COLS + A.s.n_seq
-                                     : (long long)A.s.n_seq * ((A.G + COLS - 1) / COLS);
+    const long long groups = few_groups(A, COLS);
     // shares: one per group, and at most target more over all KV heads
     const long long blocks = (groups + (a.target + A.H - 1) / A.H) * A.H;
     if (blocks * (NW * 64) > SP_FP8_MOST_THREADS) return hipErrorInvalidValue;
@@ -1114,12 +1122,11 @@ hipError_t launch_wide(const SpFp8Attn &A, hipStream_t s) {
     const long long groups = (long long)A.s.n_rows * A.G / COLS + A.s.n_seq;
     // With a block for each CU sharing gains nothing. Below that a group is shared out where the
     // others leave CUs idle, and a second launch joins the shares.
-    // (No sequence's rows see more than `most` cache blocks; up to 4 * LEAST are not shared out. Waves
+    // (Up to 4 * LEAST cache blocks are not shared out. Waves
     // of 16 columns take two blocks a share: 512 rows over 768 positions of one head of 256 20 us for 34;
     // of 32 they are the slower ones, 1024 rows from position 0 of 8 heads of 128 44 us for 40.)
     constexpr int LEAST = CW == 16 ? 2 : 4;
-    const long long most = A.window > 0 ? min((long long)A.s.stride, ((long long)A.s.n_rows + A.window + 126) / 64) : A.s.stride;
-    const bool share = groups * A.H < a.target && most > 4 * LEAST;
+    const bool share = groups * A.H < a.target && most_blocks(A) > 4 * LEAST;
     a.least = share ? LEAST : 1 << 28;
     a.join = 0.0f;
     const long long blocks = (groups + (share ? (a.target + A.H - 1) / A.H : 0)) * A.H;

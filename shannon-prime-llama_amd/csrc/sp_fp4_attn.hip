@@ -266,14 +266,30 @@ struct Fp4 {
     };
 };
 
+// Which kernel. All figures are of 8 KV heads, in us; rows are 16-bit and head_dim is 128 where not said.
+//   Many rows (MANY columns over all KV heads) go to the kernel that converts a block once, in LDS: 512 rows of 32 heads over
+//   2048 positions take it 40 and the few-row kernel 46, 256 rows 34 and 26; with float32 rows 256 take 36 and 40,
+//   128 28 and 23; at head_dim 256 256 take 45 and 59, 128 37 and 31. Behind a long cache the conversions outweigh that kernel's
+//   slower start and its second launch, and half as many columns suffice: 128 rows over 4096 / 8192 / 16000 positions take
+//   34 / 43 / 57 and 30 / 44 / 71, with float32 rows 36 / 50 / 78 and 33 / 54 / 100, at head_dim 256 45 / 60 / 93 and
+//   53 / 98 / 181 (3000 positions 41 and 43).
+//   Sequences of few rows each leave most of its columns idle (EACH): 32 sequences of 16 rows of 16 heads take 53 and 31,
+//   of 32 heads 54 and 54, 16 of 64 rows of 32 heads 69 and 99; float32 rows 52 and 46, 56 and 82, 74 and 156.
+//   Few rows: past a group for each CU half the waves a block leave a CU two blocks out of step. Decode at 4000
+//   positions of 32 / 40 / 64 sequences takes 41 / 56 / 59 with four waves and 33 / 58 / 64 with eight, at 600 positions
+//   12.7 / 16.6 / 17.1 and 12.5 / 19.5 / 21.4. With two column groups a wave eight stay ahead (64 sequences of 5 rows of
+//   32 heads 85, with four 116).
 template <int HD, int DT>
 hipError_t launch_dt(const SpFp8Attn &A, hipStream_t s) {
     constexpr int NW = HD == 256 ? 4 : 8;
     constexpr int CG = HD == 256 || DT == SP_DTYPE_F32 ? 1 : 2;
+    constexpr int MANY = 256 * 16 * CG + 1, EACH = 64, LONG = HD == 256 && DT != SP_DTYPE_F32 ? 48 : 96;
     const long long columns = (long long)A.s.n_rows * A.G;  // of each KV head
-    constexpr int MANY = 256 * 16 * CG + (HD == 256 ? 0 : 1), EACH = DT == SP_DTYPE_F32 ? 128 : 64;
-    if (A.s.row && columns * A.H >= MANY && columns >= EACH * (long long)A.s.n_seq) return launch_wide<Fp4, HD, DT>(A, s);
-    if (columns > 16ll * A.s.n_seq) return launch<Fp4, HD, DT, NW, CG>(A, s);
+    if (A.s.row && columns >= EACH * (long long)A.s.n_seq &&
+        (columns * A.H >= MANY || (columns * A.H >= MANY / 2 && most_blocks(A) >= LONG)))
+        return launch_wide<Fp4, HD, DT>(A, s);
+    if (CG == 2 && columns > 16ll * A.s.n_seq) return launch<Fp4, HD, DT, NW, CG>(A, s);
+    if (few_groups(A, 16) * A.H > 256) return launch<Fp4, HD, DT, 4, 1>(A, s);
     return launch<Fp4, HD, DT, NW, 1>(A, s);
 }
 
