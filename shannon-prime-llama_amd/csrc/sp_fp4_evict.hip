@@ -342,23 +342,29 @@ hipError_t launch_weigh(const SpFp4Weigh &A, int dtype, hipStream_t s) {
 // ---------------------------------------------------------------------------
 // evict
 // ---------------------------------------------------------------------------
-// Which positions stay: one block of threads for each (sequence, KV head) finds the key (the weight's
-// bits, in order) of the last one that stays, by counts of eleven of its bits at a time from the top
-// of the range that the keys have (attention weights span few of a float's octaves: bits above the
-// range would put them into few bins, where lanes that meet take turns: 13 us for 2 with 32768
-// positions). Then it writes the kept positions in order: each wave counts its run of the
-// positions, and with the counts of the waves before it knows where its own go.
+// Which positions stay: one block of threads for each (sequence, KV head) finds the last one that stays, by its
+// key (the weight's bits, in order) and position. Counts of eleven of the keys' bits, from the top of the range that
+// they have, find a bin (attention weights span few of a float's octaves: bits above the range would
+// put them into few bins, where lanes that meet take turns: 13 us for 2 with 32768 positions); when it holds
+// no more than MOST_FEW of them, these are listed and compared with each other. Then the kept positions are
+// written in order: each wave counts its run of the positions, and with the counts of the waves before it
+// knows where its own go.
 //
-// A wave's run is consecutive, and a lane has four neighbours of each 256 positions. The keys are made
-// once and kept in LDS where it holds them; those of longer sequences are made again for each pass.
+// A wave's run is consecutive, and a lane has four neighbours of each 256 positions. K of these fours stay in registers
+// from the first pass on (K 0, longer sequences: they are made again for each).
+//
+// Bound by latencies: with 32768 positions of 8 KV heads 16 us, 6 of them for the weights, whose 1024 lines
+// are as many as a CU has in flight in that time, 4 for the counts, 4 to list and compare 80 keys and 3 to write 8192
+// positions; with 1064 positions of 12 x 8 5 us, 2 of them for lengths, table and weights. Keys in LDS and counts
+// down to the last bit took 20 us of the first and the same of the second.
 constexpr int SN = SP_FP4_EVICT_THREADS;
 
 // Order of weights as unsigned numbers: NaN below all, -0 as 0.
+constexpr unsigned NO_PLACE = 0, NAN_KEY = 1, NO_KEY = 0xffffffffu;  // NO_KEY: stays whatever its weight
 __device__ __forceinline__ unsigned key_of(float w) {
     const unsigned u = __float_as_uint(w + 0.0f);
-    return w != w ? 0u : (u >> 31) ? ~u : u | 0x80000000u;
+    return w != w ? NAN_KEY : (u >> 31) ? ~u : u | 0x80000000u;
 }
-constexpr unsigned NO_KEY = 0xffffffffu;  // of a position that stays whatever its weight, and of places that have none
 
 __device__ __forceinline__ unsigned wave_umax(unsigned v) {
 #define SP_MAX(ctrl) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xf, 0xf, true))
@@ -371,17 +377,18 @@ __device__ __forceinline__ unsigned wave_umax(unsigned v) {
                max((unsigned)__builtin_amdgcn_readlane((int)v, 32), (unsigned)__builtin_amdgcn_readlane((int)v, 48)));
 }
 
-constexpr int MOST_KEYS = 36 * 1024;  // that LDS holds beside the counts
-
-// AT_ONCE: loads of a lane that are made together.
-template <bool HELD, int AT_ONCE>
+template <int K>
 __global__ __launch_bounds__(SN) void k_fp4_select(SpFp4Evict A) {
-    constexpr int NW = SN / 64, BITS = 11, BINS = 1 << BITS;
-    extern __shared__ __align__(16) unsigned keys[];
+    constexpr int NW = SN / 64, BITS = 11, BINS = 1 << BITS, STEP = K ? K : 4;
+    constexpr int MOST_FEW = 256;
+    typedef unsigned long long u64;
     __shared__ int bins[BINS];
-    __shared__ int wave_n[NW], wave_t[NW];
+    __shared__ __align__(16) u64 few[MOST_FEW];
+    __shared__ int wave_n[NW], wave_more[NW];
     __shared__ unsigned wave_hi[NW], wave_lo[NW];
-    __shared__ int found_bin, found_above, found_here;
+    __shared__ int found_bin, found_above, found_here, n_few;
+    __shared__ unsigned last_key;
+    __shared__ int last_pos;
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int h = blockIdx.x % A.H, seq = blockIdx.x / A.H;
     int a, b, n;
@@ -401,61 +408,54 @@ __global__ __launch_bounds__(SN) void k_fp4_select(SpFp4Evict A) {
     const int *table = A.s.table + (long long)seq * A.s.stride;
     const int last = ((n + 63) >> 6) - 1, behind = n - A.recent;
     int bad = 0;  // a block that is missing
+    uint4 key[STEP];
     // keys from memory: of positions p + 256 i + 4 lane + (0 .. 3)
-    const auto make = [&](int p, uint4 (&key)[AT_ONCE]) __attribute__((always_inline)) {
-        int blk[AT_ONCE];
-        float4 weight[AT_ONCE];
+    const auto make = [&](int p) __attribute__((always_inline)) {
+        int blk[STEP];
+        float4 weight[STEP];
 #pragma unroll
-        for (int i = 0; i < AT_ONCE; i++) blk[i] = table[min((p + i * 256 + 4 * lane) >> 6, last)];
+        for (int i = 0; i < STEP; i++) blk[i] = table[min((p + i * 256 + 4 * lane) >> 6, last)];
 #pragma unroll
-        for (int i = 0; i < AT_ONCE; i++) {
+        for (int i = 0; i < STEP; i++) {
             bad |= blk[i] < 0 || blk[i] >= A.s.n_blocks;
             weight[i] = *reinterpret_cast<const float4 *>(
                 A.weight + ((long long)min(max(blk[i], 0), A.s.n_blocks - 1) * A.H + h) * 64 + (4 * lane & 63));
         }
 #pragma unroll
-        for (int i = 0; i < AT_ONCE; i++) {
+        for (int i = 0; i < STEP; i++) {
             const int at = p + i * 256 + 4 * lane;
-            const auto one = [&](int k, float x) { return at + k < A.first || at + k >= behind ? NO_KEY : key_of(x); };
+            const auto one = [&](int k, float x) {
+                return at + k >= p1 ? NO_PLACE : at + k < A.first || at + k >= behind ? NO_KEY : key_of(x);
+            };
             key[i] = uint4{one(0, weight[i].x), one(1, weight[i].y), one(2, weight[i].z), one(3, weight[i].w)};
         }
     };
-    // the lane's keys in order, four at a time: f(their first position, key, key, key, key)
+    // f(p, i): key[i] has the keys of positions p + (0 .. 3)
     const auto each = [&](auto f) __attribute__((always_inline)) {
-        if constexpr (HELD) {
-#pragma unroll 2
-            for (int p = p0; p < p1; p += 256) {
-                const uint4 k = *reinterpret_cast<const uint4 *>(keys + p + 4 * lane);
-                f(p + 4 * lane, k.x, k.y, k.z, k.w);
-            }
-        } else {
-            for (int p = p0; p < p1; p += 256 * AT_ONCE) {
-                uint4 k[AT_ONCE];
-                make(p, k);
+        for (int p = p0; p < p1; p += 256 * STEP) {
+            if (K == 0) make(p);
 #pragma unroll
-                for (int i = 0; i < AT_ONCE; i++)
-                    if (p + i * 256 < p1) f(p + i * 256 + 4 * lane, k[i].x, k[i].y, k[i].z, k[i].w);
-            }
+            for (int i = 0; i < STEP; i++)
+                if (p + i * 256 < p1) f(p + i * 256 + 4 * lane, i);
         }
     };
     // ---- the keys' range ----
-    unsigned hi = 0, lo = 0;  // largest key + 1, complement of the least (0: no key)
-    for (int p = p0; p < p1; p += 256 * AT_ONCE) {
-        uint4 k[AT_ONCE];
-        make(p, k);
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; i++) {
-            hi = max(max(hi, max(k[i].x + 1, k[i].y + 1)), max(k[i].z + 1, k[i].w + 1));
-            lo = max(max(lo, max(~k[i].x, ~k[i].y)), max(~k[i].z, ~k[i].w));
-            if (HELD && p + i * 256 < p1) *reinterpret_cast<uint4 *>(keys + p + i * 256 + 4 * lane) = k[i];
-        }
-    }
+    unsigned hi = 0, lo = 0;  // largest key + 1, the least one's negative
+    if (K) make(p0);
+    each([&](int, int i) __attribute__((always_inline)) {
+        const uint4 k = key[i];
+        hi = max(max(hi, max(k.x + 1, k.y + 1)), max(k.z + 1, k.w + 1));
+        lo = max(max(lo, max(0 - k.x, 0 - k.y)), max(0 - k.z, 0 - k.w));
+    });
     hi = wave_umax(hi);
     lo = wave_umax(lo);
     for (int k = tid; k < BINS; k += SN) bins[k] = 0;
+    if (tid < MOST_FEW) few[tid] = 0;
+    if (tid == 0) n_few = 0;
     if (lane == 0) {
         wave_hi[w] = hi;
         wave_lo[w] = lo;
+        wave_more[w] = 0;
     }
     if (__syncthreads_or(bad)) {
         for (int j = tid; j < A.keep; j += SN) kept[j] = -1;
@@ -463,27 +463,28 @@ __global__ __launch_bounds__(SN) void k_fp4_select(SpFp4Evict A) {
     }
     hi = wave_umax(lane < NW ? wave_hi[lane] : 0u);
     lo = wave_umax(lane < NW ? wave_lo[lane] : 0u);
-    const unsigned least = ~lo;
-    // ---- the key of the last that stays: of those in [limit, limit + 2^shift) `want` stay ----
+    const unsigned least = 0 - lo;
+    // ---- the bin of the last that stays: of the `here` keys in [limit, limit + 2^shift) `want` stay ----
     int want = A.keep - A.first - A.recent, here = n - A.first - A.recent;
     unsigned limit = least;
-    int shift = want && hi > least + 1 ? 32 - __clz(hi - 1 - least) : 0;
-    for (bool fresh = true; shift > 0; fresh = false) {
+    int shift = hi > least + 1 ? 32 - __clz(hi - 1 - least) : 0;
+    // (it ends before NO_KEY)
+    const auto span = [&]() { return shift == 32 ? NO_KEY - limit : min(1u << shift, NO_KEY - limit); };
+    for (bool fresh = true; want && shift > 0 && here > want && here > MOST_FEW; fresh = false) {
         const int down = max(shift - BITS, 0);
-        // (no key but NO_KEY is past it: with 32 bits the range ends there)
-        const unsigned span = shift == 32 ? NO_KEY - limit : 1u << shift;
         if (!fresh) {
             for (int k = tid; k < BINS; k += SN) bins[k] = 0;
             __syncthreads();
         }
+        const unsigned size = span();
         const auto count = [&](unsigned k) __attribute__((always_inline)) {
-            if (k - limit < span && k != NO_KEY) atomicAdd(&bins[(k - limit) >> down], 1);
+            if (k - limit < size) atomicAdd(&bins[(k - limit) >> down], 1);
         };
-        each([&](int, unsigned k0, unsigned k1, unsigned k2, unsigned k3) __attribute__((always_inline)) {
-            count(k0);
-            count(k1);
-            count(k2);
-            count(k3);
+        each([&](int, int i) __attribute__((always_inline)) {
+            count(key[i].x);
+            count(key[i].y);
+            count(key[i].z);
+            count(key[i].w);
         });
         __syncthreads();
         // sums from the top: thread 0 has the two highest bins
@@ -504,46 +505,81 @@ __global__ __launch_bounds__(SN) void k_fp4_select(SpFp4Evict A) {
         want -= found_above;
         here = found_here;
         shift = down;
-        if (here == want) break;  // all of them stay
     }
-    // Keys from `over` on stay; but of those that equal the limit, where they are more than are wanted, the
-    // first `want`. (None wanted, and none between: `over` is NO_KEY alone.)
-    const bool tied = here != want && want > 0;
-    const unsigned over = want == 0 ? NO_KEY : tied ? limit + 1 : limit;
-    int n_stay = 0, n_tie = 0;  // of this lane, then of the wave
-    each([&](int p, unsigned k0, unsigned k1, unsigned k2, unsigned k3) __attribute__((always_inline)) {
-        n_stay += (k0 >= over && p < p1) + (k1 >= over && p + 1 < p1) + (k2 >= over && p + 2 < p1) + (k3 >= over && p + 3 < p1);
-        if (tied) n_tie += (k0 == limit) + (k1 == limit) + (k2 == limit) + (k3 == limit);
-    });
-    n_stay = sp_fp8_scan(n_stay, lane);
-    n_tie = sp_fp8_scan(n_tie, lane);
-    if (lane == 63) {
-        wave_n[w] = n_stay;
-        wave_t[w] = n_tie;
-    }
-    __syncthreads();
-    int at = 0, met = 0;  // kept before this wave's run, and keys at the limit met
-    for (int k = 0; k < w; k++) {
-        at += wave_n[k] + max(min(wave_t[k], want - met), 0);
-        met += wave_t[k];
-    }
-    each([&](int p, unsigned k0, unsigned k1, unsigned k2, unsigned k3) __attribute__((always_inline)) {
-        bool stays[4] = {k0 >= over && p < p1, k1 >= over && p + 1 < p1, k2 >= over && p + 2 < p1, k3 >= over && p + 3 < p1};
-        if (tied) {
-            const int mine = (k0 == limit) + (k1 == limit) + (k2 == limit) + (k3 == limit), sum = sp_fp8_scan(mine, lane);
-            int t = met + sum - mine;
-            const unsigned k[4] = {k0, k1, k2, k3};
+    // ---- the last that stays: a position stays if its key is larger, or the same and it is no later ----
+    unsigned end = want ? limit : NO_KEY;
+    int end_pos = 0x7fffffff;
+    const bool compare = want && here > want && here <= MOST_FEW;
+    const auto stays = [&](unsigned k, int p) { return k > end - (p <= end_pos); };
+    int n_stay = 0;  // of this lane, then of the wave
+    if (compare) {
+        const unsigned size = span();
+        each([&](int p, int i) __attribute__((always_inline)) {
+            const unsigned k[4] = {key[i].x, key[i].y, key[i].z, key[i].w};
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (k[i] == limit) stays[i] = t++ < want;
-            met += __builtin_amdgcn_readlane(sum, 63);
+            for (int x = 0; x < 4; x++)
+                if (k[x] - limit < size) few[atomicAdd(&n_few, 1)] = (u64)k[x] << 32 | (unsigned)~(p + x);  // (`here` of them)
+                else n_stay += k[x] >= limit;
+        });
+        __syncthreads();
+        if (tid < here) {
+            const u64 mine = few[tid];
+            int above = 0;
+            for (int k = 0; k < here; k += 4)  // (behind them are zeros)
+#pragma unroll
+                for (int x = 0; x < 4; x++) above += few[k + x] > mine;
+            const int p = ~(unsigned)mine;
+            if (above < want) atomicAdd(&wave_more[p / run], 1);
+            if (above == want - 1) {
+                last_key = (unsigned)(mine >> 32);
+                last_pos = p;
+            }
         }
-        const int mine = stays[0] + stays[1] + stays[2] + stays[3], sum = sp_fp8_scan(mine, lane);
+    } else {
+        if (want && here > want) {  // all the same: the first `want` of them
+            int ties = 0;
+            each([&](int, int i) __attribute__((always_inline)) {
+                ties += (key[i].x == end) + (key[i].y == end) + (key[i].z == end) + (key[i].w == end);
+            });
+            ties = sp_fp8_scan(ties, lane);
+            if (lane == 63) wave_n[w] = ties;
+            __syncthreads();
+            int met = 0;
+            for (int k = 0; k < w; k++) met += wave_n[k];
+            if (met < want && met + wave_n[w] >= want)
+                each([&](int p, int i) __attribute__((always_inline)) {
+                    const unsigned k[4] = {key[i].x, key[i].y, key[i].z, key[i].w};
+                    const int mine = (k[0] == end) + (k[1] == end) + (k[2] == end) + (k[3] == end), sum = sp_fp8_scan(mine, lane);
+                    int t = met + sum - mine;
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        if (k[x] == end && ++t == want) last_pos = p + x;
+                    met += __builtin_amdgcn_readlane(sum, 63);
+                });
+            __syncthreads();
+            end_pos = last_pos;
+        }
+        each([&](int p, int i) __attribute__((always_inline)) {
+            n_stay += stays(key[i].x, p) + stays(key[i].y, p + 1) + stays(key[i].z, p + 2) + stays(key[i].w, p + 3);
+        });
+    }
+    n_stay = sp_fp8_scan(n_stay, lane);
+    if (lane == 63) wave_n[w] = n_stay;
+    __syncthreads();
+    if (compare) {
+        end = last_key;
+        end_pos = last_pos;
+    }
+    int at = 0;  // kept before this wave's run
+    for (int k = 0; k < w; k++) at += wave_n[k] + wave_more[k];
+    each([&](int p, int i) __attribute__((always_inline)) {
+        const bool stay[4] = {stays(key[i].x, p), stays(key[i].y, p + 1), stays(key[i].z, p + 2), stays(key[i].w, p + 3)};
+        const int mine = stay[0] + stay[1] + stay[2] + stay[3], sum = sp_fp8_scan(mine, lane);
         int j = at + sum - mine;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (stays[i] && j < A.keep) kept[j] = p + i;
-            j += stays[i];
+        for (int x = 0; x < 4; x++) {
+            if (stay[x] && j < A.keep) kept[j] = p + x;
+            j += stay[x];
         }
         at += __builtin_amdgcn_readlane(sum, 63);
     });
@@ -639,11 +675,10 @@ hipError_t sp_fp4_launch_weigh(const SpFp4Weigh &A, int hd, int dtype, hipStream
 hipError_t sp_fp4_launch_evict(const SpFp4Evict &A, hipStream_t s) {
     void *args[] = {const_cast<SpFp4Evict *>(&A)};
     // no sequence is longer than its table row
-    const long long most = ((long long)A.s.stride * 64 + 255) / 256 * 256;
-    const bool held = most <= MOST_KEYS;
-    const void *select = !held ? (const void *)k_fp4_select<false, 4>
-                       : most <= 8 * SN ? (const void *)k_fp4_select<true, 2> : (const void *)k_fp4_select<true, 8>;
-    const hipError_t e = hipLaunchKernel(select, dim3((unsigned)(A.H * A.s.n_seq)), dim3(SN), args, held ? (size_t)most * 4 : 0, s);
+    const long long most = (long long)A.s.stride * 64;
+    const void *select = most <= 2 * 4 * SN ? (const void *)k_fp4_select<2>
+                       : most <= 8 * 4 * SN ? (const void *)k_fp4_select<8> : (const void *)k_fp4_select<0>;
+    const hipError_t e = hipLaunchKernel(select, dim3((unsigned)(A.H * A.s.n_seq)), dim3(SN), args, 0, s);
     if (e != hipSuccess) return e;
     // Many sequences and KV heads: blocks of 256 threads with four planes and 1024 places a round. Few, with more
     // places: blocks of 1024 threads with one plane and 8192 places.
