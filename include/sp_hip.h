@@ -603,8 +603,8 @@ int  sp_hip_fp4_weigh(sp_hip_fp4_cache_t *c, int layer, const sp_hip_fp4_batch_t
  * it is and gets 0 .. n - 1, then -1). A position of an attention call is then its place, so a window
  * counts kept positions, and keys should carry their rotation already. A sequence with a table entry
  * missing in its length is left as it is and gets -1. d_len is not changed, d_row is not read
- * (n_rows = n_seq without it). No other call may use the sequences' blocks meanwhile, and no two of
- * them share a block. */
+ * (n_rows = n_seq without it). No other call may use the sequences' blocks meanwhile, and no block
+ * is theirs twice. */
 int  sp_hip_fp4_evict(sp_hip_fp4_cache_t *c, int layer, const sp_hip_fp4_batch_t *batch, int keep, int first, int recent,
                       int32_t *d_kept, void *stream);
 

@@ -87,11 +87,6 @@ __device__ __forceinline__ h8 eight(unsigned w, float scale) {
 // Exponent bytes e of four positions relative to the block's largest, `top`: bytes of 2^(e - top) as
 // floats have them. No byte borrows from its neighbour: they are within 87 and 167 and at most top.
 __device__ __forceinline__ unsigned relative(unsigned e, int top) { return e - (unsigned)(top - 127) * 0x01010101u; }
-// The float with exponent byte B of `rel`.
-template <int B>
-__device__ __forceinline__ float power(unsigned rel) {
-    return __int_as_float((B == 3 ? rel >> 1 : rel << (23 - 8 * B)) & 0x7f800000);
-}
 
 // Largest bytes: of dwords, gathered in pairs of 16 bits.
 typedef unsigned short s2 __attribute__((ext_vector_type(2)));

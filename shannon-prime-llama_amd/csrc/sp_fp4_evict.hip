@@ -13,6 +13,7 @@ using sp_fp4::eight;
 using sp_fp4::Largest;
 using sp_fp4::relative;
 
+// The float with exponent byte b of rel.
 __device__ __forceinline__ float power(unsigned rel, int b) {
     return __int_as_float((b == 3 ? rel >> 1 : rel << (23 - 8 * b)) & 0x7f800000);
 }
@@ -518,8 +519,12 @@ __global__ __launch_bounds__(SN) void k_fp4_select(SpFp4Evict A) {
             const unsigned k[4] = {key[i].x, key[i].y, key[i].z, key[i].w};
 #pragma unroll
             for (int x = 0; x < 4; x++)
-                if (k[x] - limit < size) few[atomicAdd(&n_few, 1)] = (u64)k[x] << 32 | (unsigned)~(p + x);  // (`here` of them)
-                else n_stay += k[x] >= limit;
+                if (k[x] - limit < size) {
+                    const int at = atomicAdd(&n_few, 1);  // (`here` of them, unless weights change meanwhile)
+                    if (at < MOST_FEW) few[at] = (u64)k[x] << 32 | (unsigned)~(p + x);
+                } else {
+                    n_stay += k[x] >= limit;
+                }
         });
         __syncthreads();
         if (tid < here) {
@@ -611,7 +616,7 @@ __global__ __launch_bounds__(NT) void k_fp4_move(SpFp4Evict A) {
 #pragma unroll
         for (int k = 0; k < ROUND; k++) {
             const int j = j0 + k * NT + tid;
-            p[k] = j < A.keep ? kept[j] : j;
+            p[k] = j < A.keep ? max(min(kept[j], n - 1), j) : j;  // (where they are, whatever kept holds)
         }
 #pragma unroll
         for (int k = 0; k < ROUND; k++) {

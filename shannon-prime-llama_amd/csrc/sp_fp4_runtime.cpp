@@ -153,6 +153,7 @@ extern "C" int sp_hip_fp4_evict(sp_hip_fp4_cache_t *c, int layer, const sp_hip_f
     SpFp4Evict A;
     memset(&A, 0, sizeof(A));
     if (!batch_ok(c, layer, b, who, &A.s)) return -1;
+    A.s.row = nullptr;
     if (keep < 1 || keep > MAX_ROWS || first < 0 || recent < 0 || first > keep || recent > keep - first) {
         sp_set_error("%s: keep %d with the first %d and the last %d", who, keep, first, recent);
         return -1;

@@ -249,6 +249,44 @@ def test_many_columns_over_many_blocks():
     P.check_attend("bf16", queries(rng, P, 256, "bf16")[:, :256], 0.1)
 
 
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_a_chunk_behind_a_long_table(hd, dtype):
+    """Fewer rows than the table's length makes worth sharing a conversion: short and empty sequences among them."""
+    rng = np.random.default_rng(hd)
+    P = Pair(hd, 16, 16)
+    lens, news = [300, 40, 0, 65], [33, 32, 0, 40]
+    table = [list(t) + [-1] * (100 - len(t)) for t in tables(rng, lens, 16)]
+    P.fill(rng, table, lens, dtype)
+    P.batch(table, lens, np.concatenate([[0], np.cumsum(news)]).tolist(), sum(news) + 2)
+    P.check_attend(dtype, queries(rng, P, 64, dtype), 0.1, window=0)
+
+
+@pytest.mark.parametrize("hd,dtype", [(128, "bf16"), (256, "f32")])
+def test_a_chunk_behind_a_long_cache(hd, dtype):
+    rng = np.random.default_rng(hd)
+    P = Pair(hd, 2, 110)
+    P.fill(rng, tables(rng, [6500], 110), [6500], dtype)
+    P.batch(P.table, [6500], [0, 70])
+    P.check_attend(dtype, queries(rng, P, 64, dtype), 0.1)
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_more_column_groups_than_cus(hd, dtype):
+    rng = np.random.default_rng(hd)
+    P = Pair(hd, 32, 64)
+    lens = [1, 64, 700, 65, 0, 130, 300, 20, 513]
+    table = tables(rng, [n + 3 for n in lens], 64)
+    P.fill(rng, table, lens, dtype)
+    P.batch(table, lens)
+    P.check_attend(dtype, queries(rng, P, 96, dtype), 0.1)
+    lens = [n + 3 for n in lens]
+    P.batch(table, lens, [3 * i for i in range(len(lens) + 1)])
+    P.write(dtype, P.rows(rng, dtype), P.rows(rng, dtype))
+    P.check_attend(dtype, queries(rng, P, 192, dtype), 0.1)
+
+
 def test_tables_with_holes():
     rng = np.random.default_rng(1)
     for hd in (64, 128, 256):

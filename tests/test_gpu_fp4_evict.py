@@ -63,6 +63,17 @@ def test_weigh_groups(group):
         P.check_weigh(dtype, queries(rng, P, 3 * group, dtype), 0.1)
 
 
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype,pad", [("f32", 0), ("f16", 0), ("bf16", 0), ("bf16", 3)])
+def test_weigh_more_columns_than_a_stage(hd, dtype, pad):
+    rng = np.random.default_rng(hd + pad)
+    P = Pair(hd, 2, 24)
+    lens = [150, 1000]
+    P.fill(rng, tables(rng, lens, 24), lens, dtype)
+    P.batch(P.table, lens, [0, 150, 251], 255)
+    P.check_weigh(dtype, queries(rng, P, 10, dtype), 0.1, pad=pad)
+
+
 def test_weigh_many_sequences_and_holes():
     rng = np.random.default_rng(3)
     P = Pair(64, 1, 320)
@@ -156,6 +167,48 @@ def test_evict_long_and_ragged():
     P.check_evict(2100, 0, 0)
 
 
+@pytest.mark.parametrize("longest", [3000, 20000, 40000])
+@pytest.mark.parametrize("kind", ["spread", "few", "equal", "crowded"])
+def test_evict_by_length(longest, kind):
+    """Table rows of each length that the selection tells apart; values that are all different, that are few, one,
+    or neighbours in their last bits."""
+    rng = np.random.default_rng(longest)
+    P = Pair(64, 1, 1300)
+    lens = [longest, longest * 4 // 5 + 1, 64, longest // 4 + 200]
+    P.batch(tables(rng, lens, 1300), lens)
+    fill_device(rng, P)
+    shape = P.ref.weight.shape
+    P.set_weights({"spread": lambda: np.exp(2 * rng.standard_normal(shape)),
+                   "few": lambda: rng.integers(0, 5, shape) / 4.0,
+                   "equal": lambda: np.full(shape, 0.5),
+                   "crowded": lambda: np.float32(1.0) + rng.integers(0, 4096, shape) * 2.0 ** -23}[kind]())
+    P.check_evict(longest // 4 + 11, 4, 300)
+
+
+def test_evict_keeps_nothing_by_weight():
+    """All that stays is first or recent; and a few to choose from."""
+    rng = np.random.default_rng(12)
+    P = Pair(96, 2, 30)
+    lens = [600, 300, 201]
+    P.batch(tables(rng, lens, 30), lens)
+    fill_device(rng, P)
+    P.set_weights(rng.random(P.ref.weight.shape))
+    P.check_evict(200, 60, 140)
+    P.batch(P.table, [min(n, 200) for n in lens])
+    P.check_evict(100, 0, 1)
+
+
+def test_evict_many_sequences():
+    """More than one round of places in each of many blocks of threads."""
+    rng = np.random.default_rng(13)
+    P = Pair(64, 8, 460)
+    lens = [1600 - 7 * i for i in range(17)]
+    P.batch(tables(rng, lens, 460), lens)
+    fill_device(rng, P)
+    P.set_weights(rng.random(P.ref.weight.shape))
+    P.check_evict(1500, 4, 100)
+
+
 def test_evict_leaves_incomplete_sequences():
     rng = np.random.default_rng(3)
     P = Pair(128, 2, 30)
@@ -234,3 +287,38 @@ def test_captured_eviction_follows_lengths():
         np.testing.assert_array_equal(kept.cpu().numpy(), want)
         P.check_memory()
         lens = [200 + 37 * (turn + 1), 100 + 70 * (turn + 1)]
+
+
+def test_captured_weigh_adds_at_each_replay():
+    rng = np.random.default_rng(10)
+    H, n_q = 2, 8
+    P = Pair(128, H, 20)
+    lens = [400, 130]
+    P.fill(rng, tables(rng, [500, 300], 20), lens, "bf16")
+    P.batch(P.table, lens)
+    q = queries(rng, P, n_q, "bf16")
+    qt = q.cuda()
+    out = torch.zeros_like(qt)
+    lse = torch.zeros((2, n_q), dtype=torch.float32, device="cuda")
+    L = S.lib()
+    g = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=side):
+        s = torch.cuda.current_stream().cuda_stream
+        S.check(L.sp_hip_fp4_attn_decode(P.dev.ref, 0, P.b.ref, qt.data_ptr(), n_q * 128, n_q, S.DTYPE_BF16, 0.1, 0,
+                                         out.data_ptr(), n_q * 128, lse.data_ptr(), s), "decode")
+        S.check(L.sp_hip_fp4_weigh(P.dev.ref, 0, P.b.ref, qt.data_ptr(), n_q * 128, n_q, S.DTYPE_BF16, 0.1, 0,
+                                   lse.data_ptr(), s), "weigh")
+    for turn in range(4):
+        P.set_lens(lens)
+        before = P.weights()
+        g.replay()
+        torch.cuda.synchronize()
+        P.ref.weight = before.copy()
+        tol = P.ref.weigh(0, P.table, lens, None, 2, q.double().numpy(), float(np.float32(0.1)), 0,
+                          lse.double().cpu().numpy())
+        assert (np.abs(P.weights() - P.ref.weight) <= tol).all()
+        lens = [n - 60 for n in lens]
+        torch.full((64, 1024), 3.0, device="cuda").sum()
+        torch.cuda.synchronize()
