@@ -593,38 +593,45 @@ __global__ __launch_bounds__(SN) void k_fp4_select(SpFp4Evict A) {
 // Rows to their new places: a block of threads for each (sequence, KV head, side) and PLANES planes of
 // eight channels goes up the places. A row never moves up, so a place's row lies at or behind it:
 // a round that has loaded its rows may store them, whatever the rounds before and behind do. A
-// round is so large (NT places, ROUND of a thread) that most calls take one.
+// round is so large (NT places, ROUND of a thread) that most calls take one. It is a chain of three loads (position,
+// block, row): each round's are in flight together, and the first's with the sequence's length.
 template <int NT, int PLANES, int ROUND>
 __global__ __launch_bounds__(NT) void k_fp4_move(SpFp4Evict A) {
     constexpr int PLACES = NT * ROUND;
     const int tid = threadIdx.x;
     const int h = blockIdx.x % A.H, seq = blockIdx.x / A.H, is_v = blockIdx.y & 1, n0 = (blockIdx.y >> 1) * PLANES;
+    const int *kept = A.kept + ((long long)seq * A.H + h) * A.keep;
+    const int *table = A.s.table + (long long)seq * A.s.stride;
+    int p[ROUND], dst[ROUND];  // positions, blocks of the places
+    const auto fetch = [&](int j0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < ROUND; k++) {
+            const int j = min(j0 + k * NT + tid, A.keep - 1);
+            p[k] = kept[j];
+            dst[k] = table[min(j >> 6, A.s.stride - 1)];
+        }
+    };
+    // the first round's are on their way together with what tells whether there is one
+    fetch(0);
     int a, b, n;
     sp_fp8_seq(A.s, seq, a, b, n);
-    if (n <= A.keep) return;
-    const int *kept = A.kept + ((long long)seq * A.H + h) * A.keep;
-    if (kept[0] < 0) return;  // a block is missing
+    const int head = kept[0];
+#pragma unroll
+    for (int k = 0; k < ROUND; k++) __asm__ volatile("" : "+v"(p[k]), "+v"(dst[k]));
+    if (n <= A.keep || head < 0) return;  // head: a block is missing
     const SpFp8Side side = A.side[is_v];
-    const int *table = A.s.table + (long long)seq * A.s.stride;
     const int tile = A.NC * 256, exps = A.NC * 64;  // dwords of codes, bytes of exponents
     const bool with_exp = n0 % 4 == 0, with_weight = is_v == 0 && n0 == 0;
     unsigned *codes = reinterpret_cast<unsigned *>(side.codes) + n0 * 64;
     uint8_t *exp_plane = side.exps + n0 / 4 * 64;
     for (int j0 = 0; j0 < A.keep; j0 += PLACES) {
-        int p[ROUND];
-        long long from[ROUND], to[ROUND];  // tiles
+        int src[ROUND];  // blocks of the positions
+        if (j0) fetch(j0);
 #pragma unroll
         for (int k = 0; k < ROUND; k++) {
             const int j = j0 + k * NT + tid;
-            p[k] = j < A.keep ? max(min(kept[j], n - 1), j) : j;  // (where they are, whatever kept holds)
-        }
-#pragma unroll
-        for (int k = 0; k < ROUND; k++) {
-            const int j = j0 + k * NT + tid;
-            from[k] = to[k] = 0;
-            if (p[k] == j) continue;
-            from[k] = (long long)table[p[k] >> 6] * A.H + h;
-            to[k] = (long long)table[j >> 6] * A.H + h;
+            p[k] = j < A.keep ? max(min(p[k], n - 1), j) : j;  // (where they are, whatever kept holds)
+            src[k] = table[min(p[k], n - 1) >> 6];
         }
         unsigned code[ROUND][PLANES];
         uint8_t e[ROUND];
@@ -633,10 +640,11 @@ __global__ __launch_bounds__(NT) void k_fp4_move(SpFp4Evict A) {
         for (int k = 0; k < ROUND; k++) {
             const int j = j0 + k * NT + tid;
             if (p[k] == j) continue;
+            const long long from = (long long)src[k] * A.H + h;  // tile
 #pragma unroll
-            for (int x = 0; x < PLANES; x++) code[k][x] = codes[from[k] * tile + x * 64 + (p[k] & 63)];
-            if (with_exp) e[k] = exp_plane[from[k] * exps + sp_fp4_place(p[k] & 63)];
-            if (with_weight) weight[k] = A.weight[from[k] * 64 + (p[k] & 63)];
+            for (int x = 0; x < PLANES; x++) code[k][x] = codes[from * tile + x * 64 + (p[k] & 63)];
+            if (with_exp) e[k] = exp_plane[from * exps + sp_fp4_place(p[k] & 63)];
+            if (with_weight) weight[k] = A.weight[from * 64 + (p[k] & 63)];
         }
         // what this round loads is in registers before any of it is stored over
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -645,10 +653,11 @@ __global__ __launch_bounds__(NT) void k_fp4_move(SpFp4Evict A) {
         for (int k = 0; k < ROUND; k++) {
             const int j = j0 + k * NT + tid;
             if (p[k] == j) continue;
+            const long long to = (long long)dst[k] * A.H + h;
 #pragma unroll
-            for (int x = 0; x < PLANES; x++) codes[to[k] * tile + x * 64 + (j & 63)] = code[k][x];
-            if (with_exp) exp_plane[to[k] * exps + sp_fp4_place(j & 63)] = e[k];
-            if (with_weight) A.weight[to[k] * 64 + (j & 63)] = weight[k];
+            for (int x = 0; x < PLANES; x++) codes[to * tile + x * 64 + (j & 63)] = code[k][x];
+            if (with_exp) exp_plane[to * exps + sp_fp4_place(j & 63)] = e[k];
+            if (with_weight) A.weight[to * 64 + (j & 63)] = weight[k];
         }
     }
     // behind the last place nothing counts in its block's largest exponent
@@ -686,7 +695,8 @@ hipError_t sp_fp4_launch_evict(const SpFp4Evict &A, hipStream_t s) {
     const hipError_t e = hipLaunchKernel(select, dim3((unsigned)(A.H * A.s.n_seq)), dim3(SN), args, 0, s);
     if (e != hipSuccess) return e;
     // Many sequences and KV heads: blocks of 256 threads with four planes and 1024 places a round. Few, with more
-    // places: blocks of 1024 threads with one plane and 8192 places.
+    // places: blocks of 1024 threads with one plane and 8192 places. (1000 places of 12 x 8: 6.4 us, the other way 27.8;
+    // 8192 of 1 x 8: 24.6, the other way 9.8.)
     const long long groups = (long long)A.H * A.s.n_seq * 2 * A.NC;
     return groups < 256 && A.keep > 1024 ? launch_move<1024, 1, 8>(A, s) : launch_move<256, 4, 4>(A, s);
 }
