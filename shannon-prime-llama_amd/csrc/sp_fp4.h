@@ -51,6 +51,7 @@ struct SpFp4Weigh {
     float c;  // |kq_scale| * log2(e) / 2
     int negate;
     int cus;
+    int blocks;  // log2 of the blocks that a block of threads takes at a time
 };
 
 struct SpFp4Evict {

@@ -21,8 +21,8 @@ __device__ __forceinline__ float power(unsigned rel, int b) {
 // ---------------------------------------------------------------------------
 // weigh
 // ---------------------------------------------------------------------------
-// A wave holds one block's K as operands, converted once, and eight waves of a block of threads take
-// eight consecutive blocks of a sequence. Columns (row, query head) pass by in stages: the block of
+// A wave holds one block's K as operands, converted once, and the eight waves of a block of threads take
+// eight consecutive blocks of a sequence, or fewer and part of the columns each. Columns (row, query head) pass by in stages: the block of
 // threads brings them into LDS as operands, and each wave takes them 16 at a time. The weights are
 // summed over columns in the registers that the scores come in, and over the 16 lanes at the end.
 //
@@ -30,6 +30,11 @@ __device__ __forceinline__ float power(unsigned rel, int b) {
 // conversion. K counts relative to the block's largest exponent, for bf16 2^-12 of that, so that no
 // sum of finite queries passes a float. fp32 queries are scaled by a power of two and split in two
 // fp16 parts, as in attention.
+//
+// Bound for many columns by the matrix cores and the exponentials (for 64 positions of 16 columns 16 and 16
+// instructions of 16 and 8 cycles at head_dim 128, beside one multiplication and one addition a weight): 64 rows over 32768
+// positions, 32 / 8 heads, bf16, 26 us, 0.67 PFLOP/s. For few by latencies: one row of 12 sequences of 1 to 4.5K
+// 10.5 us (21 MB of K), of which an empty launch is 4.
 constexpr int WN = 512;  // threads
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
@@ -61,17 +66,22 @@ struct Operand<SP_DTYPE_BF16> {
 
 // DIRECT (16-bit rows at multiples of 16 bytes): a stage's pieces go from memory to LDS past the registers,
 // a wave's 16 bytes a lane as one operand, while the stage before is worked on.
-template <int HD, int DT, bool DIRECT>
-__global__ __launch_bounds__(WN, HD == 256 || (HD == 128 && !DIRECT) ? 2 : 4) void k_fp4_weigh(SpFp4Weigh A, int items) {
+// SHARED: a block of threads takes 2^A.blocks blocks, and its waves share the columns; else eight. (The shared one
+// takes 11.6 us where the other takes 10.5 for the step of 12 sequences below.)
+template <int HD, int DT, bool DIRECT, bool SHARED>
+__global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 96 && SHARED))) ? 2 : 4) void k_fp4_weigh(SpFp4Weigh A, int items) {
     typedef Operand<DT> Op;
     typedef typename Op::V V;
     constexpr int NC = HD / 32, NW = WN / 64;
     constexpr int LP = HD == 64 ? 8 : HD == 256 ? 32 : 16;  // threads of a column (96: twelve of them have a part)
     constexpr bool SPLIT2 = DT == SP_DTYPE_F32;
     constexpr int NH = SPLIT2 ? 2 : 1;
-    constexpr int PER = HD == 64 || DIRECT ? 2 : 1;                          // columns of a thread in a stage
-    constexpr int CS = DIRECT ? (HD == 256 ? 64 : 128) : PER * WN / LP;      // columns of a stage
-    constexpr int BUF = CS / 16 * NC * NH * 64;                              // eights of a stage
+    // Columns of a stage. (Staged by way of registers, 128 of them leave room for half of the waves at head_dim 96: 20 us
+    // for 13 in a step of 12 sequences of 1 to 4.5K; but waves that share them want a part each: 79 us for 114 with
+    // 512 rows over 2048 positions, 32 / 8 heads of 128.)
+    constexpr int CS = DIRECT || SHARED ? (HD == 256 ? 64 : 128) : HD == 64 ? 128 : WN / LP;
+    constexpr int PER = CS * LP / WN;            // of a thread
+    constexpr int BUF = CS / 16 * NC * NH * 64;  // eights of a stage
     typedef typename SpFp8Elem<DT>::T T;
     typedef T T8 __attribute__((ext_vector_type(8)));
     struct Column {
@@ -84,15 +94,16 @@ __global__ __launch_bounds__(WN, HD == 256 || (HD == 128 && !DIRECT) ? 2 : 4) vo
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int h = blockIdx.y, r = lane & 15, g = lane >> 4;
     const bool aligned = (uintptr_t)A.q % sizeof(T8) == 0 && A.q_stride % 8 == 0;
+    const int two = SHARED ? A.blocks : 3;
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        // ---- the sequence, and eight blocks of those that its rows see ----
+        // ---- the sequence, and 2^two blocks of those that its rows see ----
         int seq = -1, r0 = 0, n_new = 0, first = 0, j0 = 0, left = item;
         for (int i0 = 0; i0 < A.s.n_seq && seq < 0; i0 += 64) {
             int a = 0, b = 0, len = 0, lo = 0, n = 0;
             if (i0 + lane < A.s.n_seq) {
                 sp_fp8_seq(A.s, i0 + lane, a, b, len);
                 lo = A.window > 0 ? max(len - (b - a) - A.window + 1, 0) >> 6 : 0;
-                if (b > a) n = (max(min((len + 63) >> 6, A.s.stride) - lo, 0) + NW - 1) / NW;
+                if (b > a) n = (max(min((len + 63) >> 6, A.s.stride) - lo, 0) + (1 << two) - 1) >> two;
             }
             const int sum = sp_fp8_scan(n, lane);
             const unsigned long long past = __ballot(sum > left);
@@ -103,13 +114,13 @@ __global__ __launch_bounds__(WN, HD == 256 || (HD == 128 && !DIRECT) ? 2 : 4) vo
                 r0 = of(a);
                 n_new = of(b) - r0;
                 first = of(len) - n_new;
-                j0 = of(lo) + (left - (of(sum) - of(n))) * NW;
+                j0 = of(lo) + ((left - (of(sum) - of(n))) << two);
             } else {
                 left -= __builtin_amdgcn_readlane(sum, 63);
             }
         }
         if (seq < 0) return;
-        const int t = j0 + w, n_cols = n_new * A.G;
+        const int t = j0 + (w & ((1 << two) - 1)), n_cols = n_new * A.G;
         const int blk = uniform(t <= (first + n_new - 1) >> 6 ? sp_fp8_block(A.s, seq, t) : -1);
         const long long tile = (long long)max(blk, 0) * A.H + h;
         // ---- columns: this thread's eight entries of some, into LDS ----
@@ -246,7 +257,7 @@ __global__ __launch_bounds__(WN, HD == 256 || (HD == 128 && !DIRECT) ? 2 : 4) vo
             }
             if (blk < 0) continue;
 #pragma unroll 1
-            for (int y = 0; y < CS / 16 && c0 + y * 16 < n_cols; y++) {
+            for (int y = w >> two; y < CS / 16 && c0 + y * 16 < n_cols; y += NW >> two) {
                 const int n0 = c0 + y * 16;
                 bool open = all;
                 if (!all) {
@@ -303,8 +314,6 @@ __global__ __launch_bounds__(WN, HD == 256 || (HD == 128 && !DIRECT) ? 2 : 4) vo
                     for (int i = 0; i < 4; i++) acc[n][i] += __builtin_amdgcn_exp2f(s[n][i]);
             }
         }
-        lds_barrier();  // the next item's first stage
-        if (blk < 0) continue;
         // ---- over the columns' lanes: lane r of a row keeps value i = r / 4 of row block n = r % 4 ----
         float sum = 0.0f;
 #pragma unroll
@@ -320,6 +329,16 @@ __global__ __launch_bounds__(WN, HD == 256 || (HD == 128 && !DIRECT) ? 2 : 4) vo
 #undef SP_ROR
                 if (r == i * 4 + n) sum = v;
             }
+        lds_barrier();  // the next item's first stage, or the shares' sums
+        if (SHARED) {
+            float *sums = reinterpret_cast<float *>(qs);
+            sums[tid] = sum;
+            lds_barrier();
+            for (int k = tid + (64 << two); k < WN; k += 64 << two) sum += sums[k];
+            lds_barrier();
+            if (w >> two) continue;
+        }
+        if (blk < 0) continue;
         // position 16 i + 4 g + n. An atomic: two sequences of the call may share the block.
         if (sum != 0.0f) unsafeAtomicAdd(A.weight + tile * 64 + (r >> 2) * 16 + 4 * g + (r & 3), sum);
     }
@@ -327,16 +346,27 @@ __global__ __launch_bounds__(WN, HD == 256 || (HD == 128 && !DIRECT) ? 2 : 4) vo
 
 template <int HD>
 hipError_t launch_weigh(const SpFp4Weigh &A, int dtype, hipStream_t s) {
-    // Eights of blocks: no sequence has more than its table row. The grid is a few blocks of threads
-    // for each CU, which take what there is in turn.
-    const long long most = (long long)A.s.n_seq * ((A.s.stride + 7) / 8);
+    // A block of threads takes eight blocks of a sequence, or fewer and shares the columns out to its waves where
+    // eight would leave CUs idle and each share has 16 columns to work on (32 / 8 heads of 128, bf16, 128 rows over 2048 / 8192
+    // positions: 11.4 / 22.9 us, with eight 33.1 / 33.0; 32 rows over 2048 8.5 and 11.7; float32, 512 over 2048: 79 and 200).
+    SpFp4Weigh a = A;
+    const long long columns = (long long)A.s.n_rows * A.G / A.s.n_seq, all = ((long long)A.s.n_rows + A.window + 126) / 64;
+    const long long seen = A.window > 0 && all < A.s.stride ? all : A.s.stride;  // no sequence has more blocks
+    const auto count = [&](int blocks) { return (long long)A.s.n_seq * ((seen + (1 << blocks) - 1) >> blocks); };
+    a.blocks = 3;
+    while (a.blocks && count(a.blocks) * A.H < A.cus && columns >= 16 << (4 - a.blocks)) a.blocks--;
+    // The grid is a few blocks of threads for each CU, which take what there is in turn.
+    const long long most = count(a.blocks);
     int items = (int)(most < (1ll << 30) ? most : 1ll << 30);
     const int wide = (4 * A.cus + A.H - 1) / A.H;
     const bool direct = dtype != SP_DTYPE_F32 && (uintptr_t)A.q % 16 == 0 && A.q_stride % 8 == 0;
-    const void *f = dtype == SP_DTYPE_F32 ? (const void *)k_fp4_weigh<HD, SP_DTYPE_F32, false>
-                  : dtype == SP_DTYPE_F16 ? (direct ? (const void *)k_fp4_weigh<HD, SP_DTYPE_F16, true> : (const void *)k_fp4_weigh<HD, SP_DTYPE_F16, false>)
-                                          : (direct ? (const void *)k_fp4_weigh<HD, SP_DTYPE_BF16, true> : (const void *)k_fp4_weigh<HD, SP_DTYPE_BF16, false>);
-    void *args[] = {const_cast<SpFp4Weigh *>(&A), &items};
+    const auto pick = [&](auto whole, auto shared) { return a.blocks < 3 ? (const void *)shared : (const void *)whole; };
+    const void *f = dtype == SP_DTYPE_F32 ? pick(k_fp4_weigh<HD, SP_DTYPE_F32, false, false>, k_fp4_weigh<HD, SP_DTYPE_F32, false, true>)
+                  : dtype == SP_DTYPE_F16 ? (direct ? pick(k_fp4_weigh<HD, SP_DTYPE_F16, true, false>, k_fp4_weigh<HD, SP_DTYPE_F16, true, true>)
+                                                    : (const void *)k_fp4_weigh<HD, SP_DTYPE_F16, false, true>)
+                                          : (direct ? pick(k_fp4_weigh<HD, SP_DTYPE_BF16, true, false>, k_fp4_weigh<HD, SP_DTYPE_BF16, true, true>)
+                                                    : (const void *)k_fp4_weigh<HD, SP_DTYPE_BF16, false, true>);
+    void *args[] = {&a, &items};
     return hipLaunchKernel(f, dim3((unsigned)(items < wide ? items : wide), (unsigned)A.H), dim3(WN), args, 0, s);
 }
 

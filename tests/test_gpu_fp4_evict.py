@@ -74,6 +74,19 @@ def test_weigh_more_columns_than_a_stage(hd, dtype, pad):
     P.check_weigh(dtype, queries(rng, P, 10, dtype), 0.1, pad=pad)
 
 
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_weigh_with_every_cu(hd, dtype):
+    """Tables so wide that no columns are shared out."""
+    rng = np.random.default_rng(hd)
+    P = Pair(hd, 32, 8)
+    lens = [300, 70]
+    table = [list(t) + [-1] * (70 - len(t)) for t in tables(rng, lens, 8)]
+    P.fill(rng, table, lens, dtype)
+    P.batch(table, lens, [0, 45, 46], 47)
+    P.check_weigh(dtype, queries(rng, P, 96, dtype), 0.1)
+
+
 def test_weigh_many_sequences_and_holes():
     rng = np.random.default_rng(3)
     P = Pair(64, 1, 320)
