@@ -1,6 +1,7 @@
 // sp_block_attn.h -- attention over a cache in blocks of 64 positions, for one or more query tokens
 // per sequence. A format F (sp_fp8_attn.hip, sp_fp4_attn.hip) says how a block is held: where its
-// codes and exponents are, and how they become operands of the matrix instructions.
+// codes and exponents are, and how they become operands of the matrix instructions. Figures here are of
+// the 8-bit cache; those of the 4-bit one stand in sp_fp4_attn.hip.
 //
 // For the row of query head n at position p of its sequence, over the positions t <= p (and
 // t > p - window), with k_t = 2^ek(t) K_t and v_t = 2^ev(t) V_t the block's codes and scales:
@@ -1095,11 +1096,12 @@ inline long long few_groups(const SpFp8Attn &A, int cols) {
     return A.s.row ? ((long long)A.s.n_rows * A.G) / cols + A.s.n_seq : (long long)A.s.n_seq * ((A.G + cols - 1) / cols);
 }
 
+// per_cu: shares that are made for each CU; 2 with 16 columns at most (the partial results that there is room for).
 template <class F, int HD, int DT, int NW, int CG>
-hipError_t launch(const SpFp8Attn &A, hipStream_t s) {
+hipError_t launch(const SpFp8Attn &A, hipStream_t s, int per_cu = 1) {
     constexpr int COLS = 16 * CG;
     SpFp8Attn a = A;
-    a.target = min(A.target, 256);
+    a.target = min(A.target, 256) * per_cu;
     const long long groups = few_groups(A, COLS);
     // shares: one per group, and at most target more over all KV heads
     const long long blocks = (groups + (a.target + A.H - 1) / A.H) * A.H;
