@@ -17,6 +17,7 @@
 // turn puts side by side.
 #pragma once
 
+#include "../../include/sp_hip_fp4.h"
 #include "sp_fp8.h"
 
 #define SP_FP4_MAX 6.0f

@@ -676,7 +676,7 @@ __global__ __launch_bounds__(NT) void k_fp4_move(SpFp4Evict A) {
             if (with_exp) e[k] = exp_plane[from * exps + sp_fp4_place(p[k] & 63)];
             if (with_weight) weight[k] = A.weight[from * 64 + (p[k] & 63)];
         }
-        // what this round loads is in registers before any of it is stored over
+        // what the loop has loaded is in registers before any of it is stored over
         __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
 #pragma unroll

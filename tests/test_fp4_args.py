@@ -1,6 +1,7 @@
 """The 4-bit block cache's refusals: what the host can see is refused before anything is
 launched, with a reason (no GPU: a cache whose memory is never touched)."""
 import ctypes as C
+import subprocess
 
 import numpy as np
 import pytest
@@ -160,3 +161,11 @@ def test_reference_eviction():
     assert max(w[p] for p in gone) <= low
     assert max(p for p in inner if w[p] == low) < min([p for p in gone if w[p] == low], default=999)
     assert c.codes[0, 0, 1, 0, 4, 0] == kept[4] % 16
+
+
+@pytest.mark.parametrize("compiler,ext", [("gcc", "c"), ("g++", "cpp")])
+def test_the_header_stands_alone(tmp_path, compiler, ext):
+    f = tmp_path / f"t.{ext}"
+    f.write_text('#include "sp_hip_fp4.h"\nint main(void){sp_hip_fp4_cache_t c; sp_hip_fp4_cache_free(&c); return SP_FP4_BLOCK;}\n')
+    r = subprocess.run([compiler, "-fsyntax-only", "-Wall", "-Werror", "-I", S.INCLUDE_DIR, str(f)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
