@@ -153,7 +153,8 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
     if (__any(bad)) return false;  // the grid was made for rows that ascend
     T = wave_sum(T) * (float)A.H;
     int alone;
-    const int R0 = first_share(A, T, T / fmaxf(wave_sum(groups) * (float)A.H, 1.0f), least, alone);
+    const float mean = T / fmaxf(wave_sum(groups) * (float)A.H, 1.0f);
+    const int R0 = first_share(A, T, mean, least, alone);
     float n[3] = {0.0f, 0.0f, 0.0f};
     for (int i0 = 0; i0 < n_seq; i0 += 64) {
         const Extent e = i0 ? extent(A, i0 + lane, cols) : e0;
@@ -164,6 +165,44 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
 #pragma unroll
     for (int k = 2; k >= 0; k--)
         if (wave_sum(n[k]) * (float)A.H <= (float)A.target) R = R0 + k * R0 / 4;
+    // The shares of sequence i0 + l begin at `from` of the items, their partial results at `slot`.
+    const auto found = [&](const Extent &e, int i0, int l, int ns, int from, int slot) {
+        const auto of = [l](int v) { return __builtin_amdgcn_readlane(v, l); };
+        out.seq = i0 + l;
+        out.r0 = of(e.a);
+        out.n_new = of(e.b) - out.r0;
+        out.first = of(e.len) - out.n_new;
+        out.n_split = of(ns);
+        const int at = (item - of(from)) * (by_group ? out.n_split : 1);
+        // the last column group first: under the causal mask it sees most
+        out.ct = of(e.ct) - 1 - at / out.n_split;
+        out.split = at % out.n_split;
+        out.slot = of(slot) + at;
+    };
+    if (A.per_cu == 2 && !by_group && n_seq <= 64 && __any((float)e0.nb > mean + 0.25f * (float)n_seq)) {
+        // Two blocks of threads a CU of unequal length: the longest shares first, and if all run at once, the shortest
+        // beside them. 16 sequences of 1 to 4K of 32 heads of 96 take 43 us, in their own order 51, and 45 with the
+        // second half as the first; 128 sequences of 8 heads of 128 take 80, 93 and (turned) 89. To find the order costs 0.06 us
+        // a sequence, and a block's difference in length a quarter of one: 64 sequences of up to 600 positions would take
+        // 18.4 us for 15.3.
+        const int ns = shares_of(e0.nb, R, alone), mine = e0.ct * ns;
+        const unsigned each = (unsigned)(e0.nb + ns - 1) / ns * 64 + 63 - lane;  // blocks of a share; no two alike
+        const int part = ns > 1 ? mine : 0, slot = sp_fp8_scan(part, lane) - part;
+        int from = 0, all = 0;
+        for (int j0 = 0; j0 < n_seq; j0 += 8)  // (those past the last have no items)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const unsigned each_j = __builtin_amdgcn_readlane(each, j0 + j);
+                const int mine_j = __builtin_amdgcn_readlane(mine, j0 + j);
+                from += each_j > each ? mine_j : 0;
+                all += mine_j;
+            }
+        if (item >= all) return false;
+        const int round = A.target / 2 / A.H;
+        if (all <= 2 * round && item >= round) item = all - 1 - (item - round);
+        found(e0, 0, __ffsll(__ballot(item >= from && item < from + mine)) - 1, ns, from, slot);
+        return true;
+    }
     int slots = 0;
     for (int i0 = 0; i0 < n_seq; i0 += 64) {
         const Extent e = i0 ? extent(A, i0 + lane, cols) : e0;
@@ -171,18 +210,7 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
         const int part = ns > 1 ? e.ct * ns : 0, psum = sp_fp8_scan(part, lane);
         const unsigned long long past = __ballot(sum > item);
         if (past) {
-            const int l = __ffsll(past) - 1;
-            const auto of = [l](int v) { return __builtin_amdgcn_readlane(v, l); };
-            out.seq = i0 + l;
-            out.r0 = of(e.a);
-            out.n_new = of(e.b) - out.r0;
-            out.first = of(e.len) - out.n_new;
-            out.n_split = of(ns);
-            const int at = (item - (of(sum) - of(mine))) * (by_group ? out.n_split : 1);
-            // the last column group first: under the causal mask it sees most
-            out.ct = of(e.ct) - 1 - at / out.n_split;
-            out.split = at % out.n_split;
-            out.slot = slots + of(psum) - of(part) + at;
+            found(e, i0, __ffsll(past) - 1, ns, sum - mine, slots + psum - part);
             return true;
         }
         item -= __builtin_amdgcn_readlane(sum, 63);
@@ -1102,6 +1130,7 @@ hipError_t launch(const SpFp8Attn &A, hipStream_t s, int per_cu = 1) {
     constexpr int COLS = 16 * CG;
     SpFp8Attn a = A;
     a.target = min(A.target, 256) * per_cu;
+    a.per_cu = per_cu;
     const long long groups = few_groups(A, COLS);
     // shares: one per group, and at most target more over all KV heads
     const long long blocks = (groups + (a.target + A.H - 1) / A.H) * A.H;

@@ -11,7 +11,7 @@
 // permutation each. Few rows are then bound by the vector unit as much as by memory: one sequence of 32768 positions of 8 heads
 // of 128 (36 MB) 17.8 us, where 256 blocks of threads hold two blocks a wave: 2 us to the first codes, 9.5 in the loop (5
 // of them issue vector instructions), 5 for the join of 32 shares; 16 sequences of 1 to 4K of 32 heads of 96, float32
-// rows (139 MB) 52 us, 2.7 TB/s; 12 of 1 to 4.5K with up to five rows (38 MB) 22.4 us. Half blocks (32 positions a wave
+// rows (139 MB) 45.4 us, 3.1 TB/s; 12 of 1 to 4.5K with up to five rows (38 MB) 22.4 us. Half blocks (32 positions a wave
 // at a time, 137 registers for 92 + 64) took 18.6, 65 and 25.5 us; the next block's codes two blocks ahead 19.0 for the
 // first; scaled matrix instructions, which take the codes as they are, sum 32 products with 15 bits.
 // Many rows differ by the conversion alone (LDS holds fp16 in both): 2048 rows over 32768 positions, 32 / 8 heads of
@@ -288,7 +288,8 @@ struct Fp4 {
 //   Sequences of few rows each leave most of its columns idle (EACH): 32 sequences of 16 rows of 16 heads take 53 and 31,
 //   of 32 heads 54 and 54, 16 of 64 rows of 32 heads 69 and 99; float32 rows 52 and 46, 56 and 82, 74 and 156.
 //   Few rows: past a group for each CU half the waves a block leave a CU two blocks out of step, and two shares a CU
-//   even out unequal lengths: 40 sequences of 1 to 4K 35 us, with one share a CU 51 (head_dim 256: 78 and 95). Decode at 4000
+//   even out unequal lengths, beside the order in which they are begun: 40 sequences of 1 to 4K 35 us, with one share a
+//   CU 51 (head_dim 256: 78 and 95). Decode at 4000
 //   positions of 32 / 40 / 64 sequences takes 41 / 56 / 59 with four waves and 33 / 58 / 64 with eight, at 600 positions
 //   12.7 / 16.6 / 17.1 and 12.5 / 19.5 / 21.4. With two column groups a wave eight stay ahead (64 sequences of 5 rows of
 //   32 heads 85, with four 116).

@@ -65,13 +65,14 @@ struct SpFp8Attn {
     int target;     // CUs; the launch makes it the blocks that fill them
     int least;      // fewest cache blocks of a share (the launch's choice)
     float join;     // rounds in which a block of threads joins shares (the launch's)
+    int per_cu;     // target counts 2 shares a CU (the launch's choice); then the longest come first
 };
 
 hipError_t sp_fp8_launch_write(const SpFp8Copy &A, int hd, int dtype, hipStream_t s);
 hipError_t sp_fp8_launch_read(const SpFp8Copy &A, int hd, int dtype, hipStream_t s);
 hipError_t sp_fp8_launch_attn(const SpFp8Attn &A, int hd, int dtype, hipStream_t s);
-// Rows of partial results. Shares number at most 512 (twice 256 CUs): of 32 columns in the kernel
-// for few rows, of at most 256 (128 at head_dim 256) in the one for many, which only prefill calls use.
+// Rows of partial results. Shares number at most 512 (twice 256 CUs), of 32 columns in the kernel
+// for few rows (or 1024 of 16), of at most 256 (128 at head_dim 256) in the one for many, which only prefill calls use.
 #define SP_FP8_DECODE_ROWS (512 * 32)
 inline int sp_fp8_prefill_rows(int hd) { return 512 * (hd == 256 ? 128 : 256); }
 

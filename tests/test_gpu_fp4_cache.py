@@ -287,6 +287,27 @@ def test_more_column_groups_than_cus(hd, dtype):
     P.check_attend(dtype, queries(rng, P, 192, dtype), 0.1)
 
 
+@pytest.mark.parametrize("n_seq", [12, 20, 63])
+@pytest.mark.parametrize("hd,dtype", [(64, "f16"), (128, "f32"), (256, "bf16")])
+def test_unequal_lengths_past_the_cus(n_seq, hd, dtype):
+    """The longest first: some empty, several alike, and few rows of each besides."""
+    rng = np.random.default_rng(n_seq)
+    H = 32 if n_seq < 60 else 8
+    P = Pair(hd, H, 240)
+    lens = [(0, 1, 64, 65, 130)[i % 5] for i in range(n_seq)]
+    lens[n_seq // 2], lens[-1], lens[3] = 2300, 1200, 1200
+    if n_seq > 60:
+        lens = [min(n, 65) if i % 2 else n for i, n in enumerate(lens)]
+        lens[1] = 2300
+    table = tables(rng, lens, 240)
+    P.fill(rng, table, lens, dtype)
+    P.batch(table, lens)
+    P.check_attend(dtype, queries(rng, P, H * (4 if H == 8 else 1), dtype), 0.1)
+    rows = [min(n, 2) for n in lens]
+    P.batch(table, lens, np.concatenate([[0], np.cumsum(rows)]).tolist(), sum(rows) + 1)
+    P.check_attend(dtype, queries(rng, P, H * 3, dtype), 0.1)
+
+
 def test_tables_with_holes():
     rng = np.random.default_rng(1)
     for hd in (64, 128, 256):
