@@ -12,7 +12,7 @@
 // of 128 (36 MB) 17.8 us, where 256 blocks of threads hold two blocks a wave: 2 us to the first codes, 9.5 in the loop (5
 // of them issue vector instructions), 5 for the join of 32 shares; 16 sequences of 1 to 4K of 32 heads of 96, float32
 // rows (139 MB) 45.4 us, 3.1 TB/s; 12 of 1 to 4.5K with up to five rows (38 MB) 22.4 us. Half blocks (32 positions a wave
-// at a time, 137 registers for 92 + 64) took 18.6, 65 and 25.5 us; the next block's codes two blocks ahead 19.0 for the
+// at a time, 137 registers for 179) took 18.6, 65 and 25.5 us where whole ones took 17.8, 56 and 22.5; the next block's codes two blocks ahead 19.0 for the
 // first; scaled matrix instructions, which take the codes as they are, sum 32 products with 15 bits.
 // Many rows differ by the conversion alone (LDS holds fp16 in both): 2048 rows over 32768 positions, 32 / 8 heads of
 // 128, 880 to 905 us by card (1.18 to 1.21 PFLOP/s; the 8-bit cache 887 to 904); 2048 rows in a window of 1024, 16 / 8 heads of
