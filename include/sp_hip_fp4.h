@@ -64,8 +64,8 @@ int  sp_hip_fp4_attn_prefill(const sp_hip_fp4_cache_t *c, int layer, const sp_hi
                              long long out_stride, float *d_lse, void *stream);
 
 /* Adds to d_weight, for each KV head and each position that the batch's rows see, the sum over the rows
- * and the KV head's query heads of exp(kq_scale * q . K - lse): with the arguments of an attention call
- * and the d_lse [n_rows][n_q] that it gave, its softmax weights. Any rows (d_row NULL or not), so a
+ * and the KV head's query heads of exp(kq_scale * q . K - lse), K as attention sees it: with the arguments
+ * of an attention call and the d_lse [n_rows][n_q] that it gave, its softmax weights. Any rows (d_row NULL or not), so a
  * prompt may be weighed by its last rows alone. A row and head whose lse or whose q is not finite
  * adds nothing. Needs no workspace: calls may overlap, but two that meet in a block, or a batch whose
  * sequences share one, add in no certain order (fp32 sums may differ in their last bits). */

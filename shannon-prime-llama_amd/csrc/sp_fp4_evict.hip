@@ -27,9 +27,10 @@ __device__ __forceinline__ float power(unsigned rel, int b) {
 // summed over columns in the registers that the scores come in, and over the 16 lanes at the end.
 //
 // Queries of 16-bit types are operands as they are, with K in their type: no maximum to look for, no
-// conversion. K counts relative to the block's largest exponent, for bf16 2^-12 of that, so that no
-// sum of finite queries passes a float. fp32 queries are scaled by a power of two and split in two
-// fp16 parts, as in attention.
+// conversion. K counts relative to the block's largest exponent and is what attention sees of it: an fp16 number. As
+// bf16 that is the same number wherever no exponent is more than 23 below the largest; of other blocks (empty
+// rows among them) the fp16 numbers are made first (see Operand). fp32 queries are scaled by a power of two and
+// split in two fp16 parts, as in attention.
 //
 // Bound for many columns by the matrix cores and the exponentials (for 64 positions of 16 columns 16 and 16
 // instructions of 16 and 8 cycles at head_dim 128, beside one multiplication and one addition a weight): 64 rows over 32768
@@ -50,6 +51,7 @@ struct Operand {
     typedef h8 V;
     static constexpr int DOWN = 0;
     static __device__ __forceinline__ V codes(unsigned w, float scale) { return eight(w, scale); }
+    static __device__ __forceinline__ V seen(unsigned w, float scale) { return eight(w, scale); }
     static __device__ __forceinline__ f4 mma(V a, V b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
@@ -60,6 +62,15 @@ struct Operand<SP_DTYPE_BF16> {
         const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1),
                    c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
         return b8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+    // Eight codes as attention sees them: multiples of 2^-24 of the block's largest scale. (At most two bits of an
+    // fp16 number that small are left, or the code's own: exact in bf16.)
+    static __device__ __forceinline__ V seen(unsigned w, float scale) {
+        const h8 x = eight(w, scale);
+        V v;
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = (__bf16)((float)x[k] * 0x1p-12f);
+        return v;
     }
     static __device__ __forceinline__ f4 mma(V a, V b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
@@ -223,11 +234,25 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
 #pragma unroll
             for (int c = 0; c < NC; c++) m.add(ks[c]);
             top = uniform(sp_fp4::row_max(m.get()));
+            unsigned near = 0x80808080u;  // a byte's highest bit: its exponents are at most 23 below
+            if constexpr (DT == SP_DTYPE_BF16) {
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                const unsigned rel = relative(ks[c], top + Op::DOWN);
+                for (int c = 0; c < NC; c++) near &= (relative(ks[c], top) | 0x80808080u) - (127 - 23) * 0x01010101u;
+            }
+            if (DT != SP_DTYPE_BF16 || __all(near == 0x80808080u)) {
 #pragma unroll
-                for (int n = 0; n < 4; n++) ka[c][n] = Op::codes(kr[c][n], power(rel, n));
+                for (int c = 0; c < NC; c++) {
+                    const unsigned rel = relative(ks[c], top + Op::DOWN);
+#pragma unroll
+                    for (int n = 0; n < 4; n++) ka[c][n] = Op::codes(kr[c][n], power(rel, n));
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const unsigned rel = relative(ks[c], top);
+#pragma unroll
+                    for (int n = 0; n < 4; n++) ka[c][n] = Op::seen(kr[c][n], power(rel, n));
+                }
             }
         }
         f4 acc[4];
