@@ -49,15 +49,24 @@ __device__ __forceinline__ void to_lds4(const void *from, void *to) { __builtin_
 template <int DT>
 struct Operand {
     typedef h8 V;
-    static constexpr int DOWN = 0;
+    // K counts in 2^-down(c, top) of the block's largest scale.
+    static __device__ __forceinline__ int down(float, int) { return 0; }
     static __device__ __forceinline__ V codes(unsigned w, float scale) { return eight(w, scale); }
-    static __device__ __forceinline__ V seen(unsigned w, float scale) { return eight(w, scale); }
+    static __device__ __forceinline__ V seen(unsigned w, float scale, int) { return eight(w, scale); }
     static __device__ __forceinline__ f4 mma(V a, V b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Operand<SP_DTYPE_BF16> {
     typedef b8 V;
-    static constexpr int DOWN = 12;
+    // bf16 queries may be as large or small as a float, where kq_scale makes up for it: a product of a query's entry
+    // and a K that counts relative to its block alone may leave a float's range though the score is ordinary. So K
+    // counts in 2^-60 of what it adds to a score in powers of two. Sums of finite queries stay finite (but
+    // where a score's terms pass 2^188), and what vanishes below a float is less than 2^-66 of a power of two. At most 2^-100
+    // of the block's scale, where the least that is seen is still a normal bf16 number (such terms vanish below 2^-66 too).
+    static __device__ __forceinline__ int down(float c, int top) {
+        const int unit = (__float_as_int(c) >> 23) - 127 + 1 + top - 127;  // of scores, in log2
+        return min(60 - unit, 100);
+    }
     static __device__ __forceinline__ V codes(unsigned w, float scale) {
         const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1),
                    c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3);
@@ -65,11 +74,12 @@ struct Operand<SP_DTYPE_BF16> {
     }
     // Eight codes as attention sees them: multiples of 2^-24 of the block's largest scale. (At most two bits of an
     // fp16 number that small are left, or the code's own: exact in bf16.)
-    static __device__ __forceinline__ V seen(unsigned w, float scale) {
+    static __device__ __forceinline__ V seen(unsigned w, float scale, int down) {
+        const float unit = sp_fp8_pow2(-down);
         const h8 x = eight(w, scale);
         V v;
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = (__bf16)((float)x[k] * 0x1p-12f);
+        for (int k = 0; k < 8; k++) v[k] = (__bf16)((float)x[k] * unit);
         return v;
     }
     static __device__ __forceinline__ f4 mma(V a, V b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -216,7 +226,7 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
             }
         };
         // ---- K of this wave's block, relative to its largest exponent, as in attention ----
-        int top;
+        int top, down;
         V ka[NC][4];
         {
             u4 kr[NC];
@@ -234,6 +244,7 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
 #pragma unroll
             for (int c = 0; c < NC; c++) m.add(ks[c]);
             top = uniform(sp_fp4::row_max(m.get()));
+            down = Op::down(A.c, top);
             unsigned near = 0x80808080u;  // a byte's highest bit: its exponents are at most 23 below
             if constexpr (DT == SP_DTYPE_BF16) {
 #pragma unroll
@@ -242,7 +253,7 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
             if (DT != SP_DTYPE_BF16 || __all(near == 0x80808080u)) {
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
-                    const unsigned rel = relative(ks[c], top + Op::DOWN);
+                    const unsigned rel = relative(ks[c], top + down);
 #pragma unroll
                     for (int n = 0; n < 4; n++) ka[c][n] = Op::codes(kr[c][n], power(rel, n));
                 }
@@ -251,7 +262,7 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
                 for (int c = 0; c < NC; c++) {
                     const unsigned rel = relative(ks[c], top);
 #pragma unroll
-                    for (int n = 0; n < 4; n++) ka[c][n] = Op::seen(kr[c][n], power(rel, n));
+                    for (int n = 0; n < 4; n++) ka[c][n] = Op::seen(kr[c][n], power(rel, n), down);
                 }
             }
         }
@@ -261,7 +272,7 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
         // whether every column sees all of this block: nothing then depends on a column's position
         const bool all = t * 64 + 63 <= first && (A.window <= 0 || t * 64 > first + n_new - 1 - A.window);
         const auto units = [&](int qe) {  // of the scores, times log2 e
-            const float up = fminf(__builtin_amdgcn_ldexpf(A.c, qe + top + Op::DOWN - 127), 0x1.fffffep127f);
+            const float up = fminf(__builtin_amdgcn_ldexpf(A.c, qe + top + down - 127), 0x1.fffffep127f);
             return A.negate ? -up : up;
         };
         const float cs1 = units(1);
@@ -306,7 +317,7 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
                 if constexpr (DIRECT) {
                     lse = lse_of[buf * CS + y * 16 + r];
                     lse = n0 + r < n_cols && fabsf(lse) < INFINITY ? lse : INFINITY;
-                    // a query that is not finite has no finite score: one of them tells (finite ones have: see above)
+                    // a query that is not finite has no finite score: one of them tells (finite ones have: see Operand)
                     const bool odd = !(fabsf(s[0][0]) < INFINITY);
                     if (__any(odd)) {
                         lse = odd ? INFINITY : lse;

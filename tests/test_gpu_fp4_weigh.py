@@ -58,3 +58,57 @@ def test_weigh_of_scales_far_apart(hd, dtype):
         P.check_weigh(dtype, q, 2.0 ** 21)
     diff = np.abs(P.ref.stored(0, 0, 0) - P.ref.values(0, 0, 0))
     assert diff.max() > 0  # (what attention sees is not what the codes say)
+
+
+# ---- queries and kq_scale of any size ----
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("qe,ke", [(-118, 0), (-118, 20), (-60, 0), (-60, 20), (-60, -20), (60, 0), (60, 20), (60, -20),
+                                   (120, 0), (120, -20)])
+def test_weigh_of_queries_of_any_size(qe, ke, dtype):
+    """Scores near 1 from queries of 2^qe, keys of 2^ke and the kq_scale that makes up for them."""
+    se = -qe - ke - 2
+    rng = np.random.default_rng(qe + 200 + ke)
+    for hd in (64, 128):
+        P = Pair(hd, 1, 6)
+        P.batch(tables(rng, [300], 6), [300], [0, 30])
+        fill_device(rng, P)
+        set_exponents(P, 0, (P.ref.exps[0].astype(int) + ke).astype(np.uint8))
+        for n_q in (4, 1):
+            q = torch.from_numpy(rng.standard_normal((30, n_q, hd)).clip(-3, 3)).to(TORCH[dtype])
+            P.check_weigh(dtype, q * 2.0 ** qe, 2.0 ** se)
+            P.check_weigh(dtype, q * 2.0 ** qe, -(2.0 ** se), window=70)
+
+
+def test_weigh_of_the_largest_queries():
+    """bf16 queries next to the largest number, against keys next to theirs: sums that stay within a float."""
+    rng = np.random.default_rng(5)
+    for hd in (64, 256):
+        P = Pair(hd, 1, 4)
+        P.batch(tables(rng, [200], 4), [200], [0, 20])
+        fill_device(rng, P)
+        P.ref.codes[0] = rng.choice([7, 15], P.ref.codes[0].shape)  # 6 and -6
+        copy(P.dev.c.d_k_codes, torch.from_numpy(np.ascontiguousarray(P.ref.code_bytes(0))).cuda())
+        set_exponents(P, 0, np.full_like(P.ref.exps[0], 127))
+        q = torch.full((20, 2, hd), torch.finfo(torch.bfloat16).max, dtype=torch.bfloat16)
+        q[:, 1] *= torch.from_numpy(rng.choice([-1.0, 1.0], (20, hd))).bfloat16()
+        P.check_weigh("bf16", q, 2.0 ** -133)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_weigh_of_large_scores_beside_each_other(dtype):
+    """Scores past 2^12 with many positions within a few units of the largest: channel 0 lifts all of a row's
+    scores, the others tell them apart. Both are whole numbers times ln 2, exact in fp32."""
+    rng = np.random.default_rng(8)
+    P = Pair(64, 1, 6)
+    P.batch(tables(rng, [320], 6), [320], [0, 320])
+    k = np.zeros((320, 1, 64))
+    k[:, 0, 0] = 6.0
+    k[:, 0, 32:36] = rng.integers(-1, 2, (320, 4))
+    P.write("f32", torch.from_numpy(k).float(), torch.from_numpy(k).float())
+    P.batch(P.table, [320], [0, 50])
+    q = np.zeros((50, 4, 64))
+    q[..., 0] = rng.integers(128, 240, (50, 4)) * 8
+    q[..., 32:36] = 1.0
+    added = P.check_weigh(dtype, torch.from_numpy(q).to(TORCH[dtype]), float(np.float32(math.log(2))))
+    assert abs(added.sum() - 200) < 1.0 and (added > 0).sum() > 100
