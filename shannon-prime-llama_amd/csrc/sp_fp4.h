@@ -23,6 +23,7 @@
 #define SP_FP4_MAX 6.0f
 #define SP_FP4_EVICT_THREADS 1024  // of a block of eviction's kernels
 #define SP_FP4_LEAST (127 + SP_FP8_EMIN)  // exponent byte of what no row was written to
+#define SP_FP4_MOST (127 + SP_FP8_EMAX)   // and the largest
 
 __host__ __device__ constexpr int sp_fp4_tile(int hd) { return 32 * hd; }  // bytes of codes
 __host__ __device__ constexpr int sp_fp4_exps(int hd) { return 2 * hd; }   // and of exponents

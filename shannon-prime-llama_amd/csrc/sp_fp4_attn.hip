@@ -194,8 +194,10 @@ struct Fp4 {
                 }
             }
             lds_barrier();
-            ekb = area[lane] & 255;
-            evb = area[lane] >> 8;
+            // A block that is missing is masked, and what is staged in its place (block 0, which another stream may be writing)
+            // meets weights of 0: relative to the largest exponent there is it is finite whatever it is.
+            ekb = blk < 0 ? SP_FP4_MOST : area[lane] & 255;
+            evb = blk < 0 ? SP_FP4_MOST : area[lane] >> 8;
         }
         static __device__ __forceinline__ void fetch_k(const SpFp8Side &S, long long tile, int st, Raw &raw) {
             const uint8_t *p = S.codes + tile * sp_fp4_tile(HD), *e = S.exps + tile * sp_fp4_exps(HD);
