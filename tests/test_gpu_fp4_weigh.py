@@ -112,3 +112,85 @@ def test_weigh_of_large_scores_beside_each_other(dtype):
     q[..., 32:36] = 1.0
     added = P.check_weigh(dtype, torch.from_numpy(q).to(TORCH[dtype]), float(np.float32(math.log(2))))
     assert abs(added.sum() - 200) < 1.0 and (added > 0).sum() > 100
+
+
+# ---- more items than the grid has blocks of threads ----
+
+def weigh64(P, q, scale, lse, window):
+    """fp4_ref.RefCache.weigh, a sequence at a time."""
+    w, tol = np.zeros_like(P.ref.weight), np.zeros_like(P.ref.weight)
+    group = q.shape[1] // P.heads
+    split = 2.0 ** -22 if q.dtype == torch.float32 else 0.0
+    x = q.double().numpy()
+    for i, n in enumerate(P.lens):
+        r0, r1 = P.row[i], P.row[i + 1]
+        p = n - r1 + np.arange(r0, r1)
+        for j, b in enumerate(P.table[i]):
+            if not 0 <= b < P.n_blocks or j * 64 >= n or r1 == r0:
+                continue
+            K, pos = P.ref.values(0, 0, b), j * 64 + np.arange(64)
+            see = pos[None] <= p[:, None]
+            if window:
+                see &= pos[None] > p[:, None] - window
+            for h in range(P.heads):
+                qh, lh = x[r0:r1, h * group:(h + 1) * group], lse[r0:r1, h * group:(h + 1) * group, None]
+                fine = (np.isfinite(lh) & np.isfinite(qh).all(-1, keepdims=True) & see[:, None]).astype(bool)
+                qh, lh = np.where(np.isfinite(qh), qh, 0.0), np.where(np.isfinite(lh), lh, 0.0)
+                d, steep = qh @ K[h].T * scale - lh, np.abs(qh) @ np.abs(K[h]).T * abs(scale)
+                add = np.where(fine, np.exp(np.where(fine, d, 0.0)), 0.0)
+                off = steep * ((P.hd + 4) * 2.0 ** -24 + split) + np.abs(d) * 3 * 2.0 ** -24 + 2.0 ** -22
+                w[0, b, h] += add.sum((0, 1))
+                tol[0, b, h] += (add * (1.01 * off + (r1 - r0) * group * 2.0 ** -24) + fine * 2.0 ** -126).sum((0, 1))
+    return w, tol
+
+
+def check64(P, dtype, q, scale, window=0, pad=0, shift=0, lse=None):
+    if lse is None:
+        _, lse = P.attend(dtype, q, scale, window)
+    before = P.weights()
+    P.weigh(dtype, q, scale, lse, window, pad=pad, shift=shift)
+    want, tol = weigh64(P, q, float(np.float32(scale)), np.asarray(lse, np.float64), window)
+    tol += (tol > 0) * np.abs(before + want) * 2.0 ** -23
+    d = np.abs(P.weights() - before - want)
+    assert (d <= tol).all(), (float((d - tol).max()), float(d.max()))
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype,pad", [("f32", 0), ("f32", 1), ("f16", 0), ("bf16", 0), ("f16", 3), ("bf16", 4)])
+def test_weigh_second_items(hd, dtype, pad):
+    """32 heads leave 32 blocks of threads a head; these sequences have 60 items, of one, two and three
+    stages of columns, some of blocks that the table lacks, so that each block of threads goes on to others."""
+    rng = np.random.default_rng(hd + pad)
+    lens = [1290 - 37 * i for i in range(20)]
+    rows = [(i * 29) % 13 for i in range(20)]
+    rows[3], rows[4], rows[11], rows[17] = 150, 290, 129, 64
+    P = Pair(hd, 32, 330)
+    table = tables(rng, lens, 330)
+    table[4][2], table[9][0], table[19][-1] = -1, 9999, -7
+    P.batch(table, lens, np.concatenate([[0], np.cumsum(rows)]).tolist(), sum(rows) + 3)
+    fill_device(rng, P)
+    q = queries(rng, P, 32, dtype)
+    check64(P, dtype, q, 0.1, pad=pad)
+    check64(P, dtype, q, 0.1, window=100, pad=pad)
+
+
+# ---- rows that are not finite ----
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+@pytest.mark.parametrize("dtype,pad,shift", [("f32", 0, 0), ("f32", 3, 1), ("f16", 0, 0), ("f16", 4, 4), ("f16", 3, 1),
+                                             ("bf16", 0, 0), ("bf16", 5, 0)])
+def test_weigh_passes_over_what_is_not_finite_in_every_form(hd, dtype, pad, shift):
+    rng = np.random.default_rng(hd)
+    for heads, lens, rows in ((2, [300, 200], [20, 20]), (32, [700] * 5, [9, 0, 30, 1, 5])):
+        P = Pair(hd, heads, 64)
+        P.batch(tables(rng, lens, 64), lens, np.concatenate([[0], np.cumsum(rows)]).tolist())
+        fill_device(rng, P)
+        q = queries(rng, P, 2 * heads, dtype)
+        _, lse = P.attend(dtype, q, 0.2)
+        for r, n, d, x in ((5, 1, 3, math.nan), (31, 0, 0, math.inf), (32, 1, hd - 1, -math.inf), (8, 2 * heads - 1, 32, math.nan),
+                           (8, 2 * heads - 2, hd - 1, math.inf)):
+            q[r, n, d] = x
+        q[33, 3, 1], q[33, 3, 2] = math.inf, -math.inf
+        lse[7, 2], lse[8, 0], lse[9, 3] = np.nan, np.inf, -np.inf
+        check64(P, dtype, q, 0.2, pad=pad, shift=shift, lse=lse)
+        assert np.isfinite(P.weights()).all()
