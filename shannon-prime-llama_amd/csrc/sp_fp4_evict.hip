@@ -114,7 +114,6 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
     __shared__ float lse_of[DIRECT ? 2 * CS : 1];
     const int tid = threadIdx.x, lane = tid & 63, w = uniform(tid >> 6);
     const int h = blockIdx.y, r = lane & 15, g = lane >> 4;
-    const bool aligned = (uintptr_t)A.q % sizeof(T8) == 0 && A.q_stride % 8 == 0;
     const int two = SHARED ? A.blocks : 3;
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
         // ---- the sequence, and 2^two blocks of those that its rows see ----
@@ -144,7 +143,8 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
         const int t = j0 + (w & ((1 << two) - 1)), n_cols = n_new * A.G;
         const int blk = uniform(t <= (first + n_new - 1) >> 6 ? sp_fp8_block(A.s, seq, t) : -1);
         const long long tile = (long long)max(blk, 0) * A.H + h;
-        // ---- columns: this thread's eight entries of some, into LDS ----
+        // ---- columns: this thread's eight entries of some, into LDS (staged: one by one, which takes no longer
+        // than in vectors of four: 64 rows over 32768 positions, 32 / 8 heads of 128, 54.7 and 55.3 us with float32 rows) ----
         const auto direct = [&](int c0, int buf) __attribute__((always_inline)) {
             const int here = min(n_cols - c0, CS);
             for (int f = w; f < (here + 15) / 16 * NC; f += NW) {  // fragments: 16 columns, 32 channels
@@ -172,12 +172,8 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
                 lse[y] = A.lse[(long long)row * A.H * A.G + head];
                 if (part >= HD / 8) continue;
                 const T *src = reinterpret_cast<const T *>(A.q) + (long long)row * A.q_stride + (long long)head * HD + part * 8;
-                if (aligned) {
-                    raw[y] = *reinterpret_cast<const T8 *>(src);
-                } else {
 #pragma unroll
-                    for (int k = 0; k < 8; k++) raw[y][k] = src[k];
-                }
+                for (int k = 0; k < 8; k++) raw[y][k] = src[k];
             }
 #pragma unroll
             for (int y = 0; y < PER; y++) {
@@ -391,6 +387,9 @@ hipError_t launch_weigh(const SpFp4Weigh &A, int dtype, hipStream_t s) {
     const auto count = [&](int blocks) { return (long long)A.s.n_seq * ((seen + (1 << blocks) - 1) >> blocks); };
     a.blocks = 3;
     while (a.blocks && count(a.blocks) * A.H < A.cus && columns >= 16 << (4 - a.blocks)) a.blocks--;
+    // 16-bit rows that cannot go straight into LDS take the shared form always. With eight blocks the other one is ahead in
+    // steps (12 sequences of 1 to 4.5K, head_dim 64 / 96 / 128 / 256: 9.5 / 11.2 / 13.8 / 17.9 us for 10.0 / 14.7 / 15.5 / 19.3)
+    // and behind with more columns (64 rows over 32768: 22.8 / 28.8 / 42.5 / 63 for 23.5 / 39 / 40.5 / 59.5).
     // The grid is a few blocks of threads for each CU, which take what there is in turn.
     const long long most = count(a.blocks);
     int items = (int)(most < (1ll << 30) ? most : 1ll << 30);

@@ -194,3 +194,22 @@ def test_weigh_passes_over_what_is_not_finite_in_every_form(hd, dtype, pad, shif
         lse[7, 2], lse[8, 0], lse[9, 3] = np.nan, np.inf, -np.inf
         check64(P, dtype, q, 0.2, pad=pad, shift=shift, lse=lse)
         assert np.isfinite(P.weights()).all()
+
+
+# ---- rows at any address ----
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 256])
+def test_weigh_of_rows_at_any_address(hd):
+    """float32 rows at every multiple of their element's size: the same bits."""
+    rng = np.random.default_rng(hd)
+    P = Pair(hd, 2, 12)
+    P.batch(tables(rng, [300, 200], 12), [300, 200], [0, 40, 45])
+    fill_device(rng, P)
+    q = queries(rng, P, 8, "f32")
+    _, lse = P.attend("f32", q, 0.1)
+    got = []
+    for shift, pad in ((0, 0), (4, 0), (4, 4), (2, 6), (1, 0), (0, 1), (3, 5)):
+        P.set_weights(np.zeros(P.ref.weight.shape))
+        P.weigh("f32", q, 0.1, lse, pad=pad, shift=shift)
+        got.append(P.weights())
+    assert all(np.array_equal(x, got[0]) for x in got[1:])
