@@ -55,7 +55,10 @@ int  sp_hip_fp4_read(const sp_hip_fp4_cache_t *c, int layer, const sp_hip_fp4_ba
                      long long row_stride, int dtype, void *stream);
 
 /* As sp_hip_fp8_attn_decode and _prefill. Of a block's keys, and of its values, nothing finer
- * than 2^-25 of the largest scale that the block holds for the KV head is seen. */
+ * than 2^-25 of the largest scale that the block holds for the KV head is seen (a row that has been taken
+ * back counts there until it is written over). Rows are written alone, but no call may write into a block
+ * that an attention or weigh call under way reads. Which kernel serves a call goes by table_stride, which
+ * stands for the length: tables much wider than their sequences make prompts of 100 to 300 rows slower. */
 int  sp_hip_fp4_attn_decode(const sp_hip_fp4_cache_t *c, int layer, const sp_hip_fp4_batch_t *batch, const void *d_q,
                             long long q_stride, int n_q, int dtype, float kq_scale, int window, void *d_out,
                             long long out_stride, float *d_lse, void *stream);
@@ -65,8 +68,10 @@ int  sp_hip_fp4_attn_prefill(const sp_hip_fp4_cache_t *c, int layer, const sp_hi
 
 /* Adds to d_weight, for each KV head and each position that the batch's rows see, the sum over the rows
  * and the KV head's query heads of exp(kq_scale * q . K - lse), K as attention sees it: with the arguments
- * of an attention call and the d_lse [n_rows][n_q] that it gave, its softmax weights. Any rows (d_row NULL or not), so a
- * prompt may be weighed by its last rows alone. A row and head whose lse or whose q is not finite
+ * of an attention call and the d_lse [n_rows][n_q] that it gave, its softmax weights. (A 16-bit query counts
+ * whole, where attention sees nothing finer than 2^-39 of a row's largest entry; and d_lse is fp32, so that
+ * scores near 2^n put a weight off by a factor of up to about e^(2^(n - 22)).) Any rows (d_row NULL or not),
+ * so a prompt may be weighed by its last rows alone. A row and head whose lse or whose q is not finite
  * adds nothing. Needs no workspace: calls may overlap, but two that meet in a block, or a batch whose
  * sequences share one, add in no certain order (fp32 sums may differ in their last bits). */
 int  sp_hip_fp4_weigh(sp_hip_fp4_cache_t *c, int layer, const sp_hip_fp4_batch_t *batch, const void *d_q,
@@ -79,11 +84,12 @@ int  sp_hip_fp4_weigh(sp_hip_fp4_cache_t *c, int layer, const sp_hip_fp4_batch_t
  * moved, with their weights, into positions 0 .. keep - 1 of the sequence's table row; from there on
  * the sequence's length is keep, and blocks past that are the caller's again. Nothing is rounded.
  * d_kept [n_seq][n_heads_kv][keep] int32 gets the old position of each (a sequence of n <= keep is left as
- * it is and gets 0 .. n - 1, then -1). A position of an attention call is then its place, so a window
- * counts kept positions, and keys should carry their rotation already. A sequence with a table entry
- * missing in its length is left as it is and gets -1. d_len is not changed, d_row is not read
- * (n_rows = n_seq without it). No other call may use the sequences' blocks meanwhile, and no block
- * is theirs twice. */
+ * it is, whatever its table holds, and gets 0 .. n - 1, then -1). A position of an attention call is then
+ * its place, so a window counts kept positions, and keys should carry their rotation already. A longer
+ * sequence with a table entry missing in its length is left as it is and gets -1. d_len is not changed,
+ * d_row is not read (n_rows = n_seq without it). No other call may use the sequences' blocks meanwhile,
+ * and no block is theirs twice or another sequence's too (a shared prefix would be moved under it;
+ * nothing checks this). */
 int  sp_hip_fp4_evict(sp_hip_fp4_cache_t *c, int layer, const sp_hip_fp4_batch_t *batch, int keep, int first, int recent,
                       int32_t *d_kept, void *stream);
 

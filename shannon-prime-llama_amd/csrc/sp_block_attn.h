@@ -181,10 +181,10 @@ __device__ __forceinline__ bool find_share(const SpFp8Attn &A, int item, int lan
     };
     if (A.per_cu == 2 && !by_group && n_seq <= 64 && __any((float)e0.nb > mean + 0.25f * (float)n_seq)) {
         // Two blocks of threads a CU of unequal length: the longest shares first, and if all run at once, the shortest
-        // beside them. 16 sequences of 1 to 4K of 32 heads of 96 take 43 us, in their own order 51, and 45 with the
-        // second half as the first; 128 sequences of 8 heads of 128 take 80, 93 and (turned) 89. To find the order costs 0.06 us
-        // a sequence, and a block's difference in length a quarter of one: 64 sequences of up to 600 positions would take
-        // 18.4 us for 15.3.
+        // beside them. 16 sequences of 1 to 4K of 32 heads of 96, float32 rows, take 45 us, in their own order 52. To find
+        // the order costs 0.06 us a sequence, and a block's difference in length a quarter of one: 64 sequences of up to 600
+        // positions would take 18.4 us for 15.3. One lane has one sequence: past 64 they come in their own order, also
+        // where another would be faster (128 sequences of 1 to 4K of 8 heads of 128 94 us, 81 if the caller has them longest first).
         const int ns = shares_of(e0.nb, R, alone), mine = e0.ct * ns;
         const unsigned each = (unsigned)(e0.nb + ns - 1) / ns * 64 + 63 - lane;  // blocks of a share; no two alike
         const int part = ns > 1 ? mine : 0, slot = sp_fp8_scan(part, lane) - part;
@@ -1014,7 +1014,7 @@ __global__ __launch_bounds__(NW * 64) void k_attn_wide(SpFp8Attn A) {
     // of lane values i .. i + 3 of row block d: channels from
     const auto channel = [&](int d, int i) { return d * CW + i * 2 + 4 * sub; };
     const float unit = sp_fp8_pow2(ev_now);
-    if (sh.n_split > 1) {  // joined by k_fp8_attn_join
+    if (sh.n_split > 1) {  // joined by k_attn_join
         const long long slot = (long long)sh.slot * A.H + h;
         if (active && slot_fits(A, slot, COLS)) {
             float *dst = A.part + (slot * COLS + mycol) * ROW;

@@ -12,7 +12,8 @@
 // of 128 (36 MB) 17.8 us, where 256 blocks of threads hold two blocks a wave: 2 us to the first codes, 9.5 in the loop (5
 // of them issue vector instructions), 5 for the join of 32 shares; 16 sequences of 1 to 4K of 32 heads of 96, float32
 // rows (139 MB) 45.4 us, 3.1 TB/s; 12 of 1 to 4.5K with up to five rows (38 MB) 22.4 us. Half blocks (32 positions a wave
-// at a time, 137 registers for 179) took 18.6, 65 and 25.5 us where whole ones took 17.8, 56 and 22.5; the next block's codes two blocks ahead 19.0 for the
+// at a time, 137 registers for 179) took 18.6, 65 and 25.5 us where whole ones took 17.8, 56 (that case now has two
+// shares a CU, the longest first) and 22.5; the next block's codes two blocks ahead 19.0 for the
 // first; scaled matrix instructions, which take the codes as they are, sum 32 products with 15 bits.
 // Many rows differ by the conversion alone (LDS holds fp16 in both): 2048 rows over 32768 positions, 32 / 8 heads of
 // 128, 880 to 905 us by card (1.18 to 1.21 PFLOP/s; the 8-bit cache 887 to 904); 2048 rows in a window of 1024, 16 / 8 heads of
@@ -287,6 +288,10 @@ struct Fp4 {
 //   slower start and its second launch, and half as many columns suffice: 128 rows over 4096 / 8192 / 16000 positions take
 //   34 / 43 / 57 and 30 / 44 / 71, with float32 rows 36 / 50 / 78 and 33 / 54 / 100, at head_dim 256 45 / 60 / 93 and
 //   53 / 98 / 181 (3000 positions 41 and 43).
+//   The table's width stands for the cache's length, which only the device knows: in a table of 96 blocks (48 with 16-bit
+//   rows of 256) and more short sequences take that kernel too, and lose: 256 rows over 1024 / 2048 positions take 42 / 34 where
+//   a table as wide as the sequence gives them 19 / 27, 128 over 2048 28 for 23, 64 of each of 12 over 1000 51 for 42. Without the rule
+//   long ones would lose as the figures before say.
 //   Sequences of few rows each leave most of its columns idle (EACH): 32 sequences of 16 rows of 16 heads take 53 and 31,
 //   of 32 heads 54 and 54, 16 of 64 rows of 32 heads 69 and 99; float32 rows 52 and 46, 56 and 82, 74 and 156.
 //   Few rows: past a group for each CU half the waves a block leave a CU two blocks out of step, and two shares a CU
