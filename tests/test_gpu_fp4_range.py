@@ -36,9 +36,12 @@ def large_queries(n, n_q, hd, M, E, sign, dtype):
     return t
 
 
+SOME = [TOPS[i] for i in (0, 3, 6)]  # past 2^18, where a float counts in 4, and in 64
+
+
 @pytest.mark.parametrize("length", [300, 2560])  # 2560: in shares, joined
 @pytest.mark.parametrize("sign", [1, -1])
-@pytest.mark.parametrize("M,E", TOPS)
+@pytest.mark.parametrize("M,E", SOME)
 def test_large_scores(M, E, sign, length):
     """The kernel for few rows: one row, a few, and more than 16 columns a wave."""
     rng = np.random.default_rng(E)
@@ -51,9 +54,9 @@ def test_large_scores(M, E, sign, length):
                 check(P, dtype, large_queries(P.n_rows, n_q, hd, M, E, sign, dtype))
 
 
-@pytest.mark.parametrize("grade,length", [("within", 300), ("within", 2560), ("rising", 2560)])
+@pytest.mark.parametrize("grade,length", [("within", 300), ("rising", 2560)])
 @pytest.mark.parametrize("sign", [1, -1])
-@pytest.mark.parametrize("M,E", TOPS)
+@pytest.mark.parametrize("M,E", SOME)
 def test_large_scores_of_many_columns(M, E, sign, grade, length):
     """The kernel for many rows, its waves of 32 columns and of 16."""
     rng = np.random.default_rng(E)
