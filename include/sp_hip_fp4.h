@@ -47,7 +47,7 @@ void sp_hip_fp4_cache_free(sp_hip_fp4_cache_t *c);
  * even. NaN is stored as 0, magnitudes past 6 * 2^40 (infinity among them) as that. A position
  * whose K is written has attention weight 0. Only the rows' own positions are written, but
  * that a block whose first position is written starts anew: behind its rows it then counts as
- * empty. A call must not reach the same position twice. */
+ * empty. A call must not reach the same position twice, nor from two places a block that it starts anew. */
 int  sp_hip_fp4_write(sp_hip_fp4_cache_t *c, int layer, const sp_hip_fp4_batch_t *batch, const void *d_k,
                       const void *d_v, long long row_stride, int dtype, void *stream);
 /* The batch's rows read back: code * scale, rounded to dtype. */
