@@ -51,6 +51,7 @@ struct SpFp4Weigh {
     int H, G;
     int window;
     float c;  // |kq_scale| * log2(e) / 2
+    float lost;  // of an lse: what c and log2(e) lose in 32 bits, in powers of two (see weigh)
     int negate;
     int cus;
     int blocks;  // log2 of the blocks that a block of threads takes at a time

@@ -33,7 +33,7 @@ __device__ __forceinline__ float power(unsigned rel, int b) {
 // split in two fp16 parts, as in attention.
 //
 // Bound for many columns by the matrix cores and the exponentials (for 64 positions of 16 columns 16 and 16
-// instructions of 16 and 8 cycles at head_dim 128, beside one multiplication and one addition a weight): 64 rows over 32768
+// instructions of 16 and 8 cycles at head_dim 128, beside two multiply-adds a weight): 64 rows over 32768
 // positions, 32 / 8 heads, bf16, 26 us, 0.67 PFLOP/s. For few by latencies: one row of 12 sequences of 1 to 4.5K
 // 10.5 us (21 MB of K), of which an empty launch is 4.
 constexpr int WN = 512;  // threads
@@ -325,8 +325,14 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
                     lse = col.lse;
                     cs = units(col.qe);
                 }
-                // (log2 e and lse are multiplied first: what that rounds off is less than lse's own last bit)
-                lse *= 1.44269504088896341f;
+                // In powers of two a weight's exponent is s cs - lse log2 e, both products near lse where weights count, and the
+                // difference is rounded once. What the second one's rounding, log2 e's and that of kq_scale log2 e lose of a
+                // weight near 1 is a factor of the column's (of a smaller one it is that but for 2^-25 of its exponent).
+                // Without it weights near lse 60 are off by up to 2^-18. (Past 2^20 a score has lost more itself.)
+                const float of_lse = lse * 1.44269504088896341f, low = __builtin_fmaf(lse, 1.44269504088896341f, -of_lse);
+                const float more = __builtin_fmaf(lse, A.lost, -low);
+                const float factor = __builtin_amdgcn_exp2f(fabsf(of_lse) < 0x1p20f ? more : 0.0f);
+                lse = of_lse;
 #pragma unroll
                 for (int n = 0; n < 4; n++)
 #pragma unroll
@@ -343,7 +349,7 @@ __global__ __launch_bounds__(WN, HD == 256 || (!DIRECT && (HD == 128 || (HD == 9
 #pragma unroll
                 for (int n = 0; n < 4; n++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[n][i] += __builtin_amdgcn_exp2f(s[n][i]);
+                    for (int i = 0; i < 4; i++) acc[n][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(s[n][i]), factor, acc[n][i]);
             }
         }
         // ---- over the columns' lanes: lane r of a row keeps value i = r / 4 of row block n = r % 4 ----

@@ -141,7 +141,9 @@ extern "C" int sp_hip_fp4_weigh(sp_hip_fp4_cache_t *c, int layer, const sp_hip_f
     A.H = c->config.n_heads_kv;
     A.G = n_q / A.H;
     A.window = window >= MAX_ROWS ? 0 : window;  // no position is that far
-    A.c = fabsf(kq_scale) * 0.72134752044448170f;
+    const double log2e = 1.4426950408889634074, unit = fabs((double)kq_scale) * (log2e / 2);
+    A.c = (float)unit;
+    A.lost = (float)((A.c >= 0x1p-126f ? unit / A.c - 1.0 : 0.0) * log2e - (log2e - (float)log2e));
     A.negate = kq_scale < 0.0f;
     A.cus = pv->cus;
     return ok(sp_fp4_launch_weigh(A, c->config.head_dim, dtype, s), who) ? 0 : -1;

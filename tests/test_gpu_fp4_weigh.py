@@ -212,3 +212,40 @@ def test_weigh_of_rows_at_any_address(hd):
         P.weigh("f32", q, 0.1, lse, pad=pad, shift=shift)
         got.append(P.weights())
     assert all(np.array_equal(x, got[0]) for x in got[1:])
+
+
+# ---- how exact a weight is ----
+
+@pytest.mark.parametrize("dtype,pad", [("f32", 0), ("f16", 0), ("bf16", 0), ("bf16", 3)])
+@pytest.mark.parametrize("scale", [0.125, 0.1, -0.3, 0.7071])
+def test_weigh_to_the_last_bits(scale, dtype, pad):
+    """Scores near 60 that are whole numbers times kq_scale, exact in fp32: what is left is the exponential of the
+    difference to lse. In powers of two that difference e is rounded once, 2^-24 |e|, and kq_scale log2 e's own rounding counts
+    on it alone, 2^-24 |e| more; the exponential and the factor that takes up what kq_scale, lse and log2 e lose in 32 bits are
+    within 2^-22 each, their product and the sum 2^-23."""
+    rng = np.random.default_rng(int(abs(scale) * 1000))
+    P = Pair(64, 2, 24)
+    lens = [130, 64, 200, 77, 150, 99]
+    table = tables(rng, lens, 24)
+    top = round(60 / abs(scale))
+    k = np.zeros((sum(lens), 2, 64))
+    k[..., 0] = 6.0 if scale > 0 else -6.0
+    k[..., 32:40] = rng.integers(0, 2, k[..., 32:40].shape)
+    P.batch(table, lens, np.concatenate([[0], np.cumsum(lens)]).tolist())
+    P.write("f32", torch.from_numpy(k).float(), torch.from_numpy(k).float())
+    P.batch(table, lens)
+    q = np.zeros((len(lens), 2, 64))
+    q[..., 0] = (top + rng.integers(-8, 9, q.shape[:2])) // 6
+    q[..., 32:40] = rng.integers(-2, 3, q[..., 32:40].shape)
+    q = torch.from_numpy(q).to(TORCH[dtype])
+    _, lse = P.attend(dtype, q, scale)
+    assert (np.abs(lse) > 45).all()
+    P.weigh(dtype, q, scale, lse, pad=pad)
+    got, s = P.weights()[0], float(np.float32(scale))
+    for i, n in enumerate(lens):
+        for h in range(2):
+            K = np.concatenate([P.ref.stored(0, 0, b)[h] for b in table[i]])[:n]
+            w = np.exp(K @ q[i, h].double().numpy() * s - lse[i, h])
+            have = np.concatenate([got[b, h] for b in table[i]])[:n]
+            off = np.abs(np.log2(w)) * 2.0 ** -23 * math.log(2) + 2 * 2.0 ** -22 + 2.0 ** -23
+            assert (np.abs(have - w) <= off * w).all(), float((np.abs(have / w - 1) / off).max())
