@@ -34,8 +34,8 @@ __device__ __forceinline__ float power(unsigned rel, int b) {
 //
 // Bound for many columns by the matrix cores and the exponentials (for 64 positions of 16 columns 16 and 16
 // instructions of 16 and 8 cycles at head_dim 128, beside two multiply-adds a weight): 64 rows over 32768
-// positions, 32 / 8 heads, bf16, 26 us, 0.67 PFLOP/s. For few by latencies: one row of 12 sequences of 1 to 4.5K
-// 10.5 us (21 MB of K), of which an empty launch is 4.
+// positions, 32 / 8 heads, bf16, 26.5 us, 0.65 PFLOP/s. For few by latencies: one row of 12 sequences of 1 to 4.5K
+// 10.8 us (21 MB of K), of which an empty launch is 4.
 constexpr int WN = 512;  // threads
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
